@@ -12,6 +12,7 @@
 
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -34,7 +35,8 @@ PyObject *g_error = nullptr;   // native.CaifqError
   X(linear_fwd) X(linear_fwd_residual) X(linear_fwd_multi) X(linear_dx) X(linear_workspace_bytes) X(linear_fwd_ws) X(linear_dx_ws) X(linear_concat_workspace_bytes)              \
   X(linear_fwd_concat) X(linear_dx_concat) X(lora_fwd_workspace_bytes) X(lora_fwd_workspace_bytes_expanded)           \
   X(lora_bwd_workspace_bytes) X(lora_bwd_workspace_bytes_expanded) X(lora_linear_fwd) X(lora_linear_fwd_expanded)     \
-  X(lora_linear_bwd) X(lora_linear_bwd_expanded) X(rmsnorm_fwd) X(rmsnorm_bwd) X(cast) X(quantize_int8_per_tensor)    \
+  X(lora_linear_bwd) X(lora_linear_bwd_expanded) X(rmsnorm_fwd) X(rmsnorm_bwd) X(layernorm_fwd)                     \
+  X(layernorm_bwd) X(layernorm_bwd_workspace_bytes) X(cast) X(quantize_int8_per_tensor)    \
   X(quantize_int8_per_channel) X(quantize_int4_per_group) X(moe_topk) X(moe_normalize_rows) X(moe_router_softmax)     \
   X(moe_build_dispatch) X(moe_dispatch) X(moe_combine) X(moe_combine_bwd_grad_expert)                                 \
   X(moe_combine_bwd_grad_weights) X(moe_dispatch_bwd) X(moe_router_bwd) X(grouped_expert_expand)                      \
@@ -305,6 +307,56 @@ void need_matrix(const at::Tensor &t, const char *who)
                  static_cast<long long>(t.dim()));
     throw Raised{};
   }
+}
+
+// The device of a call's tensors made the current one, and their stream: a program may hold tensors of another device
+class OnDevice
+{
+public:
+  OnDevice(const at::Tensor &first, const char *who) : guard_(first.device()), device_(first.device()), who_(who) {}
+
+  // a further operand: on the same device, of one type and size (-1: any)
+  void same(const at::Tensor *t, const char *name, at::ScalarType dtype, int64_t numel) const
+  {
+    if (t == nullptr)
+    {
+      return;
+    }
+    if (t->device() != device_)
+    {
+      PyErr_Format(g_error, "%s: %s is on another device", who_, name);
+      throw Raised{};
+    }
+    if (t->scalar_type() != dtype)
+    {
+      PyErr_Format(g_error, "%s: %s must be %s, not %s", who_, name, c10::toString(dtype), c10::toString(t->scalar_type()));
+      throw Raised{};
+    }
+    if (numel >= 0 && t->numel() != numel)
+    {
+      PyErr_Format(g_error, "%s: %s has %lld elements, %lld expected", who_, name, static_cast<long long>(t->numel()),
+                   static_cast<long long>(numel));
+      throw Raised{};
+    }
+  }
+
+  void *stream() const { return c10::cuda::getCurrentCUDAStream(device_.index()).stream(); }
+
+private:
+  c10::cuda::CUDAGuard guard_;
+  c10::Device device_;
+  const char *who_;
+};
+
+// a size that the C ABI takes in 32 bits
+int32_t int32_of(int64_t v, const char *who, const char *name)
+{
+  if (v > INT32_MAX)
+  {
+    PyErr_Format(g_error, "%s: %s of %lld is more than 32 bits hold", who, name, static_cast<long long>(v));
+    throw Raised{};
+  }
+  return static_cast<int32_t>(v);
 }
 
 // numel // width as Python has it: a width of zero is an exception there, and the end of the process in C
@@ -585,6 +637,85 @@ PyObject *rmsnorm_bwd(Args &a)
         }),
         "rmsnorm_bwd");
   return pack({wrap(std::move(dx)), wrap(std::move(dg))});
+}
+
+// rows of the last dimension: a tensor without one has none to normalise
+int64_t last_dim(const at::Tensor &x, const char *who)
+{
+  if (x.dim() == 0)
+  {
+    PyErr_Format(g_error, "%s: rows expected, got a tensor without dimensions", who);
+    throw Raised{};
+  }
+  return x.size(-1);
+}
+
+// (x, gamma | None, beta | None, epsilon) -> (y, mean, rstd)
+PyObject *layernorm_fwd(Args &a)
+{
+  const char *who = "layernorm_fwd";
+  const at::Tensor &x = *a.tensor();
+  const at::Tensor *gamma = a.tensor(true);
+  const at::Tensor *beta = a.tensor(true);
+  const float eps = static_cast<float>(a.real());
+  const int64_t dim = int32_of(last_dim(x, who), who, "rows");
+  const int32_t rows = int32_of(rows_of(x, dim), who, "a number of rows");
+  const OnDevice on(x, who);
+  on.same(gamma, "gamma", at::kFloat, dim);
+  on.same(beta, "beta", at::kFloat, dim);
+  const int xc = code_of(x);
+  at::Tensor y = empty_like(x);
+  at::Tensor mean = empty({rows}, at::kFloat, x);
+  at::Tensor rstd = empty({rows}, at::kFloat, x);
+  void *s = on.stream();
+  check(unlocked([&] {
+          return api.layernorm_fwd(ptr(x), static_cast<const float *>(ptr(gamma)), static_cast<const float *>(ptr(beta)),
+                                   ptr(y), static_cast<float *>(ptr(mean)), static_cast<float *>(ptr(rstd)), eps, xc, rows,
+                                   static_cast<int32_t>(dim), s);
+        }),
+        who);
+  return pack({wrap(std::move(y)), wrap(std::move(mean)), wrap(std::move(rstd))});
+}
+
+// (dy, x, mean, rstd, gamma | None, grad_gamma | None, grad_beta | None) -> (dx, grad_gamma, grad_beta)
+PyObject *layernorm_bwd(Args &a)
+{
+  const char *who = "layernorm_bwd";
+  const at::Tensor &dy = *a.tensor();
+  const at::Tensor &x = *a.tensor();
+  const at::Tensor *mean = a.tensor();
+  const at::Tensor *rstd = a.tensor();
+  const at::Tensor *gamma = a.tensor(true);
+  const at::Tensor *given_gamma = a.tensor(true);
+  const at::Tensor *given_beta = a.tensor(true);
+  const int64_t dim = int32_of(last_dim(x, who), who, "rows");
+  const int32_t rows = int32_of(rows_of(x, dim), who, "a number of rows");
+  if ((given_gamma == nullptr) != (given_beta == nullptr))
+  {
+    raise(g_error, "layernorm_bwd: give both grad_gamma and grad_beta, or neither");
+  }
+  const OnDevice on(x, who);
+  on.same(&dy, "dy", x.scalar_type(), x.numel());
+  on.same(mean, "mean", at::kFloat, rows);
+  on.same(rstd, "rstd", at::kFloat, rows);
+  on.same(gamma, "gamma", at::kFloat, dim);
+  on.same(given_gamma, "grad_gamma", at::kFloat, dim);
+  on.same(given_beta, "grad_beta", at::kFloat, dim);
+  const int xc = code_of(x);
+  at::Tensor dx = empty_like(x);
+  at::Tensor dg = given_gamma != nullptr ? *given_gamma : empty({dim}, at::kFloat, x);
+  at::Tensor db = given_beta != nullptr ? *given_beta : empty({dim}, at::kFloat, x);
+  at::Tensor work =
+      empty({static_cast<int64_t>(api.layernorm_bwd_workspace_bytes(rows, static_cast<int32_t>(dim)))}, at::kByte, x);
+  void *s = on.stream();
+  check(unlocked([&] {
+          return api.layernorm_bwd(ptr(dy), ptr(x), static_cast<const float *>(ptr(gamma)),
+                                   static_cast<const float *>(ptr(mean)), static_cast<const float *>(ptr(rstd)), ptr(dx),
+                                   static_cast<float *>(ptr(dg)), static_cast<float *>(ptr(db)),
+                                   given_gamma != nullptr ? 1 : 0, ptr(work), xc, rows, static_cast<int32_t>(dim), s);
+        }),
+        who);
+  return pack({wrap(std::move(dx)), wrap(std::move(dg)), wrap(std::move(db))});
 }
 
 PyObject *cast(Args &a)
@@ -1017,6 +1148,8 @@ PyMethodDef methods[] = {
     CAIFQ_METHOD(lora_linear_bwd),
     CAIFQ_METHOD(rmsnorm_fwd),
     CAIFQ_METHOD(rmsnorm_bwd),
+    CAIFQ_METHOD(layernorm_fwd),
+    CAIFQ_METHOD(layernorm_bwd),
     CAIFQ_METHOD(cast),
     CAIFQ_METHOD(quantize_int8_per_tensor),
     CAIFQ_METHOD(quantize_int8_per_channel),

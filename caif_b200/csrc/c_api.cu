@@ -129,6 +129,13 @@ int launch_rmsnorm_fwd(const void *input, const float *gamma, void *output, floa
                        int rows, int dim, cudaStream_t s);
 int launch_rmsnorm_bwd(const void *grad_output, const void *input, const float *gamma, const float *rms_cache,
                        void *grad_input, float *grad_gamma, int dtype, int rows, int dim, cudaStream_t s);
+// layernorm.cu
+size_t layernorm_bwd_workspace_bytes(int rows, int dim);
+int launch_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
+                         float epsilon, int dtype, int rows, int dim, cudaStream_t s);
+int launch_layernorm_bwd(const void *dy, const void *x, const float *gamma, const float *mean, const float *rstd, void *dx,
+                         float *grad_gamma, float *grad_beta, int accumulate, float *workspace, int dtype, int rows, int dim,
+                         cudaStream_t s);
 int launch_moe_router_bwd(const void *grad_w, const void *probs, const int *indices, const void *balance_bias,
                           const void *z_lse_scaled, void *grad_topk, void *grad_logits, int dtype, int tokens,
                           int experts, int top_k, int sigmoid_gate, int normalize, float scaling, int exact_jacobian,
@@ -1245,6 +1252,36 @@ int caifq_rmsnorm_bwd(const void *dy, const void *x, const float *gamma, const f
   CAIFQ_CHECK_ARG(rows == 0 || (dy && x && gamma && rms_cache && dx), "%s: null pointer", who);
   return launch_rmsnorm_bwd(dy, x, gamma, rms_cache, dx, grad_gamma, dtype, rows, dim,
                             static_cast<cudaStream_t>(stream));
+}
+
+int caifq_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
+                        float epsilon, int32_t dtype, int32_t rows, int32_t dim, void *stream)
+{
+  const char *who = "caifq_layernorm_fwd";
+  CAIFQ_CHECK_ARG(rows >= 0 && dim > 0, "%s: bad shape rows=%d dim=%d", who, rows, dim);
+  CAIFQ_CHECK_ARG(is_float_dtype(dtype), "%s: dtype must be F32, F16 or BF16", who);
+  CAIFQ_CHECK_ARG(rows == 0 || (x && y && mean && rstd), "%s: null pointer", who);
+  return launch_layernorm_fwd(x, gamma, beta, y, mean, rstd, epsilon, dtype, rows, dim, static_cast<cudaStream_t>(stream));
+}
+
+size_t caifq_layernorm_bwd_workspace_bytes(int32_t rows, int32_t dim)
+{
+  return rows > 0 && dim > 0 ? layernorm_bwd_workspace_bytes(rows, dim) : 0;
+}
+
+int caifq_layernorm_bwd(const void *dy, const void *x, const float *gamma, const float *mean, const float *rstd, void *dx,
+                        float *grad_gamma, float *grad_beta, int32_t accumulate, void *workspace, int32_t dtype,
+                        int32_t rows, int32_t dim, void *stream)
+{
+  const char *who = "caifq_layernorm_bwd";
+  CAIFQ_CHECK_ARG(rows >= 0 && dim > 0, "%s: bad shape rows=%d dim=%d", who, rows, dim);
+  CAIFQ_CHECK_ARG(is_float_dtype(dtype), "%s: dtype must be F32, F16 or BF16", who);
+  CAIFQ_CHECK_ARG(rows == 0 || (dy && x && mean && rstd && dx), "%s: null pointer", who);
+  CAIFQ_CHECK_ARG(rows == 0 || (grad_gamma == nullptr && grad_beta == nullptr) ||
+                      (workspace != nullptr && aligned_to(workspace, 16)),
+                  "%s: the gradients of gamma and beta need a workspace, 16-byte aligned", who);
+  return launch_layernorm_bwd(dy, x, gamma, mean, rstd, dx, grad_gamma, grad_beta, accumulate != 0 ? 1 : 0,
+                              static_cast<float *>(workspace), dtype, rows, dim, static_cast<cudaStream_t>(stream));
 }
 
 int caifq_moe_bias_update(void *bias, const int32_t *counts, int32_t from_offsets, int32_t dtype, int32_t experts,

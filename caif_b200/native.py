@@ -99,6 +99,9 @@ _SIGNATURES = {
                                             ctypes.c_float, _i32, _vp]),
     "caifq_rmsnorm_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_float, _i32, _i32, _i32, _vp]),
     "caifq_rmsnorm_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "caifq_layernorm_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _i32, _i32, _i32, _vp]),
+    "caifq_layernorm_bwd_workspace_bytes": (ctypes.c_size_t, [_i32, _i32]),
+    "caifq_layernorm_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
     "caifq_moe_bias_update": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, ctypes.c_float, _vp]),
     "caifq_moe_aux_losses": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, ctypes.c_float,
                                             ctypes.c_float, _vp]),
@@ -473,6 +476,18 @@ def rmsnorm_fwd(x, gamma, epsilon=1e-5):
 def rmsnorm_bwd(dy, x, gamma, rms_cache, grad_gamma=None):
     """Returns (dx, grad_gamma); grad_gamma is accumulated onto the tensor given (zeros when None)."""
     return (_native or _binding()).rmsnorm_bwd(dy, x, gamma, rms_cache, grad_gamma)
+
+
+def layernorm_fwd(x, gamma=None, beta=None, epsilon=1e-5):
+    """Layer norm over the last dimension; gamma and beta are fp32 (None: ones, zeros).  Returns (y, mean, rstd), the last
+    two fp32 with one value a row, for layernorm_bwd."""
+    return (_native or _binding()).layernorm_fwd(x, gamma, beta, epsilon)
+
+
+def layernorm_bwd(dy, x, mean, rstd, gamma=None, grad_gamma=None, grad_beta=None):
+    """Returns (dx, grad_gamma, grad_beta); the last two are accumulated onto the tensors given (both or neither).  Equal
+    calls give equal bits."""
+    return (_native or _binding()).layernorm_bwd(dy, x, mean, rstd, gamma, grad_gamma, grad_beta)
 
 
 def moe_softmax(logits, bias=None):

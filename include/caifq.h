@@ -392,6 +392,26 @@ CAIFQ_API int caifq_rmsnorm_fwd(const void *x, const float *gamma, void *y, floa
 CAIFQ_API int caifq_rmsnorm_bwd(const void *dy, const void *x, const float *gamma, const float *rms_cache, void *dx,
                                 float *grad_gamma, int32_t dtype, int32_t rows, int32_t dim, void *stream);
 
+/*
+ * Layer norm for the same place in a block (no counterpart among the kernels this library replaces):
+ *   fwd: mean[r] = sum_c x[r,c] / dim, rstd[r] = 1 / sqrt(sum_c (x[r,c] - mean[r])^2 / dim + epsilon),
+ *        y[r,c] = T((x[r,c] - mean[r]) * rstd[r] * gamma[c] + beta[c]);  mean, rstd: fp32 [rows]
+ *   bwd: x_hat = (x - mean) * rstd, g = dy * gamma,
+ *        dx[r,c] = T(rstd * (g - mean_c(g) - x_hat * mean_c(g * x_hat)));
+ *        grad_gamma[c] = sum_r dy * x_hat, grad_beta[c] = sum_r dy (fp32 [dim]; each may be NULL), added onto what is there
+ *        when accumulate != 0, overwritten when it is 0 (with rows == 0: by zeros)
+ * x, y, dy, dx in `dtype` (F32, F16, BF16), contiguous rows of any length; gamma, beta fp32 [dim] or NULL (ones, zeros).
+ * Sums are fp32 in a fixed order: equal calls give equal bits.  In place (y == x, dx == dy, dx == x) is allowed.  The backward
+ * call's workspace holds caifq_layernorm_bwd_workspace_bytes(rows, dim) bytes, 16-byte aligned, scratch of the call alone; it may be
+ * NULL where neither gradient is asked for.  Calls that may overlap on the GPU need workspaces of their own.
+ */
+CAIFQ_API int caifq_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
+                                  float epsilon, int32_t dtype, int32_t rows, int32_t dim, void *stream);
+CAIFQ_API size_t caifq_layernorm_bwd_workspace_bytes(int32_t rows, int32_t dim);
+CAIFQ_API int caifq_layernorm_bwd(const void *dy, const void *x, const float *gamma, const float *mean, const float *rstd,
+                                  void *dx, float *grad_gamma, float *grad_beta, int32_t accumulate, void *workspace,
+                                  int32_t dtype, int32_t rows, int32_t dim, void *stream);
+
 /* ---- MoE routing and dispatch -------------------------------------------- */
 
 /* launch_topk, src/caif_cuda_kernels_moe.cu:280-345: descending values, ties to
