@@ -36,7 +36,8 @@ PyObject *g_error = nullptr;   // native.CaifqError
   X(linear_fwd_concat) X(linear_dx_concat) X(lora_fwd_workspace_bytes) X(lora_fwd_workspace_bytes_expanded)           \
   X(lora_bwd_workspace_bytes) X(lora_bwd_workspace_bytes_expanded) X(lora_linear_fwd) X(lora_linear_fwd_expanded)     \
   X(lora_linear_bwd) X(lora_linear_bwd_expanded) X(rmsnorm_fwd) X(rmsnorm_bwd) X(layernorm_fwd)                     \
-  X(layernorm_bwd) X(layernorm_bwd_workspace_bytes) X(cast) X(quantize_int8_per_tensor)    \
+  X(layernorm_bwd) X(layernorm_bwd_workspace_bytes) X(act_pack) X(act_unpack) X(lora_linear_bwd_packed)               \
+  X(lora_bwd_packed_workspace_bytes) X(lora_bank_workspace_bytes) X(lora_bank_linear_fwd) X(cast) X(quantize_int8_per_tensor)    \
   X(quantize_int8_per_channel) X(quantize_int4_per_group) X(moe_topk) X(moe_normalize_rows) X(moe_router_softmax)     \
   X(moe_build_dispatch) X(moe_dispatch) X(moe_combine) X(moe_combine_bwd_grad_expert)                                 \
   X(moe_combine_bwd_grad_weights) X(moe_dispatch_bwd) X(moe_router_bwd) X(grouped_expert_expand)                      \
@@ -596,6 +597,168 @@ PyObject *lora_linear_bwd(Args &a)
   return pack({wrap(std::move(dx)), wrap(std::move(da)), wrap(std::move(db))});
 }
 
+// a tensor of a result's or scratch's size that the caller gave
+void need_contiguous(const at::Tensor *t, const char *who, const char *name)
+{
+  if (t != nullptr && !t->is_contiguous())
+  {
+    PyErr_Format(g_error, "%s: %s must be contiguous", who, name);
+    throw Raised{};
+  }
+}
+
+// scratch of a call, given or taken: given scratch is contiguous, on the call's device and large enough
+at::Tensor workspace_on(const at::Tensor *given, size_t need, const at::Tensor &like, const OnDevice &on, const char *who)
+{
+  if (given != nullptr)
+  {
+    on.same(given, "workspace", at::kByte, -1);
+    need_contiguous(given, who, "workspace");
+  }
+  return workspace_of(given, need, like, who);
+}
+
+// (weight, bank, adapter_of_row, x, compute, out | None, workspace | None) -> y
+PyObject *lora_bank_linear_fwd(Args &a)
+{
+  const char *who = "lora_bank_linear_fwd";
+  const caifq_weight *w = a.record<caifq_weight>();
+  const caifq_lora_bank *bank = a.record<caifq_lora_bank>();
+  const at::Tensor &rows = *a.tensor();
+  const at::Tensor &x = *a.tensor();
+  const int compute = static_cast<int>(a.integer());
+  const at::Tensor *out = a.tensor(true);
+  const at::Tensor *given = a.buffer();
+  if (x.dim() == 0 || x.size(-1) != w->in_dim)
+  {
+    raise(g_error, "lora_bank_linear_fwd: the last dimension of x must be the weight's in_dim");
+  }
+  const int64_t m = rows_of(x, w->in_dim);
+  const OnDevice on(x, who);
+  on.same(&rows, "adapter_of_row", at::kInt, m);
+  const std::vector<int64_t> shape = shape_with_last(x, w->out_dim);
+  on.same(out, "out", x.scalar_type(), m * w->out_dim);
+  if (code_of(x) != bank->dtype)
+  {
+    raise(g_error, "lora_bank_linear_fwd: x must have the adapters' dtype");
+  }
+  at::Tensor y = out != nullptr ? *out : empty(shape, x.scalar_type(), x);
+  at::Tensor work = workspace_on(given, api.lora_bank_workspace_bytes(w, bank, m, compute), x, on, who);
+  void *s = on.stream();
+  check(unlocked([&] {
+          return api.lora_bank_linear_fwd(w, bank, static_cast<const int32_t *>(ptr(rows)), ptr(x), m, ptr(y), ptr(work),
+                                          static_cast<size_t>(work.numel()), compute, s);
+        }),
+        who);
+  return wrap(std::move(y));
+}
+
+// (x) -> (codes, scales)
+PyObject *act_pack(Args &a)
+{
+  const char *who = "act_pack";
+  const at::Tensor &x = *a.tensor();
+  if (x.dim() == 0)
+  {
+    raise(g_error, "act_pack: rows expected, got a tensor without dimensions");
+  }
+  const int32_t dim = int32_of(x.size(-1), who, "rows");
+  const int64_t rows = rows_of(x, dim);
+  const OnDevice on(x, who);
+  const int xc = code_of(x);
+  at::Tensor codes = empty(x.sizes(), at::kChar, x);
+  at::Tensor scales = empty(shape_with_last(x, (static_cast<int64_t>(dim) + 31) / 32), at::kByte, x);
+  void *s = on.stream();
+  check(unlocked([&] {
+          return api.act_pack(ptr(x), xc, static_cast<int8_t *>(ptr(codes)), static_cast<uint8_t *>(ptr(scales)), rows, dim, s);
+        }),
+        who);
+  return pack({wrap(std::move(codes)), wrap(std::move(scales))});
+}
+
+// codes and scales that belong together; the row length
+int32_t check_packed(const at::Tensor &codes, const at::Tensor &scales, const OnDevice &on, const char *who)
+{
+  if (codes.dim() == 0 || codes.size(-1) == 0)
+  {
+    PyErr_Format(g_error, "%s: rows of codes expected", who);
+    throw Raised{};
+  }
+  const int32_t dim = int32_of(codes.size(-1), who, "rows");
+  on.same(&codes, "codes", at::kChar, -1);
+  on.same(&scales, "scales", at::kByte, codes.numel() / dim * ((static_cast<int64_t>(dim) + 31) / 32));
+  return dim;
+}
+
+// (codes, scales, dtype) -> x
+PyObject *act_unpack(Args &a)
+{
+  const char *who = "act_unpack";
+  const at::Tensor &codes = *a.tensor();
+  const at::Tensor &scales = *a.tensor();
+  const at::ScalarType dtype = a.dtype();
+  const OnDevice on(codes, who);
+  const int32_t dim = check_packed(codes, scales, on, who);
+  at::Tensor x = empty(codes.sizes(), dtype, codes);
+  const int xc = code_of(x);
+  void *s = on.stream();
+  check(unlocked([&] {
+          return api.act_unpack(static_cast<const int8_t *>(ptr(codes)), static_cast<const uint8_t *>(ptr(scales)), ptr(x), xc,
+                                codes.numel() / dim, dim, s);
+        }),
+        who);
+  return wrap(std::move(x));
+}
+
+// (weight, lora, A, B, dy, codes, scales, hidden, compute, dx | None, dA | None, dB | None, workspace | None)
+PyObject *lora_linear_bwd_packed(Args &a)
+{
+  const char *who = "lora_linear_bwd_packed";
+  const caifq_weight *w = a.record<caifq_weight>();
+  const caifq_lora *l = a.record<caifq_lora>();
+  const at::Tensor &la = *a.tensor();
+  const at::Tensor &lb = *a.tensor();
+  const at::Tensor &dy = *a.tensor();
+  const at::Tensor &codes = *a.tensor();
+  const at::Tensor &scales = *a.tensor();
+  const at::Tensor &hidden = *a.tensor();
+  const int compute = static_cast<int>(a.integer());
+  const at::Tensor *dx_given = a.tensor(true);
+  const at::Tensor *da_given = a.tensor(true);
+  const at::Tensor *db_given = a.tensor(true);
+  const at::Tensor *given = a.buffer();
+  const int64_t m = rows_of(dy, w->out_dim);
+  if (dy.dim() == 0 || dy.size(-1) != w->out_dim)
+  {
+    raise(g_error, "lora_linear_bwd_packed: the last dimension of dy must be the weight's out_dim");
+  }
+  const OnDevice on(dy, who);
+  const at::ScalarType t = dy.scalar_type();
+  const int64_t r = l->rank;
+  on.same(&la, "A", t, r * w->in_dim);
+  on.same(&lb, "B", t, r * w->out_dim);
+  on.same(&hidden, "hidden", t, m * r);
+  on.same(dx_given, "dx", t, m * w->in_dim);
+  on.same(da_given, "d_a", t, r * w->in_dim);
+  on.same(db_given, "d_b", t, r * w->out_dim);
+  if (codes.numel() != m * w->in_dim || (m > 0 && check_packed(codes, scales, on, who) != w->in_dim))
+  {
+    raise(g_error, "lora_linear_bwd_packed: the packed rows must be those of x, one for each of dy's, in_dim wide");
+  }
+  at::Tensor dx = dx_given != nullptr ? *dx_given : empty(shape_with_last(dy, w->in_dim), t, dy);
+  at::Tensor da = da_given != nullptr ? *da_given : empty_like(la);
+  at::Tensor db = db_given != nullptr ? *db_given : empty_like(lb);
+  at::Tensor work = workspace_on(given, api.lora_bwd_packed_workspace_bytes(w, l, m, compute), dy, on, who);
+  void *s = on.stream();
+  check(unlocked([&] {
+          return api.lora_linear_bwd_packed(w, l, ptr(dy), static_cast<const int8_t *>(ptr(codes)),
+                                            static_cast<const uint8_t *>(ptr(scales)), ptr(hidden), m, ptr(dx), ptr(da),
+                                            ptr(db), ptr(work), static_cast<size_t>(work.numel()), compute, s);
+        }),
+        who);
+  return pack({wrap(std::move(dx)), wrap(std::move(da)), wrap(std::move(db))});
+}
+
 // ---- norm, casts, quantizers --------------------------------------------------------------------------------
 
 PyObject *rmsnorm_fwd(Args &a)
@@ -1148,6 +1311,10 @@ PyMethodDef methods[] = {
     CAIFQ_METHOD(lora_linear_bwd),
     CAIFQ_METHOD(rmsnorm_fwd),
     CAIFQ_METHOD(rmsnorm_bwd),
+    CAIFQ_METHOD(lora_bank_linear_fwd),
+    CAIFQ_METHOD(lora_linear_bwd_packed),
+    CAIFQ_METHOD(act_pack),
+    CAIFQ_METHOD(act_unpack),
     CAIFQ_METHOD(layernorm_fwd),
     CAIFQ_METHOD(layernorm_bwd),
     CAIFQ_METHOD(cast),

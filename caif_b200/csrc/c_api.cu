@@ -129,6 +129,15 @@ int launch_rmsnorm_fwd(const void *input, const float *gamma, void *output, floa
                        int rows, int dim, cudaStream_t s);
 int launch_rmsnorm_bwd(const void *grad_output, const void *input, const float *gamma, const float *rms_cache,
                        void *grad_input, float *grad_gamma, int dtype, int rows, int dim, cudaStream_t s);
+// lora_bank.cu
+int launch_lora_bank(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
+                     cudaStream_t s);
+// act8.cu
+int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
+int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
+size_t act_tn_scratch_bytes(int64_t m, int p, int q);
+int launch_act_tn(const void *u, int u_dtype, const void *v, int v_dtype, const uint8_t *v_scales, void *out, int out_dtype,
+                  float factor, float *scratch, int64_t m, int p, int q, cudaStream_t s);
 // layernorm.cu
 size_t layernorm_bwd_workspace_bytes(int rows, int dim);
 int launch_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
@@ -1072,6 +1081,271 @@ int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_lora *lora,
   // (fused path: dB's by the launch that prepares the factors, dA's, in the same place, by a memset after dB has been
   // rounded; general path: a memset each), and dH is fully overwritten before it is read.
   return caifq_lora_linear_bwd(w, lora, dy, x, hidden, m, dx, d_a, d_b, scratch, compute_dtype, stream);
+}
+
+// ------------------------------------------------ adapters of many requests
+
+namespace
+{
+bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes)
+{
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a);
+  const uintptr_t y = reinterpret_cast<uintptr_t>(b);
+  return x < y + b_bytes && y < x + a_bytes;
+}
+
+int check_bank(const caifq_weight *w, const caifq_lora_bank *bank, const char *who)
+{
+  const int rc = check_weight(w, who);
+  if (rc != CAIFQ_OK)
+  {
+    return rc;
+  }
+  CAIFQ_CHECK_ARG(bank != nullptr && bank->entries != nullptr && bank->count > 0, "%s: the bank is empty", who);
+  CAIFQ_CHECK_ARG(is_float_dtype(bank->dtype), "%s: the bank's dtype must be F32, F16 or BF16", who);
+  CAIFQ_CHECK_ARG(bank->max_rank >= 1 && bank->max_rank <= kBankMaxRank, "%s: ranks from 1 to %d, not %d", who, kBankMaxRank,
+                  bank->max_rank);
+  CAIFQ_CHECK_ARG(bank->in_dim == w->in_dim && bank->out_dim == w->out_dim,
+                  "%s: the bank is for %d -> %d features, the weight has %d -> %d", who, bank->in_dim, bank->out_dim,
+                  w->in_dim, w->out_dim);
+  return CAIFQ_OK;
+}
+
+size_t bank_hidden_bytes(const caifq_lora_bank *bank, int64_t m)
+{
+  return align256(static_cast<size_t>(m) * static_cast<size_t>(bank->max_rank) * sizeof(float));
+}
+}  // namespace
+
+int caifq_lora_bank_entries(const caifq_lora *loras, int32_t count, int32_t in_dim, int32_t out_dim,
+                            caifq_lora_entry *entries_host, caifq_lora_bank *bank)
+{
+  const char *who = "caifq_lora_bank_entries";
+  CAIFQ_CHECK_ARG(loras != nullptr && count > 0, "%s: no adapters", who);
+  CAIFQ_CHECK_ARG(entries_host != nullptr && bank != nullptr, "%s: null pointer", who);
+  CAIFQ_CHECK_ARG(in_dim > 0 && out_dim > 0, "%s: bad dims in=%d out=%d", who, in_dim, out_dim);
+  caifq_lora_bank b{};
+  b.count = count;
+  b.dtype = loras[0].dtype;
+  b.in_dim = in_dim;
+  b.out_dim = out_dim;
+  b.vectors = b.dtype == CAIFQ_BF16 ? 1 : 0;
+  CAIFQ_CHECK_ARG(is_float_dtype(b.dtype), "%s: dtype must be F32, F16 or BF16", who);
+  for (int i = 0; i < count; ++i)
+  {
+    const caifq_lora &l = loras[i];
+    CAIFQ_CHECK_ARG(l.a != nullptr && l.b != nullptr, "%s: factors of adapter %d are null", who, i);
+    CAIFQ_CHECK_ARG(l.rank >= 1 && l.rank <= kBankMaxRank, "%s: adapter %d has rank %d, ranks from 1 to %d are taken", who, i,
+                    l.rank, kBankMaxRank);
+    CAIFQ_CHECK_ARG(l.dtype == b.dtype, "%s: adapter %d has dtype %d, adapter 0 has %d", who, i, l.dtype, b.dtype);
+    entries_host[i] = caifq_lora_entry{l.a, l.b, l.rank, l.alpha / static_cast<float>(l.rank)};
+    b.max_rank = l.rank > b.max_rank ? l.rank : b.max_rank;
+    if ((l.rank % 8) != 0 || l.rank > 64 || !aligned_to(l.a, 16) || !aligned_to(l.b, 16))
+    {
+      b.vectors = 0;
+    }
+  }
+  *bank = b;
+  return CAIFQ_OK;
+}
+
+size_t caifq_lora_bank_workspace_bytes(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m, int32_t compute_dtype)
+{
+  if (w == nullptr || bank == nullptr || m <= 0 || w->codes == nullptr || w->in_dim <= 0 || w->out_dim <= 0 ||
+      bank->max_rank <= 0)
+  {
+    return 0;
+  }
+  return bank_hidden_bytes(bank, m) +
+         (expand_linear_ok(w, false, kAlignedProbe, bank->dtype, m, kAlignedProbe, bank->dtype, compute_dtype)
+              ? expanded_weight_bytes(w)
+              : 0);
+}
+
+int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *bank, const int32_t *adapter_of_row,
+                               const void *x, int64_t m, void *y, void *workspace, size_t workspace_bytes,
+                               int32_t compute_dtype, void *stream)
+{
+  const char *who = "caifq_lora_bank_linear_fwd";
+  const int rc = check_bank(w, bank, who);
+  if (rc != CAIFQ_OK)
+  {
+    return rc;
+  }
+  CAIFQ_CHECK_ARG(m >= 0 && m <= 0x7FFFFFFF, "%s: %lld rows", who, static_cast<long long>(m));
+  CAIFQ_CHECK_ARG(is_float_dtype(compute_dtype), "%s: the compute dtype must be F32, F16 or BF16", who);
+  if (m == 0)
+  {
+    return CAIFQ_OK;
+  }
+  CAIFQ_CHECK_ARG(adapter_of_row && x && y, "%s: null pointer", who);
+  const size_t need = caifq_lora_bank_workspace_bytes(w, bank, m, compute_dtype);
+  CAIFQ_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && aligned_to(workspace, 256),
+                  "%s: a workspace of %zu bytes on a 256-byte boundary is needed", who, need);
+  const size_t elem = dtype_bytes(bank->dtype);
+  CAIFQ_CHECK_ARG(!overlap(x, elem * static_cast<size_t>(m) * w->in_dim, y, elem * static_cast<size_t>(m) * w->out_dim),
+                  "%s: x and y overlap", who);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  float *h = static_cast<float *>(workspace);
+  int r = launch_lora_bank(*bank, adapter_of_row, x, m, y, h, s);
+  if (r != CAIFQ_OK)
+  {
+    return r;
+  }
+  if (expand_linear_ok(w, false, x, bank->dtype, m, y, bank->dtype, compute_dtype))
+  {
+    void *wb = static_cast<char *>(workspace) + bank_hidden_bytes(bank, m);
+    r = launch_expand_prepare(*w, wb, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, s);
+    if (r != CAIFQ_OK)
+    {
+      return r;
+    }
+    const caifq_weight wbf = float_weight(wb, CAIFQ_BF16, w->out_dim, w->in_dim);
+    return linear_any(&wbf, false, x, bank->dtype, 1.0f, m, y, bank->dtype, true, compute_dtype, s, who, nullptr, nullptr,
+                      epilogue_scale_ptr(w));
+  }
+  return linear_any(w, false, x, bank->dtype, 1.0f, m, y, bank->dtype, true, compute_dtype, s, who);
+}
+
+// ------------------------------------------------- activations kept in 8 bits
+
+int caifq_act_pack(const void *x, int32_t dtype, int8_t *codes, uint8_t *scales, int64_t rows, int32_t dim, void *stream)
+{
+  const char *who = "caifq_act_pack";
+  CAIFQ_CHECK_ARG(rows >= 0 && dim > 0, "%s: bad shape rows=%lld dim=%d", who, static_cast<long long>(rows), dim);
+  CAIFQ_CHECK_ARG(is_float_dtype(dtype), "%s: dtype must be F32, F16 or BF16", who);
+  CAIFQ_CHECK_ARG(rows == 0 || (x && codes && scales), "%s: null pointer", who);
+  return launch_act_pack(x, dtype, codes, scales, rows, dim, static_cast<cudaStream_t>(stream));
+}
+
+int caifq_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int32_t dtype, int64_t rows, int32_t dim,
+                     void *stream)
+{
+  const char *who = "caifq_act_unpack";
+  CAIFQ_CHECK_ARG(rows >= 0 && dim > 0, "%s: bad shape rows=%lld dim=%d", who, static_cast<long long>(rows), dim);
+  CAIFQ_CHECK_ARG(is_float_dtype(dtype), "%s: dtype must be F32, F16 or BF16", who);
+  CAIFQ_CHECK_ARG(rows == 0 || (x && codes && scales), "%s: null pointer", who);
+  return launch_act_unpack(codes, scales, x, dtype, rows, dim, static_cast<cudaStream_t>(stream));
+}
+
+namespace
+{
+struct PackedBwdWs
+{
+  LoraBwdWs lora;
+  size_t weight;   // the expanded weight, where there is one
+  size_t sums;     // fp32, of one reduction over tokens at a time
+  size_t total;
+};
+
+PackedBwdWs packed_bwd_ws(const caifq_weight *w, const caifq_lora *l, int64_t m, int compute_dtype)
+{
+  PackedBwdWs o{};
+  o.lora = lora_bwd_ws(w, l, m);
+  o.weight = o.lora.total;
+  o.sums = o.weight + (expand_ok(w, l, kAlignedProbe, m, compute_dtype) ? expanded_weight_bytes(w) : 0);
+  const size_t b = act_tn_scratch_bytes(m, w->out_dim, l->rank);
+  const size_t a = act_tn_scratch_bytes(m, l->rank, w->in_dim);
+  o.total = o.sums + align256(a > b ? a : b);
+  return o;
+}
+}  // namespace
+
+size_t caifq_lora_bwd_packed_workspace_bytes(const caifq_weight *w, const caifq_lora *lora, int64_t m, int32_t compute_dtype)
+{
+  if (w == nullptr || lora == nullptr || m <= 0 || lora->rank <= 0 || w->in_dim <= 0 || w->out_dim <= 0)
+  {
+    return 0;
+  }
+  return packed_bwd_ws(w, lora, m, compute_dtype).total;
+}
+
+int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, const void *dy, const int8_t *x_codes,
+                                 const uint8_t *x_scales, const void *hidden, int64_t m, void *dx, void *d_a, void *d_b,
+                                 void *workspace, size_t workspace_bytes, int32_t compute_dtype, void *stream)
+{
+  const char *who = "caifq_lora_linear_bwd_packed";
+  const int rc = check_lora(w, lora, who);
+  if (rc != CAIFQ_OK)
+  {
+    return rc;
+  }
+  CAIFQ_CHECK_ARG(m >= 0, "%s: negative m", who);
+  CAIFQ_CHECK_ARG(is_float_dtype(compute_dtype), "%s: the compute dtype must be F32, F16 or BF16", who);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int sd = lora->dtype;
+  const size_t elem = dtype_bytes(sd);
+  CAIFQ_CHECK_ARG(d_a && d_b, "%s: null pointer", who);
+  if (m == 0)
+  {
+    CAIFQ_CHECK_CUDA(cudaMemsetAsync(d_a, 0, elem * lora->rank * static_cast<size_t>(w->in_dim), s));
+    CAIFQ_CHECK_CUDA(cudaMemsetAsync(d_b, 0, elem * lora->rank * static_cast<size_t>(w->out_dim), s));
+    return CAIFQ_OK;
+  }
+  CAIFQ_CHECK_ARG(dy && x_codes && x_scales && hidden && dx, "%s: null pointer", who);
+  const PackedBwdWs ws = packed_bwd_ws(w, lora, m, compute_dtype);
+  CAIFQ_CHECK_ARG(workspace != nullptr && workspace_bytes >= ws.total && aligned_to(workspace, 256),
+                  "%s: a workspace of %zu bytes on a 256-byte boundary is needed", who, ws.total);
+  CAIFQ_CHECK_ARG(!overlap(dx, elem * static_cast<size_t>(m) * w->in_dim, dy, elem * static_cast<size_t>(m) * w->out_dim),
+                  "%s: dx and dy overlap", who);
+  const float scale = lora->alpha / static_cast<float>(lora->rank);
+  char *base = static_cast<char *>(workspace);
+  void *d_hidden = base + ws.lora.d_hidden;
+  float *sums = reinterpret_cast<float *>(base + ws.sums);
+  if (fused_lora_ok(w, lora, dy, m, compute_dtype) && aligned_to(dx, 16))
+  {
+    const bool expand = expand_ok(w, lora, dy, m, compute_dtype) && expansion_pays(w, true, m);
+    void *wb = base + ws.weight;
+    // transposed B, padded A and, where the call expands, the weight in one launch; dH = dy . B, and its padded copy times
+    // alpha / rank for the product's extra k-block
+    int r = launch_expand_prepare(*w, expand ? wb : nullptr, lora->a, lora->b, nullptr, base + ws.lora.bt, base + ws.lora.ap,
+                                  nullptr, 0, lora->rank, s);
+    if (r == CAIFQ_OK)
+    {
+      r = launch_skinny_nt(dy, base + ws.lora.bt, d_hidden, base + ws.lora.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
+                           w->out_dim, lora->rank, false, s);
+    }
+    if (r == CAIFQ_OK)
+    {
+      r = launch_act_tn(dy, sd, hidden, sd, nullptr, d_b, sd, scale, sums, m, w->out_dim, lora->rank, s);
+    }
+    if (r == CAIFQ_OK)
+    {
+      r = launch_act_tn(d_hidden, sd, x_codes, CAIFQ_I8, x_scales, d_a, sd, scale, sums, m, lora->rank, w->in_dim, s);
+    }
+    if (r != CAIFQ_OK)
+    {
+      return r;
+    }
+    const caifq_weight wbf = float_weight(wb, CAIFQ_BF16, w->out_dim, w->in_dim);
+    return linear_any(expand ? &wbf : w, true, dy, sd, 1.0f, m, dx, sd, false, compute_dtype, s, who, base + ws.lora.dhs,
+                      base + ws.lora.ap, expand ? epilogue_scale_ptr(w) : nullptr);
+  }
+  // dH = dy . B stays in fp32, and with it the adapter's products
+  int r = launch_act_tn(dy, sd, hidden, sd, nullptr, d_b, sd, scale, sums, m, w->out_dim, lora->rank, s);
+  if (r != CAIFQ_OK)
+  {
+    return r;
+  }
+  const caifq_weight fb = float_weight(lora->b, sd, w->out_dim, lora->rank);
+  r = linear_any(&fb, true, dy, sd, 1.0f, m, d_hidden, CAIFQ_F32, false, CAIFQ_F32, s, who);
+  if (r != CAIFQ_OK)
+  {
+    return r;
+  }
+  r = launch_act_tn(d_hidden, CAIFQ_F32, x_codes, CAIFQ_I8, x_scales, d_a, sd, scale, sums, m, lora->rank, w->in_dim, s);
+  if (r != CAIFQ_OK)
+  {
+    return r;
+  }
+  // dx = (scale dH) . A, then the frozen base on top
+  const caifq_weight fa = float_weight(lora->a, sd, lora->rank, w->in_dim);
+  r = linear_any(&fa, true, d_hidden, CAIFQ_F32, scale, m, dx, sd, false, CAIFQ_F32, s, who);
+  if (r != CAIFQ_OK)
+  {
+    return r;
+  }
+  return linear_any(w, true, dy, sd, 1.0f, m, dx, sd, true, compute_dtype, s, who);
 }
 
 // ----------------------------------------------------------------------- MoE

@@ -50,6 +50,27 @@ class CLora(ctypes.Structure):
     ]
 
 
+class CLoraEntry(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("rank", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+    ]
+
+
+class CLoraBank(ctypes.Structure):
+    _fields_ = [
+        ("entries", ctypes.c_void_p),
+        ("count", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("max_rank", ctypes.c_int32),
+        ("in_dim", ctypes.c_int32),
+        ("out_dim", ctypes.c_int32),
+        ("vectors", ctypes.c_int32),
+    ]
+
+
 _lib = None
 _native = None
 
@@ -99,6 +120,17 @@ _SIGNATURES = {
                                             ctypes.c_float, _i32, _vp]),
     "caifq_rmsnorm_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.c_float, _i32, _i32, _i32, _vp]),
     "caifq_rmsnorm_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "caifq_lora_bank_entries": (ctypes.c_int, [ctypes.POINTER(CLora), _i32, _i32, _i32, ctypes.POINTER(CLoraEntry),
+                                               ctypes.POINTER(CLoraBank)]),
+    "caifq_lora_bank_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CWeight), ctypes.POINTER(CLoraBank), _i64, _i32]),
+    "caifq_lora_bank_linear_fwd": (ctypes.c_int, [ctypes.POINTER(CWeight), ctypes.POINTER(CLoraBank), _vp, _vp, _i64, _vp,
+                                                  _vp, ctypes.c_size_t, _i32, _vp]),
+    "caifq_act_pack": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i64, _i32, _vp]),
+    "caifq_act_unpack": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i64, _i32, _vp]),
+    "caifq_lora_bwd_packed_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CWeight), ctypes.POINTER(CLora), _i64,
+                                                                _i32]),
+    "caifq_lora_linear_bwd_packed": (ctypes.c_int, [ctypes.POINTER(CWeight), ctypes.POINTER(CLora), _vp, _vp, _vp, _vp, _i64,
+                                                    _vp, _vp, _vp, _vp, ctypes.c_size_t, _i32, _vp]),
     "caifq_layernorm_fwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _i32, _i32, _i32, _vp]),
     "caifq_layernorm_bwd_workspace_bytes": (ctypes.c_size_t, [_i32, _i32]),
     "caifq_layernorm_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp]),
@@ -410,6 +442,85 @@ def lora_linear_bwd_noalloc(w, lora, dy, x, hidden, compute=F32):
                                                _ptr(d_a), _ptr(d_b), compute, _stream()),
            "lora_linear_bwd_noalloc")
     return dx, d_a, d_b
+
+
+class LoraBank:
+    """The adapters of many requests beside one frozen linear: a table of Lora objects (one dtype and shape, ranks of their
+    own) in device memory.  The factors stay where they are; the bank holds on to them."""
+
+    def __init__(self, loras):
+        loras = list(loras)
+        if not loras:
+            raise CaifqError("LoraBank: no adapters")
+        in_dim, out_dim = loras[0].a.shape[1], loras[0].b.shape[0]
+        for i, l in enumerate(loras):
+            if tuple(l.a.shape) != (l.rank, in_dim) or tuple(l.b.shape) != (out_dim, l.rank):
+                raise CaifqError("LoraBank: adapter %d has factors %s and %s, [rank, %d] and [%d, rank] expected"
+                                 % (i, tuple(l.a.shape), tuple(l.b.shape), in_dim, out_dim))
+            if l.b.dtype != l.a.dtype or l.a.device != loras[0].a.device or l.b.device != loras[0].a.device:
+                raise CaifqError("LoraBank: adapter %d has factors of two types, or on another device" % i)
+        self.loras = loras
+        self.c = CLoraBank()
+        image = (CLoraEntry * len(loras))()
+        _check(lib().caifq_lora_bank_entries((CLora * len(loras))(*[l.c for l in loras]), len(loras), in_dim, out_dim, image,
+                                             ctypes.byref(self.c)), "lora_bank_entries")
+        self.table = torch.frombuffer(bytearray(image), dtype=torch.uint8).to(loras[0].a.device)
+        self.c.entries = self.table.data_ptr()
+        self._addr = ctypes.addressof(self.c)
+
+    def __len__(self):
+        return len(self.loras)
+
+    def ref(self):
+        return ctypes.byref(self.c)
+
+
+def lora_bank_workspace_bytes(w, bank, m, compute=F32):
+    return int(lib().caifq_lora_bank_workspace_bytes(w.ref(), bank.ref(), m, compute))
+
+
+def lora_bank_linear_fwd(w, bank, adapter_of_row, x, compute=F32, out=None, workspace=None):
+    """y = W-path(x) + each row's own adapter: adapter_of_row is an int32 tensor with an index into the bank for every row of
+    x, or any value outside it (-1) for a row without one.  The indices may change between replays of a captured call."""
+    return (_native or _binding()).lora_bank_linear_fwd(w, bank, adapter_of_row, x, compute, out, workspace)
+
+
+# ---- activations kept in 8 bits ------------------------------------------------
+
+class PackedRows:
+    """Rows in 8 bits: int8 codes shaped like the rows and one scale byte for each 32 columns (2 ** (byte - 127); 255: the
+    block held a value that was not finite)."""
+
+    def __init__(self, codes, scales):
+        _need_cuda(codes, scales)
+        if codes.dtype != torch.int8 or scales.dtype != torch.uint8:
+            raise CaifqError("PackedRows: int8 codes and uint8 scales expected, got %s and %s" % (codes.dtype, scales.dtype))
+        if codes.dim() == 0 or tuple(scales.shape) != tuple(codes.shape[:-1]) + ((codes.shape[-1] + 31) // 32,):
+            raise CaifqError("PackedRows: codes %s do not go with scales %s" % (tuple(codes.shape), tuple(scales.shape)))
+        self.codes = codes
+        self.scales = scales
+
+
+def act_pack(x):
+    """x in 8 bits, for a backward pass to come."""
+    packed = PackedRows.__new__(PackedRows)
+    packed.codes, packed.scales = (_native or _binding()).act_pack(x)
+    return packed
+
+
+def act_unpack(packed, dtype=torch.bfloat16):
+    """The rows that the codes stand for (exact in fp32 and bf16)."""
+    return (_native or _binding()).act_unpack(packed.codes, packed.scales, dtype)
+
+
+def lora_bwd_packed_workspace_bytes(w, lora, m, compute=F32):
+    return int(lib().caifq_lora_bwd_packed_workspace_bytes(w.ref(), lora.ref(), m, compute))
+
+
+def lora_linear_bwd_packed(w, lora, dy, packed, hidden, compute=F32, dx=None, d_a=None, d_b=None, workspace=None):
+    """lora_linear_bwd with the layer's input as act_pack kept it: returns (dx, d_a, d_b).  Equal calls give equal bits."""
+    return (_native or _binding()).lora_linear_bwd_packed(w, lora, lora.a, lora.b, dy, packed.codes, packed.scales, hidden,
+                                                         compute, dx, d_a, d_b, workspace)
 
 
 # ---- MoE ---------------------------------------------------------------------

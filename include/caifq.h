@@ -350,6 +350,73 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
                                             void *d_b, int32_t compute_dtype, void *stream);
 
 /*
+ * Adapters of many requests beside one frozen linear, for serving (no counterpart in the reference, whose adapter layer has
+ * one pair of factors): row t of the batch takes the adapter adapter_of_row[t] of a bank,
+ *   y[t] = x[t] . W_deq^T + (alpha_a / rank_a) (x[t] . A_a^T) . B_a^T,   a = adapter_of_row[t]
+ * Rows whose index is outside [0, count) get the frozen product alone.  Indices, factors and rows may change between two
+ * replays of a captured call; rows need no order.  x . A^T is kept in fp32; the adapters' part is rounded to the result's
+ * type where the frozen product is added to it.
+ *
+ * A bank is a table of `count` entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
+ * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank]), fills the table's image in HOST memory and every
+ * field of *bank but `entries`; the caller copies the image to the device and sets bank->entries to it.  It needs no GPU.
+ * Factors stay where they are and must outlive the calls.
+ */
+typedef struct caifq_lora_entry
+{
+  const void *a;
+  const void *b;
+  int32_t rank;
+  float scale;   /* alpha / rank */
+} caifq_lora_entry;
+
+typedef struct caifq_lora_bank
+{
+  const caifq_lora_entry *entries;   /* device memory */
+  int32_t count;
+  int32_t dtype;       /* F32, F16 or BF16: of the factors, x and y */
+  int32_t max_rank;
+  int32_t in_dim;
+  int32_t out_dim;
+  int32_t vectors;     /* 1: bf16 factors on 16-byte boundaries with ranks of 8, 16, ... 64 */
+} caifq_lora_bank;
+
+CAIFQ_API int caifq_lora_bank_entries(const caifq_lora *loras, int32_t count, int32_t in_dim, int32_t out_dim,
+                                      caifq_lora_entry *entries_host, caifq_lora_bank *bank);
+/* Scratch of the call below (x . A^T, and, for many tokens, the weight expanded as by caifq_linear_fwd_ws): 256-byte aligned,
+ * at least this large; nothing in it outlives the call.  Calls that may overlap on the GPU need workspaces of their own. */
+CAIFQ_API size_t caifq_lora_bank_workspace_bytes(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m,
+                                                 int32_t compute_dtype);
+/* x [m, in], y [m, out] in bank->dtype, not overlapping; adapter_of_row int32 [m], device memory. */
+CAIFQ_API int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *bank, const int32_t *adapter_of_row,
+                                         const void *x, int64_t m, void *y, void *workspace, size_t workspace_bytes,
+                                         int32_t compute_dtype, void *stream);
+
+/*
+ * Activations kept in 8 bits between forward and backward (no counterpart in the reference, which keeps them in the storage
+ * dtype).  codes int8 [rows, dim]; scales uint8 [rows, ceil(dim / 32)]: one byte for 32 columns of a row, the last block
+ * shorter where dim is not a multiple.  The byte b stands for the scale s = 2^(b - 127), the smallest power of two, at least
+ * 2^-126, with max|x| <= 127 s over the block; codes are x / s rounded to the nearest integer, ties to even, and
+ * |x - code * s| <= s / 2 <= max|x| / 126.  A block that holds an infinity or NaN has b = 255 and codes of 0 and stands for
+ * NaN throughout.  code * s is exact in F32 and BF16 (F16 results round, and overflow where the value does).
+ */
+CAIFQ_API int caifq_act_pack(const void *x, int32_t dtype, int8_t *codes, uint8_t *scales, int64_t rows, int32_t dim,
+                             void *stream);
+CAIFQ_API int caifq_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int32_t dtype, int64_t rows, int32_t dim,
+                               void *stream);
+/*
+ * caifq_lora_linear_bwd_expanded for an adapter whose input was kept by caifq_act_pack: the same gradients, with dA taken
+ * from the codes, which are never expanded in memory.  Sums over tokens run in a fixed order (equal calls give equal bits),
+ * and alpha / rank multiplies fp32 sums instead of rounded copies of dy.  With m == 0 dA and dB are zeros.  dx may not overlap dy.
+ */
+CAIFQ_API size_t caifq_lora_bwd_packed_workspace_bytes(const caifq_weight *w, const caifq_lora *lora, int64_t m,
+                                                       int32_t compute_dtype);
+CAIFQ_API int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, const void *dy,
+                                           const int8_t *x_codes, const uint8_t *x_scales, const void *hidden, int64_t m,
+                                           void *dx, void *d_a, void *d_b, void *workspace, size_t workspace_bytes,
+                                           int32_t compute_dtype, void *stream);
+
+/*
  * Several frozen linears that share their input (q / k / v of an attention block, gate / up of an FFN) as ONE
  * tensor-core product over their weights laid one under the other -- the fusion the reference applies to its
  * own non-projection attention path (CHANGES.md:183-187), here for the frozen projections:
