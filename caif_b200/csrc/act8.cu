@@ -112,6 +112,230 @@ unsigned act_grid(int64_t blocks)
   return static_cast<unsigned>(ctas < 148 * 64 ? ctas : 148 * 64);
 }
 
+// ---- rows of whole blocks on 16-byte boundaries: a thread 16 bytes of the row ----
+// HBM-bound (8192 x 4096 bf16: 102 MB each way).  A thread holds kActTrip pieces so that all its loads are in flight before
+// the first is used; the lanes of a block (4, or 8 of fp32) meet in two or three shuffles.  A code is the low byte of
+// x / s + 1.5 * 2^23, which rounds to the nearest even integer: one fused multiply-add instead of a conversion, whose unit
+// takes a sixteenth of a warp a cycle.
+
+constexpr int kActTrip = 4;
+
+// the bits of the largest magnitude of a 16-byte piece, as those of a fp32 number
+template <typename T>
+__device__ __forceinline__ uint32_t piece_most(const uint4 v)
+{
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (sizeof(T) == 4)
+  {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+      m = max(m, w[i] & 0x7FFFFFFFu);
+    }
+    return m;
+  }
+  else
+  {
+    // two at a time as 16-bit integers: the order of magnitudes
+    uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+    {
+      m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    }
+    const uint16_t top = static_cast<uint16_t>(max(m >> 16, m & 0xFFFFu));
+    return __float_as_uint(act_f<T>(*reinterpret_cast<const T *>(&top)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float piece_get(const uint32_t (&w)[4], int i)
+{
+  if constexpr (sizeof(T) == 4)
+  {
+    return __uint_as_float(w[i]);
+  }
+  else
+  {
+    const uint16_t h = static_cast<uint16_t>((i & 1) != 0 ? w[i >> 1] >> 16 : w[i >> 1]);
+    return act_f<T>(*reinterpret_cast<const T *>(&h));
+  }
+}
+
+// four codes a word
+template <typename T>
+__device__ __forceinline__ uint32_t codes_of(const uint32_t (&w)[4], int first, float inverse)
+{
+  constexpr float kRound = 12582912.0f;   // 1.5 * 2^23
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+  {
+    b[i] = __float_as_uint(fmaf(piece_get<T>(w, first + i), inverse, kRound));
+  }
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kActThreads)
+act_pack_rows_kernel(const uint4 *x, void *codes, uint8_t *scales, int64_t pieces)
+{
+  constexpr int PER = 16 / sizeof(T);       // elements of a piece
+  constexpr int LANES = kActBlock / PER;    // pieces of a block
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kActThreads * kActTrip) + threadIdx.x;
+  uint4 v[kActTrip];
+#pragma unroll
+  for (int u = 0; u < kActTrip; ++u)
+  {
+    const int64_t i = base + u * kActThreads;
+    v[u] = i < pieces ? x[i] : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int u = 0; u < kActTrip; ++u)
+  {
+    const int64_t i = base + u * kActThreads;
+    uint32_t most = piece_most<T>(v[u]);
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1)
+    {
+      most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, off));
+    }
+    const uint32_t byte = scale_byte(most);
+    const float inverse = inverse_of(byte);
+    const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+    // (a block that is not finite: codes of 0, whatever NaN would leave in the low byte)
+    const uint32_t keep = byte == 255u ? 0u : 0xFFFFFFFFu;
+    if (i < pieces)
+    {
+      if constexpr (PER == 8)
+      {
+        static_cast<uint2 *>(codes)[i] = make_uint2(codes_of<T>(w, 0, inverse) & keep, codes_of<T>(w, 4, inverse) & keep);
+      }
+      else
+      {
+        static_cast<uint32_t *>(codes)[i] = codes_of<T>(w, 0, inverse) & keep;
+      }
+      if ((threadIdx.x & (LANES - 1)) == 0)
+      {
+        scales[i / LANES] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kActThreads)
+act_unpack_rows_kernel(const void *codes, const uint8_t *scales, uint4 *x, int64_t pieces)
+{
+  constexpr int PER = 16 / sizeof(T);
+  constexpr int LANES = kActBlock / PER;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * (kActThreads * kActTrip) + threadIdx.x;
+  uint2 c[kActTrip];
+  uint32_t b[kActTrip];
+#pragma unroll
+  for (int u = 0; u < kActTrip; ++u)
+  {
+    const int64_t i = base + u * kActThreads;
+    c[u] = make_uint2(0u, 0u);
+    b[u] = 1u;
+    if (i < pieces)
+    {
+      if constexpr (PER == 8)
+      {
+        c[u] = static_cast<const uint2 *>(codes)[i];
+      }
+      else
+      {
+        c[u].x = static_cast<const uint32_t *>(codes)[i];
+      }
+      b[u] = scales[i / LANES];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kActTrip; ++u)
+  {
+    const int64_t i = base + u * kActThreads;
+    const float s = scale_of(b[u]);
+    float f[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+    {
+      // the code with its sign turned in the low mantissa of 2^23
+      const uint32_t word = (e < 4 ? c[u].x : c[u].y) ^ 0x80808080u;
+      f[e] = (__uint_as_float(__byte_perm(word, 0x4B000000u, 0x7440 + (e & 3))) - 8388736.0f) * s;
+    }
+    uint4 out;
+    if constexpr (PER == 4)
+    {
+      out = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+    else
+    {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+      {
+        const T lo = act_t<T>(f[2 * e]);
+        const T hi = act_t<T>(f[2 * e + 1]);
+        w[e] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&lo)) |
+               (static_cast<uint32_t>(*reinterpret_cast<const uint16_t *>(&hi)) << 16);
+      }
+      out = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (i < pieces)
+    {
+      x[i] = out;
+    }
+  }
+}
+
+bool whole_pieces(const void *x, const void *codes, int dim)
+{
+  return (dim % kActBlock) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(codes)) & 15u) == 0;
+}
+
+// pieces that a launch can number
+unsigned piece_grid(int64_t pieces)
+{
+  return static_cast<unsigned>((pieces + kActThreads * kActTrip - 1) / (kActThreads * kActTrip));
+}
+
+template <typename T>
+int act_pack(const void *x, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s)
+{
+  const int64_t pieces = rows * dim / (16 / static_cast<int>(sizeof(T)));
+  if (whole_pieces(x, codes, dim) && pieces <= (static_cast<int64_t>(1) << 40))
+  {
+    CAIFQ_CHECK_CUDA(launch_dependent(act_pack_rows_kernel<T>, dim3(piece_grid(pieces)), dim3(kActThreads), 0, s,
+                                      static_cast<const uint4 *>(x), static_cast<void *>(codes), scales, pieces));
+    return CAIFQ_OK;
+  }
+  CAIFQ_CHECK_CUDA(launch_dependent(act_pack_kernel<T>, dim3(act_grid(rows * ((dim + kActBlock - 1) / kActBlock))),
+                                    dim3(kActThreads), 0, s, static_cast<const T *>(x), codes, scales, rows, dim));
+  return CAIFQ_OK;
+}
+
+template <typename T>
+int act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int64_t rows, int dim, cudaStream_t s)
+{
+  const int64_t pieces = rows * dim / (16 / static_cast<int>(sizeof(T)));
+  if (whole_pieces(x, codes, dim) && pieces <= (static_cast<int64_t>(1) << 40))
+  {
+    CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_rows_kernel<T>, dim3(piece_grid(pieces)), dim3(kActThreads), 0, s,
+                                      static_cast<const void *>(codes), scales, static_cast<uint4 *>(x), pieces));
+    return CAIFQ_OK;
+  }
+  CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_kernel<T>, dim3(act_grid(rows * ((dim + kActBlock - 1) / kActBlock))),
+                                    dim3(kActThreads), 0, s, codes, scales, static_cast<T *>(x), rows, dim));
+  return CAIFQ_OK;
+}
+
+
 // ---- reductions over tokens, any type: C[p, q] = factor * sum_m U[m, p] * V[m, q] ----
 // V may be packed rows.  gridDim.z slices the tokens; a slice's sums go to part[slice][p][q] and tn_finish_kernel adds the
 // slices in order and rounds once.
@@ -229,54 +453,36 @@ int tn_slices(int64_t m, int p, int q)
 
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s)
 {
-  const int64_t blocks = rows * ((dim + kActBlock - 1) / kActBlock);
-  if (blocks <= 0)
+  if (rows <= 0)
   {
     return CAIFQ_OK;
   }
-  const dim3 grid(act_grid(blocks));
   switch (dtype)
   {
     case CAIFQ_F32:
-      CAIFQ_CHECK_CUDA(launch_dependent(act_pack_kernel<float>, grid, dim3(kActThreads), 0, s, static_cast<const float *>(x),
-                                        codes, scales, rows, dim));
-      break;
+      return act_pack<float>(x, codes, scales, rows, dim, s);
     case CAIFQ_F16:
-      CAIFQ_CHECK_CUDA(launch_dependent(act_pack_kernel<__half>, grid, dim3(kActThreads), 0, s,
-                                        static_cast<const __half *>(x), codes, scales, rows, dim));
-      break;
+      return act_pack<__half>(x, codes, scales, rows, dim, s);
     default:
-      CAIFQ_CHECK_CUDA(launch_dependent(act_pack_kernel<__nv_bfloat16>, grid, dim3(kActThreads), 0, s,
-                                        static_cast<const __nv_bfloat16 *>(x), codes, scales, rows, dim));
-      break;
+      return act_pack<__nv_bfloat16>(x, codes, scales, rows, dim, s);
   }
-  return CAIFQ_OK;
 }
 
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s)
 {
-  const int64_t blocks = rows * ((dim + kActBlock - 1) / kActBlock);
-  if (blocks <= 0)
+  if (rows <= 0)
   {
     return CAIFQ_OK;
   }
-  const dim3 grid(act_grid(blocks));
   switch (dtype)
   {
     case CAIFQ_F32:
-      CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_kernel<float>, grid, dim3(kActThreads), 0, s, codes, scales,
-                                        static_cast<float *>(x), rows, dim));
-      break;
+      return act_unpack<float>(codes, scales, x, rows, dim, s);
     case CAIFQ_F16:
-      CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_kernel<__half>, grid, dim3(kActThreads), 0, s, codes, scales,
-                                        static_cast<__half *>(x), rows, dim));
-      break;
+      return act_unpack<__half>(codes, scales, x, rows, dim, s);
     default:
-      CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_kernel<__nv_bfloat16>, grid, dim3(kActThreads), 0, s, codes, scales,
-                                        static_cast<__nv_bfloat16 *>(x), rows, dim));
-      break;
+      return act_unpack<__nv_bfloat16>(codes, scales, x, rows, dim, s);
   }
-  return CAIFQ_OK;
 }
 
 // fp32 scratch of launch_act_tn
