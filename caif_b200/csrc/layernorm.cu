@@ -208,35 +208,430 @@ layernorm_finish_kernel(const float *part, float *grad_gamma, float *grad_beta, 
   }
 }
 
+// ---- rows in registers ----
+// WARPS warps own a row; a thread holds P pieces of V columns, 16 bytes each where the rows allow it (V = 1: rows off a
+// 16-byte boundary or of odd length, element by element).  The row comes in once and all its loads are in flight together.
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) LnPiece
+{
+  T e[V];
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_floats(float (&out)[V], const float *p, float other)
+{
+  if (p == nullptr)
+  {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      out[i] = other;
+    }
+  }
+  else if constexpr (V >= 4)
+  {
+#pragma unroll
+    for (int i = 0; i < V; i += 4)
+    {
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + i));
+      out[i] = v.x;
+      out[i + 1] = v.y;
+      out[i + 2] = v.z;
+      out[i + 3] = v.w;
+    }
+  }
+  else
+  {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      out[i] = __ldg(p + i);
+    }
+  }
+}
+
+// threads of a block: several short rows, or one long one
+template <int WARPS, int LEAST>
+constexpr int kLnBlock = WARPS * 32 > LEAST ? WARPS * 32 : LEAST;
+
+template <typename T, int V, int P, int WARPS>
+__global__ void __launch_bounds__(kLnBlock<WARPS, 128>)
+layernorm_fwd_rows_kernel(const T *x, const float *__restrict__ gamma, const float *__restrict__ beta, T *y,
+                          float *__restrict__ mean_out, float *__restrict__ rstd_out, float epsilon, int rows, int dim)
+{
+  constexpr int SLOTS = kLnBlock<WARPS, 128> / (WARPS * 32);
+  constexpr int THREADS = WARPS * 32;   // of a row
+  __shared__ float sums[SLOTS][WARPS];
+  asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(beta)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int slot = threadIdx.x / THREADS;
+  const int t = threadIdx.x % THREADS;
+  const int r = blockIdx.x * SLOTS + slot;
+  const bool live = r < rows;
+  using Piece = LnPiece<T, V>;
+  Piece v[P];
+  const T *src = x + static_cast<int64_t>(live ? r : 0) * dim;
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = (t + j * THREADS) * V;
+    if (live && c < dim)
+    {
+      v[j] = *reinterpret_cast<const Piece *>(src + c);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    if (live && (t + j * THREADS) * V < dim)
+    {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        s += to_f<T>(v[j].e[i]);
+      }
+    }
+  }
+  const float mean = sum_of<WARPS>(s, sums[slot]) / static_cast<float>(dim);
+  s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    if (live && (t + j * THREADS) * V < dim)
+    {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        const float d = to_f<T>(v[j].e[i]) - mean;
+        s = fmaf(d, d, s);
+      }
+    }
+  }
+  const float rstd = 1.0f / sqrtf(sum_of<WARPS>(s, sums[slot]) / static_cast<float>(dim) + epsilon);
+  if (!live)
+  {
+    return;
+  }
+  T *dst = y + static_cast<int64_t>(r) * dim;
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = (t + j * THREADS) * V;
+    if (c < dim)
+    {
+      float g[V], b[V];
+      load_floats<T, V>(g, gamma != nullptr ? gamma + c : nullptr, 1.0f);
+      load_floats<T, V>(b, beta != nullptr ? beta + c : nullptr, 0.0f);
+      Piece o;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        o.e[i] = from_f<T>(fmaf((to_f<T>(v[j].e[i]) - mean) * rstd, g[i], b[i]));
+      }
+      *reinterpret_cast<Piece *>(dst + c) = o;
+    }
+  }
+  if (t == 0)
+  {
+    mean_out[r] = mean;
+    rstd_out[r] = rstd;
+  }
+}
+
+// two sums at once, as sum_of
+template <int WARPS>
+__device__ __forceinline__ float2 sums_of(float2 v, float2 *slots)
+{
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+  {
+    v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, off);
+    v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, off);
+  }
+  if constexpr (WARPS > 1)
+  {
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0)
+    {
+      slots[(threadIdx.x >> 5) % WARPS] = v;
+    }
+    __syncthreads();
+    v = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+    {
+      v.x += slots[w].x;
+      v.y += slots[w].y;
+    }
+  }
+  return v;
+}
+
+// dx and this block's share of dgamma and dbeta in one pass: a block takes rows slot, slot + gridDim.x * SLOTS, ..., a thread
+// keeps its columns' sums in registers over all of them, and the row after this one is on its way while this one is summed.
+// part[block][0][c], part[block][1][c] as in layernorm_columns_kernel.
+template <typename T, int V, int P, int WARPS>
+__global__ void __launch_bounds__(kLnBlock<WARPS, 256>)
+layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gamma, const float *__restrict__ mean_in,
+                          const float *__restrict__ rstd_in, T *dx, float *__restrict__ part, int rows, int dim)
+{
+  constexpr int SLOTS = kLnBlock<WARPS, 256> / (WARPS * 32);
+  constexpr int THREADS = WARPS * 32;
+  extern __shared__ float columns[];   // [2][dim] where SLOTS > 1
+  __shared__ float2 sums[SLOTS][WARPS];
+  asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(mean_in), "+l"(rstd_in)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  using Piece = LnPiece<T, V>;
+  const int slot = threadIdx.x / THREADS;
+  const int t = threadIdx.x % THREADS;
+  float g[P][V], sg[P][V], sb[P][V];
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = (t + j * THREADS) * V;
+    if (c < dim)
+    {
+      load_floats<T, V>(g[j], gamma != nullptr ? gamma + c : nullptr, 1.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      sg[j][i] = sb[j][i] = 0.0f;
+    }
+  }
+  const int step = static_cast<int>(gridDim.x) * SLOTS;
+  Piece vx[P], vd[P];
+  float mean = 0.0f, rstd = 0.0f;
+  auto fetch = [&](int64_t r, Piece(&px)[P], Piece(&pd)[P], float &m, float &s) {
+    if (r < rows)
+    {
+      const int64_t at = r * dim;
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+      {
+        const int c = (t + j * THREADS) * V;
+        if (c < dim)
+        {
+          px[j] = *reinterpret_cast<const Piece *>(x + at + c);
+          pd[j] = *reinterpret_cast<const Piece *>(dy + at + c);
+        }
+      }
+      m = mean_in[r];
+      s = rstd_in[r];
+    }
+  };
+  const int first = static_cast<int>(blockIdx.x) * SLOTS;
+  fetch(first + slot, vx, vd, mean, rstd);
+  for (int64_t base = first; base < rows; base += step)   // (every slot takes part in the sums' barriers)
+  {
+    const int64_t r = base + slot;
+    const bool live = r < rows;
+    Piece nx[P], nd[P];
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    fetch(r + step, nx, nd, next_mean, next_rstd);
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      if (live && (t + j * THREADS) * V < dim)
+      {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          const float d = to_f<T>(vd[j].e[i]);
+          const float xh = (to_f<T>(vx[j].e[i]) - mean) * rstd;
+          const float w = d * g[j][i];
+          s.x += w;
+          s.y = fmaf(w, xh, s.y);
+          sg[j][i] = fmaf(d, xh, sg[j][i]);
+          sb[j][i] += d;
+        }
+      }
+    }
+    s = sums_of<WARPS>(s, sums[slot]);
+    const float s1 = s.x / static_cast<float>(dim);
+    const float s2 = s.y / static_cast<float>(dim);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      const int c = (t + j * THREADS) * V;
+      if (live && c < dim)
+      {
+        Piece o;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          const float xh = (to_f<T>(vx[j].e[i]) - mean) * rstd;
+          o.e[i] = from_f<T>(rstd * (to_f<T>(vd[j].e[i]) * g[j][i] - s1 - xh * s2));
+        }
+        *reinterpret_cast<Piece *>(dx + r * dim + c) = o;
+      }
+      vx[j] = nx[j];
+      vd[j] = nd[j];
+    }
+    mean = next_mean;
+    rstd = next_rstd;
+  }
+  if (part == nullptr)
+  {
+    return;
+  }
+  float *mine = part + static_cast<int64_t>(blockIdx.x) * 2 * dim;
+  float *to = SLOTS > 1 ? columns : mine;
+#pragma unroll 1
+  for (int turn = 0; turn < SLOTS; ++turn)   // slot by slot, in order
+  {
+    if (slot == turn)
+    {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+      {
+        const int c = (t + j * THREADS) * V;
+        if (c < dim)
+        {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+          {
+            to[c + i] = turn > 0 ? to[c + i] + sg[j][i] : sg[j][i];
+            to[dim + c + i] = turn > 0 ? to[dim + c + i] + sb[j][i] : sb[j][i];
+          }
+        }
+      }
+    }
+    if (SLOTS > 1)
+    {
+      __syncthreads();
+    }
+  }
+  if (SLOTS > 1)
+  {
+    for (int c = threadIdx.x; c < 2 * dim; c += kLnBlock<WARPS, 256>)
+    {
+      mine[c] = columns[c];
+    }
+  }
+}
+
 // slices of rows with partial sums of their own
 int ln_slices(int rows) { return rows < 148 * 2 ? rows : 148 * 2; }
 
 unsigned ln_grid(int rows) { return static_cast<unsigned>(rows < 148 * 8 ? rows : 148 * 8); }
 
-template <typename T>
-int ln_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd, float epsilon, int rows,
-           int dim, cudaStream_t s)
+bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <typename T, int V, int P, int WARPS>
+int ln_fwd_rows(const T *x, const float *gamma, const float *beta, T *y, float *mean, float *rstd, float epsilon, int rows,
+                int dim, cudaStream_t s)
 {
-  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s,
-                                    static_cast<const T *>(x), gamma, beta, static_cast<T *>(y), mean, rstd, epsilon, rows,
-                                    static_cast<int64_t>(dim)));
+  constexpr int BLOCK = kLnBlock<WARPS, 128>;
+  constexpr int SLOTS = BLOCK / (WARPS * 32);
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_rows_kernel<T, V, P, WARPS>,
+                                    dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + SLOTS - 1) / SLOTS)), dim3(BLOCK), 0, s, x,
+                                    gamma, beta, y, mean, rstd, epsilon, rows, dim));
   return CAIFQ_OK;
 }
 
+// the fewest warps (a power of two) whose registers hold the row
+#define CAIFQ_LN_WARPS(CALL, ELEMENTS)  \
+  if (dim <= 32 * (ELEMENTS))           \
+  {                                     \
+    return CALL(1);                     \
+  }                                     \
+  if (dim <= 64 * (ELEMENTS))           \
+  {                                     \
+    return CALL(2);                     \
+  }                                     \
+  if (dim <= 128 * (ELEMENTS))          \
+  {                                     \
+    return CALL(4);                     \
+  }                                     \
+  if (dim <= 256 * (ELEMENTS))          \
+  {                                     \
+    return CALL(8);                     \
+  }                                     \
+  if (dim <= 512 * (ELEMENTS))          \
+  {                                     \
+    return CALL(16);                    \
+  }
+
 template <typename T>
-int ln_bwd(const void *dy, const void *x, const float *gamma, const float *mean, const float *rstd, void *dx, float *part,
-           int slices, int rows, int dim, cudaStream_t s)
+int ln_fwd(const void *xv, const float *gamma, const float *beta, void *yv, float *mean, float *rstd, float epsilon, int rows,
+           int dim, cudaStream_t s)
 {
+  const T *x = static_cast<const T *>(xv);
+  T *y = static_cast<T *>(yv);
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  if ((dim % V) == 0 && on_16(x) && on_16(y) && on_16(gamma) && on_16(beta))
+  {
+#define CAIFQ_LN_CALL(W) ln_fwd_rows<T, V, 4, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 4 * V)
+    if (dim <= 1024 * 4 * V)
+    {
+      return CAIFQ_LN_CALL(32);
+    }
+#undef CAIFQ_LN_CALL
+  }
+  else
+  {
+#define CAIFQ_LN_CALL(W) ln_fwd_rows<T, 1, 16, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+    if (dim <= 1024 * 16)
+    {
+      return CAIFQ_LN_CALL(32);
+    }
+#undef CAIFQ_LN_CALL
+  }
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s, x, gamma, beta, y,
+                                    mean, rstd, epsilon, rows, static_cast<int64_t>(dim)));
+  return CAIFQ_OK;
+}
+
+template <typename T, int V, int P, int WARPS>
+int ln_bwd_rows(const T *dy, const T *x, const float *gamma, const float *mean, const float *rstd, T *dx, float *part,
+                int *slices, int rows, int dim, cudaStream_t s)
+{
+  constexpr int BLOCK = kLnBlock<WARPS, 256>;
+  constexpr int SLOTS = BLOCK / (WARPS * 32);
+  const int blocks = (rows - 1) / SLOTS + 1;
+  *slices = blocks < ln_slices(rows) ? blocks : ln_slices(rows);
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_bwd_rows_kernel<T, V, P, WARPS>, dim3(static_cast<unsigned>(*slices)), dim3(BLOCK),
+                                    SLOTS > 1 ? sizeof(float) * 2 * static_cast<size_t>(dim) : 0, s, dy, x, gamma, mean, rstd,
+                                    dx, part, rows, dim));
+  return CAIFQ_OK;
+}
+
+// part: null where the columns' sums are not wanted; *slices: how many of them the launches leave
+template <typename T>
+int ln_bwd(const void *dyv, const void *xv, const float *gamma, const float *mean, const float *rstd, void *dxv, float *part,
+           int *slices, int rows, int dim, cudaStream_t s)
+{
+  const T *dy = static_cast<const T *>(dyv);
+  const T *x = static_cast<const T *>(xv);
+  T *dx = static_cast<T *>(dxv);
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  if ((dim % V) == 0 && on_16(dy) && on_16(x) && on_16(dx) && on_16(gamma))
+  {
+#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, V, 16 / V, W>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+#undef CAIFQ_LN_CALL
+  }
+  else
+  {
+#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, 1, 16, W>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+#undef CAIFQ_LN_CALL
+  }
+  *slices = ln_slices(rows);
   if (part != nullptr)
   {
     // (before dx, which may be written over dy)
-    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_columns_kernel<T>, dim3((dim + 31) / 32, static_cast<unsigned>(slices)),
-                                      dim3(kLnThreads), 0, s, static_cast<const T *>(dy), static_cast<const T *>(x), mean,
-                                      rstd, part, rows, static_cast<int64_t>(dim)));
+    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_columns_kernel<T>, dim3((dim + 31) / 32, static_cast<unsigned>(*slices)),
+                                      dim3(kLnThreads), 0, s, dy, x, mean, rstd, part, rows, static_cast<int64_t>(dim)));
   }
-  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_dx_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s,
-                                    static_cast<const T *>(dy), static_cast<const T *>(x), gamma, mean, rstd,
-                                    static_cast<T *>(dx), rows, static_cast<int64_t>(dim)));
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_dx_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s, dy, x, gamma, mean,
+                                    rstd, dx, rows, static_cast<int64_t>(dim)));
   return CAIFQ_OK;
 }
 
@@ -270,7 +665,7 @@ int launch_layernorm_bwd(const void *dy, const void *x, const float *gamma, cons
                          cudaStream_t s)
 {
   const bool columns = grad_gamma != nullptr || grad_beta != nullptr;
-  const int slices = ln_slices(rows);
+  int slices = 0;
   if (rows > 0)
   {
     float *part = columns ? workspace : nullptr;
@@ -278,13 +673,13 @@ int launch_layernorm_bwd(const void *dy, const void *x, const float *gamma, cons
     switch (dtype)
     {
       case CAIFQ_F32:
-        rc = ln_bwd<float>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s);
+        rc = ln_bwd<float>(dy, x, gamma, mean, rstd, dx, part, &slices, rows, dim, s);
         break;
       case CAIFQ_F16:
-        rc = ln_bwd<__half>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s);
+        rc = ln_bwd<__half>(dy, x, gamma, mean, rstd, dx, part, &slices, rows, dim, s);
         break;
       default:
-        rc = ln_bwd<__nv_bfloat16>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s);
+        rc = ln_bwd<__nv_bfloat16>(dy, x, gamma, mean, rstd, dx, part, &slices, rows, dim, s);
         break;
     }
     if (rc != CAIFQ_OK)
