@@ -5,6 +5,8 @@
 // All sums are fp32 and run in a fixed order: a row's variance is taken around its mean (a second pass over the row, not the
 // difference of two large sums), and the gradients of gamma and beta are partial sums per slice of rows, added slice by
 // slice by a second launch, so that two calls give the same bits.  y and dx are rounded once.
+#include <atomic>
+
 #include "common.cuh"
 
 namespace caifq
@@ -340,7 +342,21 @@ layernorm_fwd_rows_kernel(const T *x, const float *__restrict__ gamma, const flo
   }
 }
 
-// two sums at once, as sum_of
+// ---- many rows: a block takes rows one after the other ----
+// gamma and beta (or the columns' sums of the backward pass) stay in registers from row to row, and the next rows are on their
+// way: 16-byte pieces come by asynchronous copies through a ring of RING rows in shared memory, of which every thread reads
+// back exactly what it copied, so that no barrier belongs to the copies.  Rows that no 16-byte piece fits are fetched one row
+// ahead into registers.  A sum's slots alternate from row to row: one barrier a sum.
+
+template <typename T>
+constexpr int kLnRing = sizeof(T) == 4 ? 3 : 4;
+
+__device__ __forceinline__ void copy_16(void *to, const void *from)
+{
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
+               : "memory");
+}
+
 template <int WARPS>
 __device__ __forceinline__ float2 sums_of(float2 v, float2 *slots)
 {
@@ -352,7 +368,6 @@ __device__ __forceinline__ float2 sums_of(float2 v, float2 *slots)
   }
   if constexpr (WARPS > 1)
   {
-    __syncthreads();
     if ((threadIdx.x & 31) == 0)
     {
       slots[(threadIdx.x >> 5) % WARPS] = v;
@@ -369,23 +384,260 @@ __device__ __forceinline__ float2 sums_of(float2 v, float2 *slots)
   return v;
 }
 
-// dx and this block's share of dgamma and dbeta in one pass: a block takes rows slot, slot + gridDim.x * SLOTS, ..., a thread
-// keeps its columns' sums in registers over all of them, and the row after this one is on its way while this one is summed.
+template <int WARPS>
+__device__ __forceinline__ float one_sum_of(float v, float *slots)
+{
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
+  {
+    v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+  }
+  if constexpr (WARPS > 1)
+  {
+    if ((threadIdx.x & 31) == 0)
+    {
+      slots[(threadIdx.x >> 5) % WARPS] = v;
+    }
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w)
+    {
+      v += slots[w];
+    }
+  }
+  return v;
+}
+
+// the rows of N tensors that a block walks over: start() once, then next() for each row in turn gives this thread's pieces
+template <typename T, int V, int P, int THREADS, int BLOCK, int N>
+struct RowsAhead
+{
+  using Piece = LnPiece<T, V>;
+  static constexpr int RING = kLnRing<T>;
+  static constexpr size_t kBytes = V > 1 ? static_cast<size_t>(RING) * N * P * BLOCK * 16 : 0;
+  const T *src[N];
+  int64_t row;     // the next row to fetch
+  int64_t step;
+  int rows, dim, t;
+  uint4 *ring;
+  int at;          // ring row that next() reads
+  Piece ahead[V > 1 ? 1 : N][V > 1 ? 1 : P];
+
+  __device__ __forceinline__ void fetch(int stage)
+  {
+    if constexpr (V > 1)
+    {
+      if (row < rows)
+      {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+        {
+#pragma unroll
+          for (int j = 0; j < P; ++j)
+          {
+            const int c = (t + j * THREADS) * V;
+            if (c < dim)
+            {
+              copy_16(ring + ((stage * N + n) * P + j) * BLOCK + threadIdx.x, src[n] + row * dim + c);
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    else
+    {
+      if (row < rows)
+      {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+        {
+#pragma unroll
+          for (int j = 0; j < P; ++j)
+          {
+            const int c = (t + j * THREADS) * V;
+            if (c < dim)
+            {
+              ahead[n][j] = *reinterpret_cast<const Piece *>(src[n] + row * dim + c);
+            }
+          }
+        }
+      }
+    }
+    row += step;
+  }
+
+  __device__ __forceinline__ void start()
+  {
+    at = 0;
+#pragma unroll
+    for (int i = 0; i < (V > 1 ? RING - 1 : 1); ++i)
+    {
+      fetch(i);
+    }
+  }
+
+  __device__ __forceinline__ void next(Piece (&out)[N][P])
+  {
+    if constexpr (V > 1)
+    {
+      // (the ring row before this one, which this thread has read, is filled again)
+      fetch(at == 0 ? RING - 1 : at - 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+      {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+        {
+          const uint4 v = ring[((at * N + n) * P + j) * BLOCK + threadIdx.x];
+          out[n][j] = *reinterpret_cast<const Piece *>(&v);
+        }
+      }
+      at = at == RING - 1 ? 0 : at + 1;
+    }
+    else
+    {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+      {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+        {
+          out[n][j] = ahead[n][j];
+        }
+      }
+      fetch(0);
+    }
+  }
+};
+
+template <typename T, int V, int P, int WARPS>
+__global__ void __launch_bounds__(kLnBlock<WARPS, 256>, WARPS <= 8 ? 3 : 1)
+layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const float *__restrict__ beta, T *y,
+                          float *__restrict__ mean_out, float *__restrict__ rstd_out, float epsilon, int rows, int dim)
+{
+  constexpr int BLOCK = kLnBlock<WARPS, 256>;
+  constexpr int SLOTS = BLOCK / (WARPS * 32);
+  constexpr int THREADS = WARPS * 32;
+  extern __shared__ uint4 ln_ring[];
+  __shared__ float sums[2][2][SLOTS][WARPS];
+  asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(beta)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  using Rows = RowsAhead<T, V, P, THREADS, BLOCK, 1>;
+  const int slot = threadIdx.x / THREADS;
+  const int t = threadIdx.x % THREADS;
+  const int first = static_cast<int>(blockIdx.x) * SLOTS;
+  const int step = static_cast<int>(gridDim.x) * SLOTS;
+  Rows in;
+  in.src[0] = x;
+  in.row = first + slot;
+  in.step = step;
+  in.rows = rows;
+  in.dim = dim;
+  in.t = t;
+  in.ring = ln_ring;
+  in.start();
+  float g[P][V], b[P][V];
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = (t + j * THREADS) * V;
+    if (c < dim)
+    {
+      load_floats<T, V>(g[j], gamma != nullptr ? gamma + c : nullptr, 1.0f);
+      load_floats<T, V>(b[j], beta != nullptr ? beta + c : nullptr, 0.0f);
+    }
+  }
+  int turn = 0;
+  for (int64_t base = first; base < rows; base += step, turn ^= 1)   // (every slot takes part in the sums' barriers)
+  {
+    const int64_t r = base + slot;
+    const bool live = r < rows;
+    LnPiece<T, V> v[1][P];
+    in.next(v);
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      if (live && (t + j * THREADS) * V < dim)
+      {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          s += to_f<T>(v[0][j].e[i]);
+        }
+      }
+    }
+    const float mean = one_sum_of<WARPS>(s, sums[turn][0][slot]) / static_cast<float>(dim);
+    s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      if (live && (t + j * THREADS) * V < dim)
+      {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          const float d = to_f<T>(v[0][j].e[i]) - mean;
+          s = fmaf(d, d, s);
+        }
+      }
+    }
+    const float rstd = 1.0f / sqrtf(one_sum_of<WARPS>(s, sums[turn][1][slot]) / static_cast<float>(dim) + epsilon);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      const int c = (t + j * THREADS) * V;
+      if (live && c < dim)
+      {
+        LnPiece<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          o.e[i] = from_f<T>(fmaf((to_f<T>(v[0][j].e[i]) - mean) * rstd, g[j][i], b[j][i]));
+        }
+        *reinterpret_cast<LnPiece<T, V> *>(y + r * dim + c) = o;
+      }
+    }
+    if (live && t == 0)
+    {
+      mean_out[r] = mean;
+      rstd_out[r] = rstd;
+    }
+  }
+}
+
+// dx and this block's share of dgamma and dbeta in one pass: a thread keeps its columns' sums over all rows of the block.
 // part[block][0][c], part[block][1][c] as in layernorm_columns_kernel.
 template <typename T, int V, int P, int WARPS>
 __global__ void __launch_bounds__(kLnBlock<WARPS, 256>)
 layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gamma, const float *__restrict__ mean_in,
                           const float *__restrict__ rstd_in, T *dx, float *__restrict__ part, int rows, int dim)
 {
-  constexpr int SLOTS = kLnBlock<WARPS, 256> / (WARPS * 32);
+  constexpr int BLOCK = kLnBlock<WARPS, 256>;
+  constexpr int SLOTS = BLOCK / (WARPS * 32);
   constexpr int THREADS = WARPS * 32;
-  extern __shared__ float columns[];   // [2][dim] where SLOTS > 1
-  __shared__ float2 sums[SLOTS][WARPS];
+  extern __shared__ uint4 ln_ring[];   // the ring; then, where SLOTS > 1, the columns' sums [2][dim]
+  __shared__ float2 sums[2][SLOTS][WARPS];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(mean_in), "+l"(rstd_in)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  using Piece = LnPiece<T, V>;
+  using Rows = RowsAhead<T, V, P, THREADS, BLOCK, 2>;
   const int slot = threadIdx.x / THREADS;
   const int t = threadIdx.x % THREADS;
+  const int first = static_cast<int>(blockIdx.x) * SLOTS;
+  const int step = static_cast<int>(gridDim.x) * SLOTS;
+  Rows in;
+  in.src[0] = x;
+  in.src[1] = dy;
+  in.row = first + slot;
+  in.step = step;
+  in.rows = rows;
+  in.dim = dim;
+  in.t = t;
+  in.ring = ln_ring;
+  in.start();
   float g[P][V], sg[P][V], sb[P][V];
 #pragma unroll
   for (int j = 0; j < P; ++j)
@@ -401,36 +653,25 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
       sg[j][i] = sb[j][i] = 0.0f;
     }
   }
-  const int step = static_cast<int>(gridDim.x) * SLOTS;
-  Piece vx[P], vd[P];
-  float mean = 0.0f, rstd = 0.0f;
-  auto fetch = [&](int64_t r, Piece(&px)[P], Piece(&pd)[P], float &m, float &s) {
-    if (r < rows)
-    {
-      const int64_t at = r * dim;
-#pragma unroll
-      for (int j = 0; j < P; ++j)
-      {
-        const int c = (t + j * THREADS) * V;
-        if (c < dim)
-        {
-          px[j] = *reinterpret_cast<const Piece *>(x + at + c);
-          pd[j] = *reinterpret_cast<const Piece *>(dy + at + c);
-        }
-      }
-      m = mean_in[r];
-      s = rstd_in[r];
-    }
-  };
-  const int first = static_cast<int>(blockIdx.x) * SLOTS;
-  fetch(first + slot, vx, vd, mean, rstd);
-  for (int64_t base = first; base < rows; base += step)   // (every slot takes part in the sums' barriers)
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  if (first + slot < rows)
+  {
+    next_mean = mean_in[first + slot];
+    next_rstd = rstd_in[first + slot];
+  }
+  int turn = 0;
+  for (int64_t base = first; base < rows; base += step, turn ^= 1)   // (every slot takes part in the sums' barriers)
   {
     const int64_t r = base + slot;
     const bool live = r < rows;
-    Piece nx[P], nd[P];
-    float next_mean = 0.0f, next_rstd = 0.0f;
-    fetch(r + step, nx, nd, next_mean, next_rstd);
+    LnPiece<T, V> v[2][P];
+    in.next(v);
+    const float mean = next_mean, rstd = next_rstd;
+    if (r + step < rows)
+    {
+      next_mean = mean_in[r + step];
+      next_rstd = rstd_in[r + step];
+    }
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for (int j = 0; j < P; ++j)
@@ -440,8 +681,8 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
 #pragma unroll
         for (int i = 0; i < V; ++i)
         {
-          const float d = to_f<T>(vd[j].e[i]);
-          const float xh = (to_f<T>(vx[j].e[i]) - mean) * rstd;
+          const float d = to_f<T>(v[1][j].e[i]);
+          const float xh = (to_f<T>(v[0][j].e[i]) - mean) * rstd;
           const float w = d * g[j][i];
           s.x += w;
           s.y = fmaf(w, xh, s.y);
@@ -450,7 +691,7 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
         }
       }
     }
-    s = sums_of<WARPS>(s, sums[slot]);
+    s = sums_of<WARPS>(s, sums[turn][slot]);
     const float s1 = s.x / static_cast<float>(dim);
     const float s2 = s.y / static_cast<float>(dim);
 #pragma unroll
@@ -459,31 +700,28 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
       const int c = (t + j * THREADS) * V;
       if (live && c < dim)
       {
-        Piece o;
+        LnPiece<T, V> o;
 #pragma unroll
         for (int i = 0; i < V; ++i)
         {
-          const float xh = (to_f<T>(vx[j].e[i]) - mean) * rstd;
-          o.e[i] = from_f<T>(rstd * (to_f<T>(vd[j].e[i]) * g[j][i] - s1 - xh * s2));
+          const float xh = (to_f<T>(v[0][j].e[i]) - mean) * rstd;
+          o.e[i] = from_f<T>(rstd * (to_f<T>(v[1][j].e[i]) * g[j][i] - s1 - xh * s2));
         }
-        *reinterpret_cast<Piece *>(dx + r * dim + c) = o;
+        *reinterpret_cast<LnPiece<T, V> *>(dx + r * dim + c) = o;
       }
-      vx[j] = nx[j];
-      vd[j] = nd[j];
     }
-    mean = next_mean;
-    rstd = next_rstd;
   }
   if (part == nullptr)
   {
     return;
   }
+  float *columns = reinterpret_cast<float *>(reinterpret_cast<char *>(ln_ring) + Rows::kBytes);
   float *mine = part + static_cast<int64_t>(blockIdx.x) * 2 * dim;
   float *to = SLOTS > 1 ? columns : mine;
 #pragma unroll 1
-  for (int turn = 0; turn < SLOTS; ++turn)   // slot by slot, in order
+  for (int i = 0; i < SLOTS; ++i)   // slot by slot, in order
   {
-    if (slot == turn)
+    if (slot == i)
     {
 #pragma unroll
       for (int j = 0; j < P; ++j)
@@ -492,10 +730,10 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
         if (c < dim)
         {
 #pragma unroll
-          for (int i = 0; i < V; ++i)
+          for (int e = 0; e < V; ++e)
           {
-            to[c + i] = turn > 0 ? to[c + i] + sg[j][i] : sg[j][i];
-            to[dim + c + i] = turn > 0 ? to[dim + c + i] + sb[j][i] : sb[j][i];
+            to[c + e] = i > 0 ? to[c + e] + sg[j][e] : sg[j][e];
+            to[dim + c + e] = i > 0 ? to[dim + c + e] + sb[j][e] : sb[j][e];
           }
         }
       }
@@ -507,7 +745,7 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
   }
   if (SLOTS > 1)
   {
-    for (int c = threadIdx.x; c < 2 * dim; c += kLnBlock<WARPS, 256>)
+    for (int c = threadIdx.x; c < 2 * dim; c += BLOCK)
     {
       mine[c] = columns[c];
     }
@@ -519,6 +757,8 @@ int ln_slices(int rows) { return rows < 148 * 2 ? rows : 148 * 2; }
 
 unsigned ln_grid(int rows) { return static_cast<unsigned>(rows < 148 * 8 ? rows : 148 * 8); }
 
+constexpr size_t kLnPlainSmem = 40 * 1024;   // dynamic, beside the static slots, without asking
+
 bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <typename T, int V, int P, int WARPS>
@@ -529,6 +769,45 @@ int ln_fwd_rows(const T *x, const float *gamma, const float *beta, T *y, float *
   constexpr int SLOTS = BLOCK / (WARPS * 32);
   CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_rows_kernel<T, V, P, WARPS>,
                                     dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + SLOTS - 1) / SLOTS)), dim3(BLOCK), 0, s, x,
+                                    gamma, beta, y, mean, rstd, epsilon, rows, dim));
+  return CAIFQ_OK;
+}
+
+// dynamic shared memory beyond 48 KB is asked for once per kernel and device
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t> &done)
+{
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev >= kMaxDevices || (done.load(std::memory_order_relaxed) >> dev & 1u) != 0)
+  {
+    return e;
+  }
+  const cudaError_t set =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (set == cudaSuccess)
+  {
+    done.fetch_or(static_cast<uint64_t>(1) << dev, std::memory_order_relaxed);
+  }
+  return set;
+}
+
+template <typename T, int V, int P, int WARPS>
+int ln_fwd_many(const T *x, const float *gamma, const float *beta, T *y, float *mean, float *rstd, float epsilon, int rows,
+                int dim, cudaStream_t s)
+{
+  constexpr int BLOCK = kLnBlock<WARPS, 256>;
+  constexpr int SLOTS = BLOCK / (WARPS * 32);
+  constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 1>::kBytes;
+  static std::atomic<uint64_t> done{0};
+  if (kBytes > kLnPlainSmem)
+  {
+    CAIFQ_CHECK_CUDA(allow_smem(layernorm_fwd_many_kernel<T, V, P, WARPS>, kBytes, done));
+  }
+  const int blocks = (rows - 1) / SLOTS + 1;
+  const int most = 148 * (WARPS <= 8 ? 3 : 1);
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_many_kernel<T, V, P, WARPS>,
+                                    dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(BLOCK), kBytes, s, x,
                                     gamma, beta, y, mean, rstd, epsilon, rows, dim));
   return CAIFQ_OK;
 }
@@ -565,6 +844,12 @@ int ln_fwd(const void *xv, const float *gamma, const float *beta, void *yv, floa
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   if ((dim % V) == 0 && on_16(x) && on_16(y) && on_16(gamma) && on_16(beta))
   {
+#define CAIFQ_LN_CALL(W) ln_fwd_many<T, V, 16 / V, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
+    if (rows > 148)
+    {
+      CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+    }
+#undef CAIFQ_LN_CALL
 #define CAIFQ_LN_CALL(W) ln_fwd_rows<T, V, 4, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
     CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 4 * V)
     if (dim <= 1024 * 4 * V)
@@ -594,11 +879,19 @@ int ln_bwd_rows(const T *dy, const T *x, const float *gamma, const float *mean, 
 {
   constexpr int BLOCK = kLnBlock<WARPS, 256>;
   constexpr int SLOTS = BLOCK / (WARPS * 32);
+  constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 2>::kBytes;
+  constexpr size_t kColumns = SLOTS > 1 ? sizeof(float) * 2 * 16 * WARPS * 32 : 0;   // of the widest row
+  static std::atomic<uint64_t> done{0};
+  if (kBytes + kColumns > kLnPlainSmem)
+  {
+    CAIFQ_CHECK_CUDA(allow_smem(layernorm_bwd_rows_kernel<T, V, P, WARPS>, kBytes + kColumns, done));
+  }
   const int blocks = (rows - 1) / SLOTS + 1;
-  *slices = blocks < ln_slices(rows) ? blocks : ln_slices(rows);
+  const int most = WARPS <= 8 ? 148 * 2 : 148;
+  *slices = blocks < most ? blocks : most;
   CAIFQ_CHECK_CUDA(launch_dependent(layernorm_bwd_rows_kernel<T, V, P, WARPS>, dim3(static_cast<unsigned>(*slices)), dim3(BLOCK),
-                                    SLOTS > 1 ? sizeof(float) * 2 * static_cast<size_t>(dim) : 0, s, dy, x, gamma, mean, rstd,
-                                    dx, part, rows, dim));
+                                    kBytes + (SLOTS > 1 ? sizeof(float) * 2 * static_cast<size_t>(dim) : 0), s, dy, x, gamma,
+                                    mean, rstd, dx, part, rows, dim));
   return CAIFQ_OK;
 }
 
