@@ -173,11 +173,12 @@ layernorm_columns_kernel(const T *dy, const T *x, const float *__restrict__ mean
   }
 }
 
-// the slices' sums, in a fixed order: eight threads a column take every eighth slice each
-__global__ void __launch_bounds__(kLnThreads)
+// the slices' sums, in a fixed order: 32 threads a column take every 32nd slice each (with eight, 296 slices of 4096 columns
+// took 10 us)
+__global__ void __launch_bounds__(1024)
 layernorm_finish_kernel(const float *part, float *grad_gamma, float *grad_beta, int slices, int64_t dim, int accumulate)
 {
-  __shared__ float tile[8][33];
+  __shared__ float tile[32][33];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
@@ -192,21 +193,24 @@ layernorm_finish_kernel(const float *part, float *grad_gamma, float *grad_beta, 
   if (c < dim)
   {
     const float *src = part + static_cast<int64_t>(blockIdx.y) * dim + c;
-#pragma unroll 8
-    for (int i = group; i < slices; i += 8)
+#pragma unroll 10
+    for (int i = group; i < slices; i += 32)
     {
       s += src[static_cast<int64_t>(i) * 2 * dim];
     }
   }
   tile[group][lane] = s;
   __syncthreads();
-  if (group == 0 && c < dim)
+  s = tile[lane][group];   // a warp a column
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1)
   {
-    for (int i = 1; i < 8; ++i)
-    {
-      s += tile[i][lane];
-    }
-    grad[c] = accumulate != 0 ? grad[c] + s : s;
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, off);
+  }
+  const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + group;
+  if (lane == 0 && column < dim)
+  {
+    grad[column] = accumulate != 0 ? grad[column] + s : s;
   }
 }
 
@@ -357,56 +361,92 @@ __device__ __forceinline__ void copy_16(void *to, const void *from)
                : "memory");
 }
 
-template <int WARPS>
-__device__ __forceinline__ float2 sums_of(float2 v, float2 *slots)
+// pairs of floats: Blackwell adds and multiplies two at a time, and these kernels would be bound by their instructions
+// (forward, 16384 x 4096 bf16: 20 an element one by one, 0.75 of the issue slots, 54 us)
+using Two = uint64_t;
+
+__device__ __forceinline__ Two two(float a, float b)
 {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1)
-  {
-    v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, off);
-    v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, off);
-  }
-  if constexpr (WARPS > 1)
-  {
-    if ((threadIdx.x & 31) == 0)
-    {
-      slots[(threadIdx.x >> 5) % WARPS] = v;
-    }
-    __syncthreads();
-    v = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-    {
-      v.x += slots[w].x;
-      v.y += slots[w].y;
-    }
-  }
-  return v;
+  return static_cast<Two>(__float_as_uint(a)) | (static_cast<Two>(__float_as_uint(b)) << 32);
+}
+__device__ __forceinline__ float first_of(Two v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float second_of(Two v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+__device__ __forceinline__ Two add2(Two a, Two b)
+{
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b)
+{
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
+{
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
 }
 
-template <int WARPS>
-__device__ __forceinline__ float one_sum_of(float v, float *slots)
+// sums of N values a thread over WARPS warps, every thread gets them; `slots` [N][WARPS] must not be in use by an earlier sum
+// that a barrier of these threads has not closed
+template <int WARPS, int N>
+__device__ __forceinline__ void sums_of(float (&v)[N], float (*slots)[WARPS])
 {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1)
   {
-    v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+    {
+      v[n] += __shfl_xor_sync(0xFFFFFFFFu, v[n], off);
+    }
   }
   if constexpr (WARPS > 1)
   {
     if ((threadIdx.x & 31) == 0)
     {
-      slots[(threadIdx.x >> 5) % WARPS] = v;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+      {
+        slots[n][(threadIdx.x >> 5) % WARPS] = v[n];
+      }
     }
     __syncthreads();
-    v = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w)
+    for (int n = 0; n < N; ++n)
     {
-      v += slots[w];
+      if constexpr (WARPS >= 4)
+      {
+        const float4 *p = reinterpret_cast<const float4 *>(slots[n]);
+        float4 s = p[0];
+#pragma unroll
+        for (int w = 1; w < WARPS / 4; ++w)
+        {
+          const float4 o = p[w];
+          s.x += o.x;
+          s.y += o.y;
+          s.z += o.z;
+          s.w += o.w;
+        }
+        v[n] = (s.x + s.y) + (s.z + s.w);
+      }
+      else
+      {
+        v[n] = slots[n][0] + slots[n][1];
+      }
     }
   }
-  return v;
+}
+
+// 1 / sqrt(v): the approximation and one step of Newton's method, except where the step would meet 0 * infinity
+__device__ __forceinline__ float inverse_root(float v)
+{
+  const float r = rsqrtf(v);
+  const float better = fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r);
+  return v > 0.0f && v < __int_as_float(0x7F800000) ? better : r;
 }
 
 // the rows of N tensors that a block walks over: start() once, then next() for each row in turn gives this thread's pieces
@@ -478,8 +518,10 @@ struct RowsAhead
     }
   }
 
-  __device__ __forceinline__ void next(Piece (&out)[N][P])
+  // the row's values of this thread in pairs; zeros where the thread has no column, or the block no row
+  __device__ __forceinline__ void next(Two (&out)[N][P * V / 2], bool live)
   {
+    Piece piece[N][P];
     if constexpr (V > 1)
     {
       // (the ring row before this one, which this thread has read, is filled again)
@@ -491,8 +533,12 @@ struct RowsAhead
 #pragma unroll
         for (int j = 0; j < P; ++j)
         {
-          const uint4 v = ring[((at * N + n) * P + j) * BLOCK + threadIdx.x];
-          out[n][j] = *reinterpret_cast<const Piece *>(&v);
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (live && (t + j * THREADS) * V < dim)
+          {
+            v = ring[((at * N + n) * P + j) * BLOCK + threadIdx.x];
+          }
+          pairs_of(out[n] + j * (V / 2), v);
         }
       }
       at = at == RING - 1 ? 0 : at + 1;
@@ -503,14 +549,83 @@ struct RowsAhead
       for (int n = 0; n < N; ++n)
       {
 #pragma unroll
-        for (int j = 0; j < P; ++j)
+        for (int j = 0; j < P; j += 2)
         {
-          out[n][j] = ahead[n][j];
+          out[n][j / 2] = two(live && t + j * THREADS < dim ? to_f<T>(ahead[n][j].e[0]) : 0.0f,
+                              live && t + (j + 1) * THREADS < dim ? to_f<T>(ahead[n][j + 1].e[0]) : 0.0f);
         }
       }
       fetch(0);
     }
   }
+
+  static __device__ __forceinline__ void pairs_of(Two *out, const uint4 &v)
+  {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (sizeof(T) == 4)
+    {
+      out[0] = static_cast<Two>(w[0]) | (static_cast<Two>(w[1]) << 32);
+      out[1] = static_cast<Two>(w[2]) | (static_cast<Two>(w[3]) << 32);
+    }
+    else
+    {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+      {
+        const LnPiece<T, 2> p = *reinterpret_cast<const LnPiece<T, 2> *>(&w[i]);
+        out[i] = two(to_f<T>(p.e[0]), to_f<T>(p.e[1]));
+      }
+    }
+  }
+
+  // the row's results
+  __device__ __forceinline__ void store(T *row_out, const Two (&v)[P * V / 2]) const
+  {
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      const int c = (t + j * THREADS) * V;
+      if (c < dim)
+      {
+        Piece o;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          const int e = j * V + i;
+          o.e[i] = from_f<T>((e & 1) != 0 ? second_of(v[e / 2]) : first_of(v[e / 2]));
+        }
+        *reinterpret_cast<Piece *>(row_out + c) = o;
+      }
+    }
+  }
+
+  // fp32 values of this thread's columns; `other` without a vector, zeros where the thread has no column
+  __device__ __forceinline__ void columns(Two (&out)[P * V / 2], const float *p, float other) const
+  {
+    float f[P][V];
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+    {
+      const int c = (t + j * THREADS) * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        f[j][i] = 0.0f;
+      }
+      if (c < dim)
+      {
+        load_floats<T, V>(f[j], p != nullptr ? p + c : nullptr, other);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < P * V; e += 2)
+    {
+      out[e / 2] = two(f[e / V][e % V], f[(e + 1) / V][(e + 1) % V]);
+    }
+  }
+
+  // whether element e of the thread is a column
+  __device__ __forceinline__ bool has(int e) const { return (t + (e / V) * THREADS) * V < dim; }
 };
 
 template <typename T, int V, int P, int WARPS>
@@ -521,16 +636,16 @@ layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const flo
   constexpr int BLOCK = kLnBlock<WARPS, 256>;
   constexpr int SLOTS = BLOCK / (WARPS * 32);
   constexpr int THREADS = WARPS * 32;
+  constexpr int PAIRS = P * V / 2;
   extern __shared__ uint4 ln_ring[];
-  __shared__ float sums[2][2][SLOTS][WARPS];
+  __shared__ __align__(16) float sums[2][2][SLOTS][1][WARPS];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(beta)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  using Rows = RowsAhead<T, V, P, THREADS, BLOCK, 1>;
   const int slot = threadIdx.x / THREADS;
   const int t = threadIdx.x % THREADS;
   const int first = static_cast<int>(blockIdx.x) * SLOTS;
   const int step = static_cast<int>(gridDim.x) * SLOTS;
-  Rows in;
+  RowsAhead<T, V, P, THREADS, BLOCK, 1> in;
   in.src[0] = x;
   in.row = first + slot;
   in.step = step;
@@ -539,72 +654,54 @@ layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const flo
   in.t = t;
   in.ring = ln_ring;
   in.start();
-  float g[P][V], b[P][V];
-#pragma unroll
-  for (int j = 0; j < P; ++j)
-  {
-    const int c = (t + j * THREADS) * V;
-    if (c < dim)
-    {
-      load_floats<T, V>(g[j], gamma != nullptr ? gamma + c : nullptr, 1.0f);
-      load_floats<T, V>(b[j], beta != nullptr ? beta + c : nullptr, 0.0f);
-    }
-  }
+  Two g[PAIRS], b[PAIRS];
+  in.columns(g, gamma, 1.0f);
+  in.columns(b, beta, 0.0f);
+  const bool ragged = dim < THREADS * P * V;
+  const float inverse = 1.0f / static_cast<float>(dim);
   int turn = 0;
   for (int64_t base = first; base < rows; base += step, turn ^= 1)   // (every slot takes part in the sums' barriers)
   {
     const int64_t r = base + slot;
     const bool live = r < rows;
-    LnPiece<T, V> v[1][P];
-    in.next(v);
-    float s = 0.0f;
+    Two v[1][PAIRS];
+    in.next(v, live);
+    Two a = v[0][0];
 #pragma unroll
-    for (int j = 0; j < P; ++j)
+    for (int i = 1; i < PAIRS; ++i)
     {
-      if (live && (t + j * THREADS) * V < dim)
-      {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-        {
-          s += to_f<T>(v[0][j].e[i]);
-        }
-      }
+      a = add2(a, v[0][i]);
     }
-    const float mean = one_sum_of<WARPS>(s, sums[turn][0][slot]) / static_cast<float>(dim);
-    s = 0.0f;
+    float s[1] = {first_of(a) + second_of(a)};
+    sums_of<WARPS>(s, sums[turn][0][slot]);
+    const float mean = s[0] * inverse;
+    a = two(0.0f, 0.0f);
 #pragma unroll
-    for (int j = 0; j < P; ++j)
+    for (int i = 0; i < PAIRS; ++i)
     {
-      if (live && (t + j * THREADS) * V < dim)
+      v[0][i] = add2(v[0][i], two(-mean, -mean));
+      if (ragged)
       {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-        {
-          const float d = to_f<T>(v[0][j].e[i]) - mean;
-          s = fmaf(d, d, s);
-        }
+        v[0][i] = two(in.has(2 * i) ? first_of(v[0][i]) : 0.0f, in.has(2 * i + 1) ? second_of(v[0][i]) : 0.0f);
       }
+      a = fma2(v[0][i], v[0][i], a);
     }
-    const float rstd = 1.0f / sqrtf(one_sum_of<WARPS>(s, sums[turn][1][slot]) / static_cast<float>(dim) + epsilon);
+    s[0] = first_of(a) + second_of(a);
+    sums_of<WARPS>(s, sums[turn][1][slot]);
+    const float rstd = inverse_root(fmaf(s[0], inverse, epsilon));
 #pragma unroll
-    for (int j = 0; j < P; ++j)
+    for (int i = 0; i < PAIRS; ++i)
     {
-      const int c = (t + j * THREADS) * V;
-      if (live && c < dim)
+      v[0][i] = fma2(mul2(v[0][i], two(rstd, rstd)), g[i], b[i]);
+    }
+    if (live)
+    {
+      in.store(y + r * dim, v[0]);
+      if (t == 0)
       {
-        LnPiece<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-        {
-          o.e[i] = from_f<T>(fmaf((to_f<T>(v[0][j].e[i]) - mean) * rstd, g[j][i], b[j][i]));
-        }
-        *reinterpret_cast<LnPiece<T, V> *>(y + r * dim + c) = o;
+        mean_out[r] = mean;
+        rstd_out[r] = rstd;
       }
-    }
-    if (live && t == 0)
-    {
-      mean_out[r] = mean;
-      rstd_out[r] = rstd;
     }
   }
 }
@@ -612,15 +709,16 @@ layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const flo
 // dx and this block's share of dgamma and dbeta in one pass: a thread keeps its columns' sums over all rows of the block.
 // part[block][0][c], part[block][1][c] as in layernorm_columns_kernel.
 template <typename T, int V, int P, int WARPS>
-__global__ void __launch_bounds__(kLnBlock<WARPS, 256>)
+__global__ void __launch_bounds__(kLnBlock<WARPS, 256>, WARPS <= 8 ? 2 : 1)
 layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gamma, const float *__restrict__ mean_in,
                           const float *__restrict__ rstd_in, T *dx, float *__restrict__ part, int rows, int dim)
 {
   constexpr int BLOCK = kLnBlock<WARPS, 256>;
   constexpr int SLOTS = BLOCK / (WARPS * 32);
   constexpr int THREADS = WARPS * 32;
+  constexpr int PAIRS = P * V / 2;
   extern __shared__ uint4 ln_ring[];   // the ring; then, where SLOTS > 1, the columns' sums [2][dim]
-  __shared__ float2 sums[2][SLOTS][WARPS];
+  __shared__ __align__(16) float sums[2][SLOTS][2][WARPS];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(mean_in), "+l"(rstd_in)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   using Rows = RowsAhead<T, V, P, THREADS, BLOCK, 2>;
@@ -638,77 +736,61 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
   in.t = t;
   in.ring = ln_ring;
   in.start();
-  float g[P][V], sg[P][V], sb[P][V];
+  Two g[PAIRS], sg[PAIRS], sb[PAIRS];
+  in.columns(g, gamma, 1.0f);
 #pragma unroll
-  for (int j = 0; j < P; ++j)
+  for (int i = 0; i < PAIRS; ++i)
   {
-    const int c = (t + j * THREADS) * V;
-    if (c < dim)
-    {
-      load_floats<T, V>(g[j], gamma != nullptr ? gamma + c : nullptr, 1.0f);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-    {
-      sg[j][i] = sb[j][i] = 0.0f;
-    }
+    sg[i] = sb[i] = two(0.0f, 0.0f);
   }
-  float next_mean = 0.0f, next_rstd = 0.0f;
-  if (first + slot < rows)
+  const float inverse = 1.0f / static_cast<float>(dim);
+  // the statistics of this row and the two after it
+  float means[3], rstds[3];
+  auto statistics = [&](int64_t r, float &m, float &s) {
+    m = r < rows ? mean_in[r] : 0.0f;
+    s = r < rows ? rstd_in[r] : 0.0f;
+  };
+  for (int i = 0; i < 3; ++i)
   {
-    next_mean = mean_in[first + slot];
-    next_rstd = rstd_in[first + slot];
+    statistics(first + slot + i * static_cast<int64_t>(step), means[i], rstds[i]);
   }
   int turn = 0;
   for (int64_t base = first; base < rows; base += step, turn ^= 1)   // (every slot takes part in the sums' barriers)
   {
     const int64_t r = base + slot;
     const bool live = r < rows;
-    LnPiece<T, V> v[2][P];
-    in.next(v);
-    const float mean = next_mean, rstd = next_rstd;
-    if (r + step < rows)
+    Two v[2][PAIRS];   // x, then x_hat; dy, then dy * gamma
+    in.next(v, live);
+    const float mean = means[0];
+    const float rstd = rstds[0];
+    means[0] = means[1];
+    rstds[0] = rstds[1];
+    means[1] = means[2];
+    rstds[1] = rstds[2];
+    statistics(r + 3 * static_cast<int64_t>(step), means[2], rstds[2]);
+    Two a = two(0.0f, 0.0f), b = two(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i)
     {
-      next_mean = mean_in[r + step];
-      next_rstd = rstd_in[r + step];
+      v[0][i] = mul2(add2(v[0][i], two(-mean, -mean)), two(rstd, rstd));
+      sg[i] = fma2(v[1][i], v[0][i], sg[i]);
+      sb[i] = add2(sb[i], v[1][i]);
+      v[1][i] = mul2(v[1][i], g[i]);
+      a = add2(a, v[1][i]);
+      b = fma2(v[1][i], v[0][i], b);
     }
-    float2 s = make_float2(0.0f, 0.0f);
+    float s[2] = {first_of(a) + second_of(a), first_of(b) + second_of(b)};
+    sums_of<WARPS>(s, sums[turn][slot]);
+    const float s1 = -s[0] * inverse;
+    const float s2 = -s[1] * inverse;
 #pragma unroll
-    for (int j = 0; j < P; ++j)
+    for (int i = 0; i < PAIRS; ++i)
     {
-      if (live && (t + j * THREADS) * V < dim)
-      {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-        {
-          const float d = to_f<T>(v[1][j].e[i]);
-          const float xh = (to_f<T>(v[0][j].e[i]) - mean) * rstd;
-          const float w = d * g[j][i];
-          s.x += w;
-          s.y = fmaf(w, xh, s.y);
-          sg[j][i] = fmaf(d, xh, sg[j][i]);
-          sb[j][i] += d;
-        }
-      }
+      v[1][i] = mul2(fma2(v[0][i], two(s2, s2), add2(v[1][i], two(s1, s1))), two(rstd, rstd));
     }
-    s = sums_of<WARPS>(s, sums[turn][slot]);
-    const float s1 = s.x / static_cast<float>(dim);
-    const float s2 = s.y / static_cast<float>(dim);
-#pragma unroll
-    for (int j = 0; j < P; ++j)
+    if (live)
     {
-      const int c = (t + j * THREADS) * V;
-      if (live && c < dim)
-      {
-        LnPiece<T, V> o;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-        {
-          const float xh = (to_f<T>(v[0][j].e[i]) - mean) * rstd;
-          o.e[i] = from_f<T>(rstd * (to_f<T>(v[1][j].e[i]) * g[j][i] - s1 - xh * s2));
-        }
-        *reinterpret_cast<LnPiece<T, V> *>(dx + r * dim + c) = o;
-      }
+      in.store(dx + r * dim, v[1]);
     }
   }
   if (part == nullptr)
@@ -719,22 +801,20 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
   float *mine = part + static_cast<int64_t>(blockIdx.x) * 2 * dim;
   float *to = SLOTS > 1 ? columns : mine;
 #pragma unroll 1
-  for (int i = 0; i < SLOTS; ++i)   // slot by slot, in order
+  for (int turns = 0; turns < SLOTS; ++turns)   // slot by slot, in order
   {
-    if (slot == i)
+    if (slot == turns)
     {
 #pragma unroll
-      for (int j = 0; j < P; ++j)
+      for (int e = 0; e < P * V; ++e)
       {
-        const int c = (t + j * THREADS) * V;
+        const int c = (t + (e / V) * THREADS) * V + e % V;
         if (c < dim)
         {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-          {
-            to[c + e] = i > 0 ? to[c + e] + sg[j][e] : sg[j][e];
-            to[dim + c + e] = i > 0 ? to[dim + c + e] + sb[j][e] : sb[j][e];
-          }
+          const float vg = (e & 1) != 0 ? second_of(sg[e / 2]) : first_of(sg[e / 2]);
+          const float vb = (e & 1) != 0 ? second_of(sb[e / 2]) : first_of(sb[e / 2]);
+          to[c] = turns > 0 ? to[c] + vg : vg;
+          to[dim + c] = turns > 0 ? to[dim + c] + vb : vb;
         }
       }
     }
@@ -842,31 +922,34 @@ int ln_fwd(const void *xv, const float *gamma, const float *beta, void *yv, floa
   const T *x = static_cast<const T *>(xv);
   T *y = static_cast<T *>(yv);
   constexpr int V = 16 / static_cast<int>(sizeof(T));
+  // (gamma and beta of 16 columns a thread fit the registers; of eight where every column has an address of its own)
   if ((dim % V) == 0 && on_16(x) && on_16(y) && on_16(gamma) && on_16(beta))
   {
 #define CAIFQ_LN_CALL(W) ln_fwd_many<T, V, 16 / V, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
-    if (rows > 148)
-    {
-      CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
-    }
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
 #undef CAIFQ_LN_CALL
-#define CAIFQ_LN_CALL(W) ln_fwd_rows<T, V, 4, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
-    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 4 * V)
+    if (sizeof(T) == 2 && dim <= 512 * 4 * V)
+    {
+      return ln_fwd_rows<T, V, 4, 16>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
+    }
     if (dim <= 1024 * 4 * V)
     {
-      return CAIFQ_LN_CALL(32);
+      return ln_fwd_rows<T, V, 4, 32>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
     }
-#undef CAIFQ_LN_CALL
   }
   else
   {
-#define CAIFQ_LN_CALL(W) ln_fwd_rows<T, 1, 16, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
-    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+#define CAIFQ_LN_CALL(W) ln_fwd_many<T, 1, 8, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 8)
+#undef CAIFQ_LN_CALL
+    if (dim <= 512 * 16)
+    {
+      return ln_fwd_rows<T, 1, 16, 16>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
+    }
     if (dim <= 1024 * 16)
     {
-      return CAIFQ_LN_CALL(32);
+      return ln_fwd_rows<T, 1, 16, 32>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
     }
-#undef CAIFQ_LN_CALL
   }
   CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s, x, gamma, beta, y,
                                     mean, rstd, epsilon, rows, static_cast<int64_t>(dim)));
@@ -880,7 +963,7 @@ int ln_bwd_rows(const T *dy, const T *x, const float *gamma, const float *mean, 
   constexpr int BLOCK = kLnBlock<WARPS, 256>;
   constexpr int SLOTS = BLOCK / (WARPS * 32);
   constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 2>::kBytes;
-  constexpr size_t kColumns = SLOTS > 1 ? sizeof(float) * 2 * 16 * WARPS * 32 : 0;   // of the widest row
+  constexpr size_t kColumns = SLOTS > 1 ? sizeof(float) * 2 * P * V * WARPS * 32 : 0;   // of the widest row
   static std::atomic<uint64_t> done{0};
   if (kBytes + kColumns > kLnPlainSmem)
   {
@@ -912,9 +995,13 @@ int ln_bwd(const void *dyv, const void *xv, const float *gamma, const float *mea
   }
   else
   {
-#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, 1, 16, W>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
-    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, 1, 8, W>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 8)
 #undef CAIFQ_LN_CALL
+    if (dim <= 512 * 16)
+    {
+      return ln_bwd_rows<T, 1, 16, 16>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s);
+    }
   }
   *slices = ln_slices(rows);
   if (part != nullptr)
@@ -982,7 +1069,7 @@ int launch_layernorm_bwd(const void *dy, const void *x, const float *gamma, cons
   }
   if (columns)
   {
-    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_finish_kernel, dim3((dim + 31) / 32, 2), dim3(kLnThreads), 0, s,
+    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_finish_kernel, dim3((dim + 31) / 32, 2), dim3(1024), 0, s,
                                       static_cast<const float *>(workspace), grad_gamma, grad_beta, slices,
                                       static_cast<int64_t>(dim), accumulate));
   }
