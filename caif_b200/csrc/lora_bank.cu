@@ -5,7 +5,7 @@
 // Rows need no order.  The adapters lie in a table in device memory that the kernels read, so a batch is described by the
 // rows' indices alone and a captured call follows them.  A row whose index is outside the table gets zeros here; what its
 // x or another adapter's factors hold (infinities, NaN) never reaches it, since rows are selected, not multiplied by zero.
-#include "common.cuh"
+#include "umma.cuh"
 
 namespace caifq
 {
@@ -120,6 +120,316 @@ bank_up_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, const
   y[row * out_dim + col] = bank_t<T>(v);
 }
 
+// ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on 16 rows of the batch as they lie ----
+// A block takes 16 neighbouring rows and goes through the adapters that they name, one after the other (gridDim blocks share
+// them).  The rows of a prompt share one adapter, 16 decoding sequences may name 16: their factors are read once a tile in
+// either case, and no sorting of rows, and no launch for it, comes before.  Each adapter's product has accumulators of its
+// own and is stored for its own rows alone.
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1)
+{
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// the adapters of 16 rows: ids[i] of row i (-1: none); returns the rows at which one appears for the first time
+__device__ __forceinline__ uint32_t first_rows(const int (&ids)[16])
+{
+  const int lane = threadIdx.x & 31;
+  const int id = lane < 16 ? ids[lane] : -1;
+  const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
+  return __ballot_sync(0xFFFFFFFFu, id >= 0 && (same & ((1u << lane) - 1u)) == 0u);
+}
+
+__device__ __forceinline__ void load_ids(int (&ids)[16], const int32_t *adapter_of_row, int64_t row0, int64_t m, int count)
+{
+  if (threadIdx.x < 16)
+  {
+    const int64_t row = row0 + threadIdx.x;
+    const int id = row < m ? adapter_of_row[row] : -1;
+    ids[threadIdx.x] = id < count ? (id < 0 ? -1 : id) : -1;
+  }
+  __syncthreads();
+}
+
+// h of 16 rows.  As in the adapter's own thin product, a lane streams 16 bytes of two rows of x and of a row of A per 32
+// columns straight into fragments (the order of the columns inside a fragment is the same for both); the eight warps split
+// the columns, and so do the blocks of a cluster where there are few rows.
+template <int NT>   // eights of the largest rank
+__global__ void __launch_bounds__(256)
+bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter_of_row,
+                     const caifq_lora_entry *__restrict__ entries, int count, float *h, int ld, int64_t m, int in_dim,
+                     int cluster)
+{
+  __shared__ float part[8][16][NT * 8 + 1];
+  __shared__ int ids[16];
+  // (what invariant loads read is addressed out of the wait, so that they stay behind it)
+  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int rank_in_cluster = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / cluster) * 16;
+  load_ids(ids, adapter_of_row, row0, m, count);
+  uint32_t firsts = first_rows(ids);
+  const int steps = in_dim / 32;
+  const int begin = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp) / (8 * cluster));
+  const int end = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp + 1) / (8 * cluster));
+  const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
+  // (ids has the same content in all blocks of a cluster, so they run the same turns)
+  for (int turn = 0; firsts != 0u; ++turn, firsts &= firsts - 1u)
+  {
+    if (turn % static_cast<int>(gridDim.y) != static_cast<int>(blockIdx.y))
+    {
+      continue;
+    }
+    const int id = ids[__ffs(static_cast<int>(firsts)) - 1];
+    const int eights = entries[id].rank / 8;
+    const __nv_bfloat16 *a = static_cast<const __nv_bfloat16 *>(entries[id].a);
+    const bool lo = ids[g] == id;
+    const bool hi = ids[g + 8] == id;
+    const uint4 *x_lo = reinterpret_cast<const uint4 *>(x + (lo ? row0 + g : 0) * in_dim) + t;
+    const uint4 *x_hi = reinterpret_cast<const uint4 *>(x + (hi ? row0 + g + 8 : 0) * in_dim) + t;
+    const uint4 *a_row = reinterpret_cast<const uint4 *>(a + static_cast<int64_t>(g) * in_dim) + t;
+    float c[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+    {
+      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+    }
+#pragma unroll 4
+    for (int st = begin; st < end; ++st)
+    {
+      const uint4 xa = lo ? __ldg(x_lo + st * 4) : zero4;
+      const uint4 xb = hi ? __ldg(x_hi + st * 4) : zero4;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+      {
+        if (nt < eights)
+        {
+          const uint4 w = __ldg(a_row + static_cast<int64_t>(nt) * in_dim + st * 4);
+          mma_16816(c[nt], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+          mma_16816(c[nt], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+    {
+      part[warp][g][nt * 8 + 2 * t] = c[nt][0];
+      part[warp][g][nt * 8 + 2 * t + 1] = c[nt][1];
+      part[warp][g + 8][nt * 8 + 2 * t] = c[nt][2];
+      part[warp][g + 8][nt * 8 + 2 * t + 1] = c[nt][3];
+    }
+    __syncthreads();
+    // the block's eight partial tiles become one, in the first of them (an element is one thread's)
+    for (int e = threadIdx.x; e < 16 * NT * 8; e += 256)
+    {
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w)
+      {
+        v += part[w][e / (NT * 8)][e % (NT * 8)];
+      }
+      part[0][e / (NT * 8)][e % (NT * 8)] = v;
+    }
+    if (cluster > 1)
+    {
+      cluster_sync_all();
+    }
+    else
+    {
+      __syncthreads();
+    }
+    const int share = 16 / cluster;
+    for (int e = threadIdx.x; e < share * NT * 8; e += 256)
+    {
+      const int rr = rank_in_cluster * share + e / (NT * 8);
+      const int col = e % (NT * 8);
+      if (ids[rr] == id && col < eights * 8)
+      {
+        float v = part[0][rr][col];
+        if (cluster > 1)
+        {
+          v = 0.0f;
+          const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(&part[0][rr][col]));
+          for (int b = 0; b < cluster; ++b)
+          {
+            v += __uint_as_float(ld_shared_cluster(map_to_cta(mine, static_cast<uint32_t>(b))));
+          }
+        }
+        h[(row0 + rr) * ld + col] = v;
+      }
+    }
+    // nobody's partial tile is written again, or left, while it is read
+    if (cluster > 1)
+    {
+      cluster_sync_all();
+    }
+    else
+    {
+      __syncthreads();
+    }
+  }
+}
+
+// y of 16 rows and 128 columns: a warp 32 columns.  h enters as two bf16 terms (2^-16 relative).  The columns of a warp's four
+// 8-wide tiles are dealt out so that a lane ends with eight neighbouring ones of a row: 16-byte stores.
+__global__ void __launch_bounds__(128)
+bank_up_mma_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries,
+                   int count, __nv_bfloat16 *y, int ld, int64_t m, int out_dim)
+{
+  __shared__ int ids[16];
+  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int col0 = static_cast<int>(blockIdx.y) * 128 + static_cast<int>(threadIdx.x >> 5) * 32;
+  load_ids(ids, adapter_of_row, row0, m, count);
+  uint32_t firsts = first_rows(ids);
+  const bool stores = col0 + 8 * t < out_dim;
+  const int n0 = col0 + 8 * (g >> 1) + (g & 1);   // the column whose row of B this lane feeds, plus 2 * tile
+  for (int turn = 0; firsts != 0u; ++turn, firsts &= firsts - 1u)
+  {
+    if (turn % static_cast<int>(gridDim.z) != static_cast<int>(blockIdx.z))
+    {
+      continue;
+    }
+    const int id = ids[__ffs(static_cast<int>(firsts)) - 1];
+    const int rank = entries[id].rank;
+    const float scale = entries[id].scale;
+    const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entries[id].b);
+    const bool mine[2] = {ids[g] == id, ids[g + 8] == id};
+    float c[4][4];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+    {
+      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+    }
+#pragma unroll 1
+    for (int k = 0; k < rank; k += 16)
+    {
+      const int kk = k + 4 * t;
+      uint2 w[4];
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+      {
+        w[nt] = make_uint2(0u, 0u);
+        if (kk < rank && n0 + 2 * nt < out_dim)
+        {
+          w[nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n0 + 2 * nt) * rank + kk));
+        }
+      }
+      uint32_t top[2][2], rest[2][2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+      {
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (mine[half] && kk < rank)
+        {
+          v = *reinterpret_cast<const float4 *>(h + (row0 + g + 8 * half) * ld + kk);
+        }
+        const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+          top[half][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
+          const float r0 = f[2 * i] - __uint_as_float(top[half][i] << 16);
+          const float r1 = f[2 * i + 1] - __uint_as_float(top[half][i] & 0xFFFF0000u);
+          // (an infinity has no second term)
+          rest[half][i] = pack_bf16x2(isfinite(f[2 * i]) ? r0 : 0.0f, isfinite(f[2 * i + 1]) ? r1 : 0.0f);
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+      {
+        mma_16816(c[nt], top[0][0], top[1][0], top[0][1], top[1][1], w[nt].x, w[nt].y);
+        mma_16816(c[nt], rest[0][0], rest[1][0], rest[0][1], rest[1][1], w[nt].x, w[nt].y);
+      }
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      if (mine[half] && stores)
+      {
+        uint4 o;
+        o.x = pack_bf16x2(c[0][2 * half] * scale, c[0][2 * half + 1] * scale);
+        o.y = pack_bf16x2(c[1][2 * half] * scale, c[1][2 * half + 1] * scale);
+        o.z = pack_bf16x2(c[2][2 * half] * scale, c[2][2 * half + 1] * scale);
+        o.w = pack_bf16x2(c[3][2 * half] * scale, c[3][2 * half + 1] * scale);
+        *reinterpret_cast<uint4 *>(y + (row0 + g + 8 * half) * out_dim + col0 + 8 * t) = o;
+      }
+    }
+  }
+  if (blockIdx.z == 0 && stores)
+  {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      const int64_t row = row0 + g + 8 * half;
+      if (row < m && ids[g + 8 * half] < 0)
+      {
+        *reinterpret_cast<uint4 *>(y + row * out_dim + col0 + 8 * t) = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+}
+
+// blocks that share a tile's adapters: as many as keep the launch near `most` blocks, and no more than there can be adapters
+int bank_shares(int64_t blocks, int64_t most, int64_t m, int count)
+{
+  int64_t n = most / blocks;
+  n = n > 16 ? 16 : n;
+  n = n > m ? m : n;
+  n = n > count ? count : n;
+  return static_cast<int>(n < 1 ? 1 : n);
+}
+
+int bank_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
+             cudaStream_t s)
+{
+  const int64_t tiles = (m + 15) / 16;
+  const int shares = bank_shares(tiles, 4 * 148, m, bank.count);
+  // blocks of a cluster: as in the adapter's own thin product, with at least two steps of 32 columns for every warp
+  int cluster = 1;
+  while (cluster < 8 && tiles * shares * cluster < 4 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
+  {
+    cluster *= 2;
+  }
+  void (*down)(const __nv_bfloat16 *, const int32_t *, const caifq_lora_entry *, int, float *, int, int64_t, int, int) =
+      bank.max_rank <= 8 ? bank_down_mma_kernel<1>
+                         : (bank.max_rank <= 16 ? bank_down_mma_kernel<2>
+                                                : (bank.max_rank <= 32 ? bank_down_mma_kernel<4> : bank_down_mma_kernel<8>));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * cluster), static_cast<unsigned>(shares));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launches() ? 2 : 1;
+  CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, down, static_cast<const __nv_bfloat16 *>(x), adapter_of_row, bank.entries,
+                                      bank.count, h, bank.max_rank, m, bank.in_dim, cluster));
+  const int64_t columns = (bank.out_dim + 127) / 128;
+  CAIFQ_CHECK_CUDA(launch_dependent(bank_up_mma_kernel,
+                                    dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(columns),
+                                         static_cast<unsigned>(bank_shares(tiles * columns, 16 * 148, m, bank.count))),
+                                    dim3(128), 0, s, static_cast<const float *>(h), adapter_of_row, bank.entries, bank.count,
+                                    static_cast<__nv_bfloat16 *>(y), bank.max_rank, m, bank.out_dim));
+  return CAIFQ_OK;
+}
+
 template <typename T>
 int bank_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
                  cudaStream_t s)
@@ -140,6 +450,13 @@ int bank_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, con
 int launch_lora_bank(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
                      cudaStream_t s)
 {
+  // (16-byte loads of x and stores of y; m, so that the grid's first dimension holds it with the clusters)
+  if (bank.dtype == CAIFQ_BF16 && bank.vectors != 0 && bank.max_rank <= 64 && (bank.max_rank % 8) == 0 && (bank.in_dim % 32) == 0 &&
+      (bank.out_dim % 8) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0 &&
+      bank.out_dim <= 65535 * 128)
+  {
+    return bank_mma(bank, adapter_of_row, x, m, y, h, s);
+  }
   switch (bank.dtype)
   {
     case CAIFQ_F32:
