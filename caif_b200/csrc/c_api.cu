@@ -130,8 +130,10 @@ int launch_rmsnorm_fwd(const void *input, const float *gamma, void *output, floa
 int launch_rmsnorm_bwd(const void *grad_output, const void *input, const float *gamma, const float *rms_cache,
                        void *grad_input, float *grad_gamma, int dtype, int rows, int dim, cudaStream_t s);
 // lora_bank.cu
-int launch_lora_bank(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
-                     cudaStream_t s);
+int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h,
+                          cudaStream_t s);
+int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h,
+                        int64_t m, void *y, cudaStream_t s);
 // act8.cu
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
@@ -1111,9 +1113,24 @@ int check_bank(const caifq_weight *w, const caifq_lora_bank *bank, const char *w
   return CAIFQ_OK;
 }
 
-size_t bank_hidden_bytes(const caifq_lora_bank *bank, int64_t m)
+struct BankWs
 {
-  return align256(static_cast<size_t>(m) * static_cast<size_t>(bank->max_rank) * sizeof(float));
+  size_t frozen;   // fp32 [m, out], unless y is fp32
+  size_t weight;   // the expanded weight, where there is one
+  size_t total;
+};
+
+BankWs bank_ws(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m, int compute_dtype)
+{
+  BankWs o{};
+  o.frozen = align256(static_cast<size_t>(m) * static_cast<size_t>(bank->max_rank) * sizeof(float));
+  o.weight = o.frozen + (bank->dtype == CAIFQ_F32
+                             ? 0
+                             : align256(static_cast<size_t>(m) * static_cast<size_t>(w->out_dim) * sizeof(float)));
+  o.total = o.weight + (expand_linear_ok(w, false, kAlignedProbe, bank->dtype, m, kAlignedProbe, CAIFQ_F32, compute_dtype)
+                            ? expanded_weight_bytes(w)
+                            : 0);
+  return o;
 }
 }  // namespace
 
@@ -1156,10 +1173,7 @@ size_t caifq_lora_bank_workspace_bytes(const caifq_weight *w, const caifq_lora_b
   {
     return 0;
   }
-  return bank_hidden_bytes(bank, m) +
-         (expand_linear_ok(w, false, kAlignedProbe, bank->dtype, m, kAlignedProbe, bank->dtype, compute_dtype)
-              ? expanded_weight_bytes(w)
-              : 0);
+  return bank_ws(w, bank, m, compute_dtype).total;
 }
 
 int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *bank, const int32_t *adapter_of_row,
@@ -1186,25 +1200,20 @@ int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *ban
   CAIFQ_CHECK_ARG(!overlap(x, elem * static_cast<size_t>(m) * w->in_dim, y, elem * static_cast<size_t>(m) * w->out_dim),
                   "%s: x and y overlap", who);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const BankWs ws = bank_ws(w, bank, m, compute_dtype);
+  char *base = static_cast<char *>(workspace);
   float *h = static_cast<float *>(workspace);
-  int r = launch_lora_bank(*bank, adapter_of_row, x, m, y, h, s);
-  if (r != CAIFQ_OK)
+  float *frozen = static_cast<float *>(bank->dtype == CAIFQ_F32 ? y : static_cast<void *>(base + ws.frozen));
+  int r = launch_lora_bank_down(*bank, adapter_of_row, x, m, h, s);
+  if (r == CAIFQ_OK)
   {
-    return r;
+    r = linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who);
   }
-  if (expand_linear_ok(w, false, x, bank->dtype, m, y, bank->dtype, compute_dtype))
+  if (r == CAIFQ_OK)
   {
-    void *wb = static_cast<char *>(workspace) + bank_hidden_bytes(bank, m);
-    r = launch_expand_prepare(*w, wb, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, s);
-    if (r != CAIFQ_OK)
-    {
-      return r;
-    }
-    const caifq_weight wbf = float_weight(wb, CAIFQ_BF16, w->out_dim, w->in_dim);
-    return linear_any(&wbf, false, x, bank->dtype, 1.0f, m, y, bank->dtype, true, compute_dtype, s, who, nullptr, nullptr,
-                      epilogue_scale_ptr(w));
+    r = launch_lora_bank_up(*bank, adapter_of_row, frozen, h, m, y, s);
   }
-  return linear_any(w, false, x, bank->dtype, 1.0f, m, y, bank->dtype, true, compute_dtype, s, who);
+  return r;
 }
 
 // ------------------------------------------------- activations kept in 8 bits

@@ -1,10 +1,15 @@
 // Low-rank adapters of many requests beside one frozen projection: row t of the batch takes adapter a = adapter_of_row[t],
 //   y[t] = x[t] . W^T + scale_a (x[t] . A_a^T) . B_a^T
-// Two kernels write the adapters' part into y, and the frozen product then adds itself to it in its own epilogue:
-//   down: h[t, :] = x[t] . A_a^T, fp32        up: y[t, :] = scale_a h[t, :] . B_a^T, rounded once
+//   down: h[t, :] = x[t] . A_a^T, fp32
+//   the frozen product, fp32
+//   up: y[t, :] = frozen[t, :] + scale_a h[t, :] . B_a^T, rounded once
+// Why the frozen product first and in fp32, not the adapters' part first and the product added to it in the epilogues that add
+// a residual: those read y where their other operands leave no time for it (4096 -> 14336 int4, 768 rows: 78 us without, 145
+// with; 4096 -> 4096 bf16, 8192 rows: 176 and 209), and y would be rounded twice.
 // Rows need no order.  The adapters lie in a table in device memory that the kernels read, so a batch is described by the
-// rows' indices alone and a captured call follows them.  A row whose index is outside the table gets zeros here; what its
-// x or another adapter's factors hold (infinities, NaN) never reaches it, since rows are selected, not multiplied by zero.
+// rows' indices alone and a captured call follows them.  A row whose index is outside the table is the frozen product alone;
+// what another row or another row's adapter holds (infinities, NaN) never reaches it, since rows are selected, not
+// multiplied by zero.
 #include "umma.cuh"
 
 namespace caifq
@@ -87,8 +92,8 @@ bank_down_kernel(const T *x, const int32_t *__restrict__ adapter_of_row, const c
 // a thread a column of y
 template <typename T>
 __global__ void __launch_bounds__(kBankThreads)
-bank_up_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries,
-               int count, T *y, int ld, int out_dim)
+bank_up_kernel(const float *frozen, const float *h, const int32_t *__restrict__ adapter_of_row,
+               const caifq_lora_entry *__restrict__ entries, int count, T *y, int ld, int out_dim)
 {
   __shared__ float sh[kBankMaxRank];
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
@@ -117,7 +122,8 @@ bank_up_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, const
     }
     v *= entries[id].scale;
   }
-  y[row * out_dim + col] = bank_t<T>(v);
+  const float f = frozen[row * out_dim + col];
+  y[row * out_dim + col] = bank_t<T>(mine ? f + v : f);
 }
 
 // ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on 16 rows of the batch as they lie ----
@@ -143,13 +149,20 @@ __device__ __forceinline__ uint32_t first_rows(const int (&ids)[16])
   return __ballot_sync(0xFFFFFFFFu, id >= 0 && (same & ((1u << lane) - 1u)) == 0u);
 }
 
-__device__ __forceinline__ void load_ids(int (&ids)[16], const int32_t *adapter_of_row, int64_t row0, int64_t m, int count)
+// ids and table entries of a tile's rows, once for all turns
+__device__ __forceinline__ void load_ids(int (&ids)[16], caifq_lora_entry (&mine)[16], const int32_t *adapter_of_row,
+                                         const caifq_lora_entry *entries, int64_t row0, int64_t m, int count)
 {
   if (threadIdx.x < 16)
   {
     const int64_t row = row0 + threadIdx.x;
-    const int id = row < m ? adapter_of_row[row] : -1;
-    ids[threadIdx.x] = id < count ? (id < 0 ? -1 : id) : -1;
+    int id = row < m ? adapter_of_row[row] : -1;
+    id = id < count ? (id < 0 ? -1 : id) : -1;
+    ids[threadIdx.x] = id;
+    if (id >= 0)
+    {
+      mine[threadIdx.x] = entries[id];
+    }
   }
   __syncthreads();
 }
@@ -165,6 +178,7 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
 {
   __shared__ float part[8][16][NT * 8 + 1];
   __shared__ int ids[16];
+  __shared__ caifq_lora_entry entry[16];
   // (what invariant loads read is addressed out of the wait, so that they stay behind it)
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -174,7 +188,7 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
   const int t = lane & 3;
   const int rank_in_cluster = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x / cluster) * 16;
-  load_ids(ids, adapter_of_row, row0, m, count);
+  load_ids(ids, entry, adapter_of_row, entries, row0, m, count);
   uint32_t firsts = first_rows(ids);
   const int steps = in_dim / 32;
   const int begin = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp) / (8 * cluster));
@@ -187,9 +201,10 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
     {
       continue;
     }
-    const int id = ids[__ffs(static_cast<int>(firsts)) - 1];
-    const int eights = entries[id].rank / 8;
-    const __nv_bfloat16 *a = static_cast<const __nv_bfloat16 *>(entries[id].a);
+    const int at = __ffs(static_cast<int>(firsts)) - 1;
+    const int id = ids[at];
+    const int eights = entry[at].rank / 8;
+    const __nv_bfloat16 *a = static_cast<const __nv_bfloat16 *>(entry[at].a);
     const bool lo = ids[g] == id;
     const bool hi = ids[g + 8] == id;
     const uint4 *x_lo = reinterpret_cast<const uint4 *>(x + (lo ? row0 + g : 0) * in_dim) + t;
@@ -278,12 +293,20 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
 }
 
 // y of 16 rows and 128 columns: a warp 32 columns.  h enters as two bf16 terms (2^-16 relative).  The columns of a warp's four
-// 8-wide tiles are dealt out so that a lane ends with eight neighbouring ones of a row: 16-byte stores.
+// 8-wide tiles are dealt out so that a lane ends with eight neighbouring ones of a row: 16-byte accesses of y.
+struct UpOperands
+{
+  uint2 w[4];                // rows of B, four columns of it each
+  uint32_t top[2][2];        // h of rows g and g + 8: the first terms
+  uint32_t rest[2][2];       // and the second
+};
+
 __global__ void __launch_bounds__(128)
-bank_up_mma_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries,
-                   int count, __nv_bfloat16 *y, int ld, int64_t m, int out_dim)
+bank_up_mma_kernel(const float *frozen, const float *h, const int32_t *__restrict__ adapter_of_row,
+                   const caifq_lora_entry *__restrict__ entries, int count, __nv_bfloat16 *y, int ld, int64_t m, int out_dim)
 {
   __shared__ int ids[16];
+  __shared__ caifq_lora_entry entry[16];
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
@@ -291,80 +314,124 @@ bank_up_mma_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, c
   const int t = lane & 3;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 16;
   const int col0 = static_cast<int>(blockIdx.y) * 128 + static_cast<int>(threadIdx.x >> 5) * 32;
-  load_ids(ids, adapter_of_row, row0, m, count);
-  uint32_t firsts = first_rows(ids);
   const bool stores = col0 + 8 * t < out_dim;
-  const int n0 = col0 + 8 * (g >> 1) + (g & 1);   // the column whose row of B this lane feeds, plus 2 * tile
-  for (int turn = 0; firsts != 0u; ++turn, firsts &= firsts - 1u)
+  // the frozen product's part of this lane's sixteen results is on its way meanwhile
+  float4 f[2][2];
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
   {
-    if (turn % static_cast<int>(gridDim.z) != static_cast<int>(blockIdx.z))
+    const int64_t row = row0 + g + 8 * half;
+    if (stores && row < m)
     {
-      continue;
+      const float4 *src = reinterpret_cast<const float4 *>(frozen + row * out_dim + col0 + 8 * t);
+      f[half][0] = src[0];
+      f[half][1] = src[1];
     }
-    const int id = ids[__ffs(static_cast<int>(firsts)) - 1];
-    const int rank = entries[id].rank;
-    const float scale = entries[id].scale;
-    const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entries[id].b);
-    const bool mine[2] = {ids[g] == id, ids[g + 8] == id};
-    float c[4][4];
+  }
+  load_ids(ids, entry, adapter_of_row, entries, row0, m, count);
+  uint32_t firsts = first_rows(ids);
+  const int n0 = col0 + 8 * (g >> 1) + (g & 1);   // the column whose row of B this lane feeds, plus 2 * tile
+  const int id_of[2] = {ids[g], ids[g + 8]};
+  auto operands = [&](int at, int k) {
+    UpOperands o;
+    const int rank = entry[at].rank;
+    const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entry[at].b);
+    const int kk = k + 4 * t;
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt)
     {
-      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
-    }
-#pragma unroll 1
-    for (int k = 0; k < rank; k += 16)
-    {
-      const int kk = k + 4 * t;
-      uint2 w[4];
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+      o.w[nt] = make_uint2(0u, 0u);
+      if (kk < rank && n0 + 2 * nt < out_dim)
       {
-        w[nt] = make_uint2(0u, 0u);
-        if (kk < rank && n0 + 2 * nt < out_dim)
-        {
-          w[nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n0 + 2 * nt) * rank + kk));
-        }
-      }
-      uint32_t top[2][2], rest[2][2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-      {
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (mine[half] && kk < rank)
-        {
-          v = *reinterpret_cast<const float4 *>(h + (row0 + g + 8 * half) * ld + kk);
-        }
-        const float f[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-        {
-          top[half][i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-          const float r0 = f[2 * i] - __uint_as_float(top[half][i] << 16);
-          const float r1 = f[2 * i + 1] - __uint_as_float(top[half][i] & 0xFFFF0000u);
-          // (an infinity has no second term)
-          rest[half][i] = pack_bf16x2(isfinite(f[2 * i]) ? r0 : 0.0f, isfinite(f[2 * i + 1]) ? r1 : 0.0f);
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
-      {
-        mma_16816(c[nt], top[0][0], top[1][0], top[0][1], top[1][1], w[nt].x, w[nt].y);
-        mma_16816(c[nt], rest[0][0], rest[1][0], rest[0][1], rest[1][1], w[nt].x, w[nt].y);
+        o.w[nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n0 + 2 * nt) * rank + kk));
       }
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half)
     {
-      if (mine[half] && stores)
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (id_of[half] == ids[at] && kk < rank)
+      {
+        v = *reinterpret_cast<const float4 *>(h + (row0 + g + 8 * half) * ld + kk);
+      }
+      const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+      {
+        const uint32_t top = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+        // (an infinity has no second term)
+        const float r0 = isfinite(e[2 * i]) ? e[2 * i] - __uint_as_float(top << 16) : 0.0f;
+        const float r1 = isfinite(e[2 * i + 1]) ? e[2 * i + 1] - __uint_as_float(top & 0xFFFF0000u) : 0.0f;
+        o.top[half][i] = top;
+        o.rest[half][i] = pack_bf16x2(r0, r1);
+      }
+    }
+    return o;
+  };
+  auto multiply = [](float(&c)[4][4], const UpOperands &o) {
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+    {
+      mma_16816(c[nt], o.top[0][0], o.top[1][0], o.top[0][1], o.top[1][1], o.w[nt].x, o.w[nt].y);
+      mma_16816(c[nt], o.rest[0][0], o.rest[1][0], o.rest[0][1], o.rest[1][1], o.w[nt].x, o.w[nt].y);
+    }
+  };
+  auto add = [&](const float(&c)[4][4], int at) {
+    const float scale = entry[at].scale;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      if (id_of[half] == ids[at] && stores)
       {
         uint4 o;
-        o.x = pack_bf16x2(c[0][2 * half] * scale, c[0][2 * half + 1] * scale);
-        o.y = pack_bf16x2(c[1][2 * half] * scale, c[1][2 * half + 1] * scale);
-        o.z = pack_bf16x2(c[2][2 * half] * scale, c[2][2 * half + 1] * scale);
-        o.w = pack_bf16x2(c[3][2 * half] * scale, c[3][2 * half + 1] * scale);
+        o.x = pack_bf16x2(fmaf(c[0][2 * half], scale, f[half][0].x), fmaf(c[0][2 * half + 1], scale, f[half][0].y));
+        o.y = pack_bf16x2(fmaf(c[1][2 * half], scale, f[half][0].z), fmaf(c[1][2 * half + 1], scale, f[half][0].w));
+        o.z = pack_bf16x2(fmaf(c[2][2 * half], scale, f[half][1].x), fmaf(c[2][2 * half + 1], scale, f[half][1].y));
+        o.w = pack_bf16x2(fmaf(c[3][2 * half], scale, f[half][1].z), fmaf(c[3][2 * half + 1], scale, f[half][1].w));
         *reinterpret_cast<uint4 *>(y + (row0 + g + 8 * half) * out_dim + col0 + 8 * t) = o;
       }
+    }
+  };
+  // this block's share of the tile's adapters, two at a time so that the loads of one hide behind the other's
+  int turn = 0;
+  auto next = [&]() {
+    while (firsts != 0u)
+    {
+      const int at = __ffs(static_cast<int>(firsts)) - 1;
+      firsts &= firsts - 1u;
+      if (turn++ % static_cast<int>(gridDim.z) == static_cast<int>(blockIdx.z))
+      {
+        return at;
+      }
+    }
+    return -1;
+  };
+  for (int a = next(); a >= 0; a = next())
+  {
+    const int b = next();
+    UpOperands oa = operands(a, 0);
+    UpOperands ob = oa;
+    if (b >= 0)
+    {
+      ob = operands(b, 0);
+    }
+    float ca[4][4] = {}, cb[4][4] = {};
+    multiply(ca, oa);
+#pragma unroll 1
+    for (int k = 16; k < entry[a].rank; k += 16)
+    {
+      multiply(ca, operands(a, k));
+    }
+    add(ca, a);
+    if (b >= 0)
+    {
+      multiply(cb, ob);
+#pragma unroll 1
+      for (int k = 16; k < entry[b].rank; k += 16)
+      {
+        multiply(cb, operands(b, k));
+      }
+      add(cb, b);
     }
   }
   if (blockIdx.z == 0 && stores)
@@ -373,15 +440,18 @@ bank_up_mma_kernel(const float *h, const int32_t *__restrict__ adapter_of_row, c
     for (int half = 0; half < 2; ++half)
     {
       const int64_t row = row0 + g + 8 * half;
-      if (row < m && ids[g + 8 * half] < 0)
+      if (row < m && id_of[half] < 0)
       {
-        *reinterpret_cast<uint4 *>(y + row * out_dim + col0 + 8 * t) = make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4 *>(y + row * out_dim + col0 + 8 * t) =
+            make_uint4(pack_bf16x2(f[half][0].x, f[half][0].y), pack_bf16x2(f[half][0].z, f[half][0].w),
+                       pack_bf16x2(f[half][1].x, f[half][1].y), pack_bf16x2(f[half][1].z, f[half][1].w));
       }
     }
   }
 }
 
-// blocks that share a tile's adapters: as many as keep the launch near `most` blocks, and no more than there can be adapters
+// blocks that share a tile's adapters, no more than there can be: as many as keep the launch near `most` blocks.  (Most of
+// them find nothing to do where a tile's rows are one prompt's, and leave at once.)
 int bank_shares(int64_t blocks, int64_t most, int64_t m, int count)
 {
   int64_t n = most / blocks;
@@ -391,17 +461,16 @@ int bank_shares(int64_t blocks, int64_t most, int64_t m, int count)
   return static_cast<int>(n < 1 ? 1 : n);
 }
 
-int bank_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
-             cudaStream_t s)
+int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h, cudaStream_t s)
 {
   const int64_t tiles = (m + 15) / 16;
-  const int shares = bank_shares(tiles, 4 * 148, m, bank.count);
   // blocks of a cluster: as in the adapter's own thin product, with at least two steps of 32 columns for every warp
   int cluster = 1;
-  while (cluster < 8 && tiles * shares * cluster < 4 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
+  while (cluster < 8 && tiles * cluster < 4 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
   {
     cluster *= 2;
   }
+  const int shares = bank_shares(tiles * cluster, 32 * 148, m, bank.count);
   void (*down)(const __nv_bfloat16 *, const int32_t *, const caifq_lora_entry *, int, float *, int, int64_t, int, int) =
       bank.max_rank <= 8 ? bank_down_mma_kernel<1>
                          : (bank.max_rank <= 16 ? bank_down_mma_kernel<2>
@@ -421,50 +490,81 @@ int bank_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
   cfg.numAttrs = dependent_launches() ? 2 : 1;
   CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, down, static_cast<const __nv_bfloat16 *>(x), adapter_of_row, bank.entries,
                                       bank.count, h, bank.max_rank, m, bank.in_dim, cluster));
+  return CAIFQ_OK;
+}
+
+int up_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h, int64_t m, void *y,
+           cudaStream_t s)
+{
+  const int64_t tiles = (m + 15) / 16;
   const int64_t columns = (bank.out_dim + 127) / 128;
   CAIFQ_CHECK_CUDA(launch_dependent(bank_up_mma_kernel,
                                     dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(columns),
                                          static_cast<unsigned>(bank_shares(tiles * columns, 16 * 148, m, bank.count))),
-                                    dim3(128), 0, s, static_cast<const float *>(h), adapter_of_row, bank.entries, bank.count,
+                                    dim3(128), 0, s, frozen, h, adapter_of_row, bank.entries, bank.count,
                                     static_cast<__nv_bfloat16 *>(y), bank.max_rank, m, bank.out_dim));
   return CAIFQ_OK;
 }
 
 template <typename T>
-int bank_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
-                 cudaStream_t s)
+int down_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h, cudaStream_t s)
 {
-  const unsigned parts = static_cast<unsigned>((bank.max_rank + 7) / 8);
-  CAIFQ_CHECK_CUDA(launch_dependent(bank_down_kernel<T>, dim3(static_cast<unsigned>(m), parts), dim3(kBankThreads), 0, s,
-                                    static_cast<const T *>(x), adapter_of_row, bank.entries, bank.count, h, bank.max_rank,
-                                    bank.in_dim));
-  CAIFQ_CHECK_CUDA(launch_dependent(bank_up_kernel<T>, dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.out_dim + kBankThreads - 1) / kBankThreads)),
-                                    dim3(kBankThreads), 0, s, static_cast<const float *>(h), adapter_of_row, bank.entries,
-                                    bank.count, static_cast<T *>(y), bank.max_rank, bank.out_dim));
+  CAIFQ_CHECK_CUDA(launch_dependent(bank_down_kernel<T>, dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.max_rank + 7) / 8)),
+                                    dim3(kBankThreads), 0, s, static_cast<const T *>(x), adapter_of_row, bank.entries, bank.count,
+                                    h, bank.max_rank, bank.in_dim));
   return CAIFQ_OK;
 }
 
+template <typename T>
+int up_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h, int64_t m, void *y,
+               cudaStream_t s)
+{
+  CAIFQ_CHECK_CUDA(launch_dependent(bank_up_kernel<T>,
+                                    dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.out_dim + kBankThreads - 1) / kBankThreads)),
+                                    dim3(kBankThreads), 0, s, frozen, h, adapter_of_row, bank.entries, bank.count,
+                                    static_cast<T *>(y), bank.max_rank, bank.out_dim));
+  return CAIFQ_OK;
+}
+
+bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
 }  // namespace
 
-// y[m, out] = the adapters' part alone, zeros for rows without one; h: fp32 [m, max_rank].  m >= 1
-int launch_lora_bank(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *y, float *h,
-                     cudaStream_t s)
+// h[m, max_rank] (fp32, 16-byte aligned) = x . A^T of each row's adapter; rows without one are left as they are.  m >= 1
+int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h,
+                          cudaStream_t s)
 {
-  // (16-byte loads of x and stores of y; m, so that the grid's first dimension holds it with the clusters)
-  if (bank.dtype == CAIFQ_BF16 && bank.vectors != 0 && bank.max_rank <= 64 && (bank.max_rank % 8) == 0 && (bank.in_dim % 32) == 0 &&
-      (bank.out_dim % 8) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15u) == 0 &&
-      bank.out_dim <= 65535 * 128)
+  if (bank.vectors != 0 && (bank.in_dim % 32) == 0 && on_16(x))
   {
-    return bank_mma(bank, adapter_of_row, x, m, y, h, s);
+    return down_mma(bank, adapter_of_row, x, m, h, s);
   }
   switch (bank.dtype)
   {
     case CAIFQ_F32:
-      return bank_general<float>(bank, adapter_of_row, x, m, y, h, s);
+      return down_general<float>(bank, adapter_of_row, x, m, h, s);
     case CAIFQ_F16:
-      return bank_general<__half>(bank, adapter_of_row, x, m, y, h, s);
+      return down_general<__half>(bank, adapter_of_row, x, m, h, s);
     default:
-      return bank_general<__nv_bfloat16>(bank, adapter_of_row, x, m, y, h, s);
+      return down_general<__nv_bfloat16>(bank, adapter_of_row, x, m, h, s);
+  }
+}
+
+// y[m, out] = frozen[m, out] + the adapters' part; frozen (fp32) may be y itself.  m >= 1
+int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h,
+                        int64_t m, void *y, cudaStream_t s)
+{
+  if (bank.vectors != 0 && (bank.out_dim % 8) == 0 && bank.out_dim <= 65535 * 128 && on_16(y) && on_16(frozen))
+  {
+    return up_mma(bank, adapter_of_row, frozen, h, m, y, s);
+  }
+  switch (bank.dtype)
+  {
+    case CAIFQ_F32:
+      return up_general<float>(bank, adapter_of_row, frozen, h, m, y, s);
+    case CAIFQ_F16:
+      return up_general<__half>(bank, adapter_of_row, frozen, h, m, y, s);
+    default:
+      return up_general<__nv_bfloat16>(bank, adapter_of_row, frozen, h, m, y, s);
   }
 }
 

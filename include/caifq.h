@@ -354,8 +354,8 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
  * one pair of factors): row t of the batch takes the adapter adapter_of_row[t] of a bank,
  *   y[t] = x[t] . W_deq^T + (alpha_a / rank_a) (x[t] . A_a^T) . B_a^T,   a = adapter_of_row[t]
  * Rows whose index is outside [0, count) get the frozen product alone.  Indices, factors and rows may change between two
- * replays of a captured call; rows need no order.  x . A^T is kept in fp32; the adapters' part is rounded to the result's
- * type where the frozen product is added to it.
+ * replays of a captured call; rows need no order.  x . A^T and the frozen product are kept in fp32; the result is rounded
+ * once.
  *
  * A bank is a table of `count` entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
  * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank]), fills the table's image in HOST memory and every
@@ -383,7 +383,8 @@ typedef struct caifq_lora_bank
 
 CAIFQ_API int caifq_lora_bank_entries(const caifq_lora *loras, int32_t count, int32_t in_dim, int32_t out_dim,
                                       caifq_lora_entry *entries_host, caifq_lora_bank *bank);
-/* Scratch of the call below (x . A^T, and, for many tokens, the weight expanded as by caifq_linear_fwd_ws): 256-byte aligned,
+/* Scratch of the call below (x . A^T, the frozen product where y has 16 bits, and, for many tokens, the weight expanded as by
+ * caifq_linear_fwd_ws): 256-byte aligned,
  * at least this large; nothing in it outlives the call.  Calls that may overlap on the GPU need workspaces of their own. */
 CAIFQ_API size_t caifq_lora_bank_workspace_bytes(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m,
                                                  int32_t compute_dtype);
