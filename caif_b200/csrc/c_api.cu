@@ -130,10 +130,11 @@ int launch_rmsnorm_fwd(const void *input, const float *gamma, void *output, floa
 int launch_rmsnorm_bwd(const void *grad_output, const void *input, const float *gamma, const float *rms_cache,
                        void *grad_input, float *grad_gamma, int dtype, int rows, int dim, cudaStream_t s);
 // lora_bank.cu
-int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h,
-                          cudaStream_t s);
-int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h,
-                        int64_t m, void *y, cudaStream_t s);
+size_t lora_bank_scratch_bytes(const caifq_lora_bank &bank, int64_t m);
+int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m,
+                          const void *y, void *scratch, cudaStream_t s);
+int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m,
+                        void *y, void *scratch, cudaStream_t s);
 // act8.cu
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
@@ -1123,7 +1124,7 @@ struct BankWs
 BankWs bank_ws(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m, int compute_dtype)
 {
   BankWs o{};
-  o.frozen = align256(static_cast<size_t>(m) * static_cast<size_t>(bank->max_rank) * sizeof(float));
+  o.frozen = lora_bank_scratch_bytes(*bank, m);
   o.weight = o.frozen + (bank->dtype == CAIFQ_F32
                              ? 0
                              : align256(static_cast<size_t>(m) * static_cast<size_t>(w->out_dim) * sizeof(float)));
@@ -1202,16 +1203,15 @@ int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *ban
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const BankWs ws = bank_ws(w, bank, m, compute_dtype);
   char *base = static_cast<char *>(workspace);
-  float *h = static_cast<float *>(workspace);
   float *frozen = static_cast<float *>(bank->dtype == CAIFQ_F32 ? y : static_cast<void *>(base + ws.frozen));
-  int r = launch_lora_bank_down(*bank, adapter_of_row, x, m, h, s);
+  int r = launch_lora_bank_down(*bank, adapter_of_row, x, frozen, m, y, workspace, s);
   if (r == CAIFQ_OK)
   {
     r = linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who);
   }
   if (r == CAIFQ_OK)
   {
-    r = launch_lora_bank_up(*bank, adapter_of_row, frozen, h, m, y, s);
+    r = launch_lora_bank_up(*bank, adapter_of_row, x, frozen, m, y, workspace, s);
   }
   return r;
 }

@@ -126,11 +126,143 @@ bank_up_kernel(const float *frozen, const float *h, const int32_t *__restrict__ 
   y[row * out_dim + col] = bank_t<T>(mine ? f + v : f);
 }
 
-// ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on 16 rows of the batch as they lie ----
-// A block takes 16 neighbouring rows and goes through the adapters that they name, one after the other (gridDim blocks share
-// them).  The rows of a prompt share one adapter, 16 decoding sequences may name 16: their factors are read once a tile in
-// either case, and no sorting of rows, and no launch for it, comes before.  Each adapter's product has accumulators of its
-// own and is stored for its own rows alone.
+// ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on tiles of up to 16 rows of one adapter ----
+// Rows are dealt to tiles by adapter first, wherever they stand in the batch (those without one make tiles of their own, which
+// `up` copies).  A call of up to 256 rows does that inside every block of `down`, longer ones in a launch ahead of it.  Tiles
+// of neighbouring rows as they lie, with a turn for every adapter that they name, need neither; but 200 decoding sequences of
+// 24 adapters are then 13 tiles of 14 turns, which held up `up` for 28 us beside 131 tiles of prompts, and here they are 24.
+// Which tile and slot a row gets does not change its arithmetic, so results do not depend on the rows' order.
+
+constexpr int kTileRows = 16;
+constexpr int kSmallCall = 256;     // rows that a block of `down` sorts by itself
+constexpr int kTableMost = 4096;    // adapters that the launch ahead counts in shared memory
+
+// what `down` leaves for `up`, in the workspace
+struct BankPlan
+{
+  caifq_lora_entry *entry;   // [tiles] of the tile's adapter; rank 0: rows without one; rank -1: no tile
+  int32_t *rows;             // [tiles][16], -1: no row
+  float *h;                  // [tiles][16][ld]
+};
+
+int64_t most_tiles(int64_t m, int count)
+{
+  const int64_t groups = m < count + 1 ? m : count + 1;
+  return (m + 15 * groups) / 16;
+}
+
+__device__ __forceinline__ int group_of(const int32_t *adapter_of_row, int64_t row, int count)
+{
+  const int id = adapter_of_row[row];
+  return id >= 0 && id < count ? id : count;
+}
+
+// tiles of a longer call: count, number the tiles, deal the rows.  (The slots inside an adapter follow the order in which
+// atomics are served; nothing but the rows' places depends on it.)
+__global__ void __launch_bounds__(1024)
+bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries, int count,
+                 const BankPlan plan, int64_t m, int most)
+{
+  extern __shared__ int table[];   // [count + 1] rows so far, [count + 1] first tile
+  __shared__ int warp_sums[32];
+  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  int *rows_of = table;
+  int *first = table + count + 1;
+  for (int i = threadIdx.x; i <= count; i += 1024)
+  {
+    rows_of[i] = 0;
+  }
+  __syncthreads();
+  // one addition for the lanes of a warp that have one adapter; the row's place in it, where `deal`
+  auto place = [&](int64_t row) {
+    const bool live = row < m;
+    const int id = live ? group_of(adapter_of_row, row, count) : -1;
+    const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
+    const int leader = __ffs(static_cast<int>(same)) - 1;
+    int at = 0;
+    if (live && lane == leader)
+    {
+      at = atomicAdd(&rows_of[id], __popc(same));
+    }
+    at = __shfl_sync(0xFFFFFFFFu, at, leader) + __popc(same & ((1u << lane) - 1u));
+    return make_int2(id, at);
+  };
+  const int64_t trips = (m + 1023) / 1024;
+  for (int64_t i = 0; i < trips; ++i)
+  {
+    place(i * 1024 + threadIdx.x);
+  }
+  __syncthreads();
+  // first tiles: an exclusive sum over the adapters, a run of them for each thread
+  const int run = (count + 1024) / 1024;
+  const int begin = static_cast<int>(threadIdx.x) * run;
+  int sum = 0;
+  for (int i = begin; i < begin + run && i <= count; ++i)
+  {
+    sum += (rows_of[i] + kTileRows - 1) / kTileRows;
+  }
+  int inclusive = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1)
+  {
+    const int other = __shfl_up_sync(0xFFFFFFFFu, inclusive, off);
+    inclusive += lane >= off ? other : 0;
+  }
+  if (lane == 31)
+  {
+    warp_sums[warp] = inclusive;
+  }
+  __syncthreads();
+  int before = 0, tiles = 0;
+  for (int w = 0; w < 32; ++w)
+  {
+    before += w < warp ? warp_sums[w] : 0;
+    tiles += warp_sums[w];
+  }
+  int tile = before + inclusive - sum;
+  for (int i = begin; i < begin + run && i <= count; ++i)
+  {
+    first[i] = tile;
+    const int rows = rows_of[i];
+    const int mine = (rows + kTileRows - 1) / kTileRows;
+    caifq_lora_entry e{};
+    if (i < count && rows > 0)
+    {
+      e = entries[i];
+    }
+    for (int k = 0; k < mine; ++k)
+    {
+      plan.entry[tile + k] = e;
+    }
+    for (int r = rows; r < mine * kTileRows; ++r)
+    {
+      plan.rows[static_cast<int64_t>(tile) * kTileRows + r] = -1;
+    }
+    tile += mine;
+  }
+  for (int i = tiles + static_cast<int>(threadIdx.x); i < most; i += 1024)
+  {
+    plan.entry[i].rank = -1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i <= count; i += 1024)
+  {
+    rows_of[i] = 0;
+  }
+  __syncthreads();
+  for (int64_t i = 0; i < trips; ++i)
+  {
+    const int64_t row = i * 1024 + threadIdx.x;
+    const int2 p = place(row);
+    if (row < m)
+    {
+      plan.rows[static_cast<int64_t>(first[p.x]) * kTileRows + p.y] = static_cast<int32_t>(row);
+    }
+  }
+}
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1)
@@ -140,45 +272,75 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// the adapters of 16 rows: ids[i] of row i (-1: none); returns the rows at which one appears for the first time
-__device__ __forceinline__ uint32_t first_rows(const int (&ids)[16])
+// the rows and adapter of tile `tile` of a call of m <= kSmallCall rows; false: there is no such tile.  All 256 threads.
+__device__ __forceinline__ bool small_tile(const int32_t *adapter_of_row, const caifq_lora_entry *entries, int count, int m, int tile,
+                                           int (&rows)[kTileRows], caifq_lora_entry &entry)
 {
-  const int lane = threadIdx.x & 31;
-  const int id = lane < 16 ? ids[lane] : -1;
-  const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
-  return __ballot_sync(0xFFFFFFFFu, id >= 0 && (same & ((1u << lane) - 1u)) == 0u);
-}
-
-// ids and table entries of a tile's rows, once for all turns
-__device__ __forceinline__ void load_ids(int (&ids)[16], caifq_lora_entry (&mine)[16], const int32_t *adapter_of_row,
-                                         const caifq_lora_entry *entries, int64_t row0, int64_t m, int count)
-{
-  if (threadIdx.x < 16)
+  __shared__ int id_of[kSmallCall];
+  __shared__ int warp_tiles[kSmallCall / 32];
+  __shared__ int lead[2];   // the row that begins the tile, and how many of its adapter come before it
+  const int i = threadIdx.x;
+  const int id = i < m ? group_of(adapter_of_row, i, count) : -1;
+  id_of[i] = id;
+  if (i < kTileRows)
   {
-    const int64_t row = row0 + threadIdx.x;
-    int id = row < m ? adapter_of_row[row] : -1;
-    id = id < count ? (id < 0 ? -1 : id) : -1;
-    ids[threadIdx.x] = id;
-    if (id >= 0)
+    rows[i] = -1;
+  }
+  __syncthreads();
+  int before = 0;
+  for (int k = 0; k < m; ++k)
+  {
+    before += k < i && id_of[k] == id ? 1 : 0;
+  }
+  const bool begins = i < m && before % kTileRows == 0;
+  const uint32_t mask = __ballot_sync(0xFFFFFFFFu, begins);
+  if ((i & 31) == 0)
+  {
+    warp_tiles[i >> 5] = __popc(mask);
+  }
+  __syncthreads();
+  int tiles = 0, mine = __popc(mask & ((1u << (i & 31)) - 1u));
+#pragma unroll
+  for (int w = 0; w < kSmallCall / 32; ++w)
+  {
+    mine += w < (i >> 5) ? warp_tiles[w] : 0;
+    tiles += warp_tiles[w];
+  }
+  if (begins && mine == tile)
+  {
+    lead[0] = i;
+    lead[1] = before;
+    entry = caifq_lora_entry{};
+    if (id < count)
     {
-      mine[threadIdx.x] = entries[id];
+      entry = entries[id];
     }
   }
   __syncthreads();
+  if (tile >= tiles)
+  {
+    return false;
+  }
+  if (i < m && id == id_of[lead[0]] && before >= lead[1] && before < lead[1] + kTileRows)
+  {
+    rows[before - lead[1]] = i;
+  }
+  __syncthreads();
+  return true;
 }
 
-// h of 16 rows.  As in the adapter's own thin product, a lane streams 16 bytes of two rows of x and of a row of A per 32
-// columns straight into fragments (the order of the columns inside a fragment is the same for both); the eight warps split
-// the columns, and so do the blocks of a cluster where there are few rows.
-template <int NT>   // eights of the largest rank
+// h of a tile.  As in the adapter's own thin product, a lane streams 16 bytes of two rows of x and of a row of A per 32 columns
+// straight into fragments (the order of the columns inside a fragment is the same for both); the eight warps split the columns,
+// and so do the blocks of a cluster where there are few tiles.
+template <int NT, bool SMALL>   // eights of the largest rank
 __global__ void __launch_bounds__(256)
 bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter_of_row,
-                     const caifq_lora_entry *__restrict__ entries, int count, float *h, int ld, int64_t m, int in_dim,
+                     const caifq_lora_entry *__restrict__ entries, int count, const BankPlan plan, int ld, int64_t m, int in_dim,
                      int cluster)
 {
-  __shared__ float part[8][16][NT * 8 + 1];
-  __shared__ int ids[16];
-  __shared__ caifq_lora_entry entry[16];
+  __shared__ float part[8][kTileRows][NT * 8 + 1];
+  __shared__ int rows[kTileRows];
+  __shared__ caifq_lora_entry entry;
   // (what invariant loads read is addressed out of the wait, so that they stay behind it)
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -187,296 +349,312 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
   const int g = lane >> 2;
   const int t = lane & 3;
   const int rank_in_cluster = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x / cluster) * 16;
-  load_ids(ids, entry, adapter_of_row, entries, row0, m, count);
-  uint32_t firsts = first_rows(ids);
+  const int64_t tile = blockIdx.x / cluster;
+  if constexpr (SMALL)
+  {
+    // (every block of a cluster finds the same)
+    const bool any = small_tile(adapter_of_row, entries, count, static_cast<int>(m), static_cast<int>(tile), rows, entry);
+    if (rank_in_cluster == 0)
+    {
+      if (threadIdx.x == 0)
+      {
+        if (any)
+        {
+          plan.entry[tile] = entry;
+        }
+        else
+        {
+          plan.entry[tile].rank = -1;
+        }
+      }
+      if (any && threadIdx.x < kTileRows)
+      {
+        plan.rows[tile * kTileRows + threadIdx.x] = rows[threadIdx.x];
+      }
+    }
+    if (!any)
+    {
+      return;
+    }
+  }
+  else
+  {
+    if (threadIdx.x < kTileRows)
+    {
+      rows[threadIdx.x] = plan.rows[tile * kTileRows + threadIdx.x];
+    }
+    if (threadIdx.x == 0)
+    {
+      entry = plan.entry[tile];
+    }
+    __syncthreads();
+  }
+  const int eights = entry.rank / 8;
+  if (eights <= 0)
+  {
+    return;
+  }
   const int steps = in_dim / 32;
   const int begin = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp) / (8 * cluster));
   const int end = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp + 1) / (8 * cluster));
   const uint4 zero4 = make_uint4(0u, 0u, 0u, 0u);
-  // (ids has the same content in all blocks of a cluster, so they run the same turns)
-  for (int turn = 0; firsts != 0u; ++turn, firsts &= firsts - 1u)
+  const bool lo = rows[g] >= 0;
+  const bool hi = rows[g + 8] >= 0;
+  const uint4 *x_lo = reinterpret_cast<const uint4 *>(x + static_cast<int64_t>(lo ? rows[g] : 0) * in_dim) + t;
+  const uint4 *x_hi = reinterpret_cast<const uint4 *>(x + static_cast<int64_t>(hi ? rows[g + 8] : 0) * in_dim) + t;
+  const uint4 *a_row = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(entry.a) + static_cast<int64_t>(g) * in_dim) + t;
+  float c[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
   {
-    if (turn % static_cast<int>(gridDim.y) != static_cast<int>(blockIdx.y))
-    {
-      continue;
-    }
-    const int at = __ffs(static_cast<int>(firsts)) - 1;
-    const int id = ids[at];
-    const int eights = entry[at].rank / 8;
-    const __nv_bfloat16 *a = static_cast<const __nv_bfloat16 *>(entry[at].a);
-    const bool lo = ids[g] == id;
-    const bool hi = ids[g + 8] == id;
-    const uint4 *x_lo = reinterpret_cast<const uint4 *>(x + (lo ? row0 + g : 0) * in_dim) + t;
-    const uint4 *x_hi = reinterpret_cast<const uint4 *>(x + (hi ? row0 + g + 8 : 0) * in_dim) + t;
-    const uint4 *a_row = reinterpret_cast<const uint4 *>(a + static_cast<int64_t>(g) * in_dim) + t;
-    float c[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-    {
-      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
-    }
+    c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+  }
 #pragma unroll 4
-    for (int st = begin; st < end; ++st)
-    {
-      const uint4 xa = lo ? __ldg(x_lo + st * 4) : zero4;
-      const uint4 xb = hi ? __ldg(x_hi + st * 4) : zero4;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-      {
-        if (nt < eights)
-        {
-          const uint4 w = __ldg(a_row + static_cast<int64_t>(nt) * in_dim + st * 4);
-          mma_16816(c[nt], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
-          mma_16816(c[nt], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
-        }
-      }
-    }
+  for (int st = begin; st < end; ++st)
+  {
+    const uint4 xa = lo ? __ldg(x_lo + st * 4) : zero4;
+    const uint4 xb = hi ? __ldg(x_hi + st * 4) : zero4;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
     {
-      part[warp][g][nt * 8 + 2 * t] = c[nt][0];
-      part[warp][g][nt * 8 + 2 * t + 1] = c[nt][1];
-      part[warp][g + 8][nt * 8 + 2 * t] = c[nt][2];
-      part[warp][g + 8][nt * 8 + 2 * t + 1] = c[nt][3];
+      if (nt < eights)
+      {
+        const uint4 w = __ldg(a_row + static_cast<int64_t>(nt) * in_dim + st * 4);
+        mma_16816(c[nt], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+        mma_16816(c[nt], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+      }
     }
-    __syncthreads();
-    // the block's eight partial tiles become one, in the first of them (an element is one thread's)
-    for (int e = threadIdx.x; e < 16 * NT * 8; e += 256)
-    {
-      float v = 0.0f;
+  }
 #pragma unroll
-      for (int w = 0; w < 8; ++w)
+  for (int nt = 0; nt < NT; ++nt)
+  {
+    part[warp][g][nt * 8 + 2 * t] = c[nt][0];
+    part[warp][g][nt * 8 + 2 * t + 1] = c[nt][1];
+    part[warp][g + 8][nt * 8 + 2 * t] = c[nt][2];
+    part[warp][g + 8][nt * 8 + 2 * t + 1] = c[nt][3];
+  }
+  __syncthreads();
+  // the block's eight partial tiles become one, in the first of them (an element is one thread's)
+  for (int e = threadIdx.x; e < kTileRows * NT * 8; e += 256)
+  {
+    float v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w)
+    {
+      v += part[w][e / (NT * 8)][e % (NT * 8)];
+    }
+    part[0][e / (NT * 8)][e % (NT * 8)] = v;
+  }
+  if (cluster > 1)
+  {
+    cluster_sync_all();
+  }
+  else
+  {
+    __syncthreads();
+  }
+  const int share = kTileRows / cluster;
+  for (int e = threadIdx.x; e < share * NT * 8; e += 256)
+  {
+    const int rr = rank_in_cluster * share + e / (NT * 8);
+    const int col = e % (NT * 8);
+    if (rows[rr] >= 0 && col < eights * 8)
+    {
+      float v = part[0][rr][col];
+      if (cluster > 1)
       {
-        v += part[w][e / (NT * 8)][e % (NT * 8)];
-      }
-      part[0][e / (NT * 8)][e % (NT * 8)] = v;
-    }
-    if (cluster > 1)
-    {
-      cluster_sync_all();
-    }
-    else
-    {
-      __syncthreads();
-    }
-    const int share = 16 / cluster;
-    for (int e = threadIdx.x; e < share * NT * 8; e += 256)
-    {
-      const int rr = rank_in_cluster * share + e / (NT * 8);
-      const int col = e % (NT * 8);
-      if (ids[rr] == id && col < eights * 8)
-      {
-        float v = part[0][rr][col];
-        if (cluster > 1)
+        const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(&part[0][rr][col]));
+        float from[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b)   // (all on their way before the first is added)
         {
-          v = 0.0f;
-          const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(&part[0][rr][col]));
-          for (int b = 0; b < cluster; ++b)
-          {
-            v += __uint_as_float(ld_shared_cluster(map_to_cta(mine, static_cast<uint32_t>(b))));
-          }
+          from[b] = b < cluster ? __uint_as_float(ld_shared_cluster(map_to_cta(mine, static_cast<uint32_t>(b)))) : 0.0f;
         }
-        h[(row0 + rr) * ld + col] = v;
+        v = ((from[0] + from[1]) + (from[2] + from[3])) + ((from[4] + from[5]) + (from[6] + from[7]));
       }
+      plan.h[(tile * kTileRows + rr) * ld + col] = v;
     }
-    // nobody's partial tile is written again, or left, while it is read
-    if (cluster > 1)
-    {
-      cluster_sync_all();
-    }
-    else
-    {
-      __syncthreads();
-    }
+  }
+  if (cluster > 1)
+  {
+    cluster_sync_all();   // nobody's partial tile is left while it is read
   }
 }
 
-// y of 16 rows and 128 columns: a warp 32 columns.  h enters as two bf16 terms (2^-16 relative).  The columns of a warp's four
-// 8-wide tiles are dealt out so that a lane ends with eight neighbouring ones of a row: 16-byte accesses of y.
-struct UpOperands
-{
-  uint2 w[4];                // rows of B, four columns of it each
-  uint32_t top[2][2];        // h of rows g and g + 8: the first terms
-  uint32_t rest[2][2];       // and the second
-};
-
+// y of a tile's rows and 128 * GROUPS columns: a warp GROUPS times 32.  h enters as two bf16 terms (2^-16 relative).  The columns
+// of a group of 32 are dealt out to its four 8-wide tiles so that a lane ends with eight neighbouring ones of a row.  Bound by
+// latency (tile, then operands, then results) at few rows and by the frozen product's 4 bytes and y's 2 at many.
+template <int KS, int GROUPS>   // KS: sixteens of the largest rank
 __global__ void __launch_bounds__(128)
-bank_up_mma_kernel(const float *frozen, const float *h, const int32_t *__restrict__ adapter_of_row,
-                   const caifq_lora_entry *__restrict__ entries, int count, __nv_bfloat16 *y, int ld, int64_t m, int out_dim)
+bank_up_mma_kernel(const float *frozen, const BankPlan plan, __nv_bfloat16 *y, int ld, int out_dim)
 {
-  __shared__ int ids[16];
-  __shared__ caifq_lora_entry entry[16];
-  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2;
   const int t = lane & 3;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int col0 = static_cast<int>(blockIdx.y) * 128 + static_cast<int>(threadIdx.x >> 5) * 32;
-  const bool stores = col0 + 8 * t < out_dim;
-  // the frozen product's part of this lane's sixteen results is on its way meanwhile
-  float4 f[2][2];
-#pragma unroll
-  for (int half = 0; half < 2; ++half)
+  const int64_t tile = blockIdx.x;
+  const int col0 = (static_cast<int>(blockIdx.y) * 4 + warp) * 32 * GROUPS;
+  const caifq_lora_entry entry = plan.entry[tile];
+  const int32_t row_of[2] = {plan.rows[tile * kTileRows + g], plan.rows[tile * kTileRows + g + 8]};
+  const int rank = entry.rank;
+  if (rank < 0)
   {
-    const int64_t row = row0 + g + 8 * half;
-    if (stores && row < m)
+    return;
+  }
+  const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entry.b);
+  uint2 w[GROUPS][KS][4];
+  float4 f[GROUPS][2][2];
+  float4 v[KS][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+  {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
     {
-      const float4 *src = reinterpret_cast<const float4 *>(frozen + row * out_dim + col0 + 8 * t);
-      f[half][0] = src[0];
-      f[half][1] = src[1];
+      v[ks][half] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (row_of[half] >= 0 && 16 * ks + 4 * t < rank)
+      {
+        v[ks][half] = *reinterpret_cast<const float4 *>(plan.h + (tile * kTileRows + g + 8 * half) * ld + 16 * ks + 4 * t);
+      }
     }
   }
-  load_ids(ids, entry, adapter_of_row, entries, row0, m, count);
-  uint32_t firsts = first_rows(ids);
-  const int n0 = col0 + 8 * (g >> 1) + (g & 1);   // the column whose row of B this lane feeds, plus 2 * tile
-  const int id_of[2] = {ids[g], ids[g + 8]};
-  auto operands = [&](int at, int k) {
-    UpOperands o;
-    const int rank = entry[at].rank;
-    const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entry[at].b);
-    const int kk = k + 4 * t;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i)
+  {
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt)
     {
-      o.w[nt] = make_uint2(0u, 0u);
-      if (kk < rank && n0 + 2 * nt < out_dim)
+      const int n = col0 + 32 * i + 8 * (g >> 1) + 2 * nt + (g & 1);   // the column whose row of B this lane feeds
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
       {
-        o.w[nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n0 + 2 * nt) * rank + kk));
+        w[i][ks][nt] = make_uint2(0u, 0u);
+        if (16 * ks + 4 * t < rank && n < out_dim)
+        {
+          w[i][ks][nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n) * rank + 16 * ks + 4 * t));
+        }
       }
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half)
     {
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (id_of[half] == ids[at] && kk < rank)
+      if (row_of[half] >= 0 && col0 + 32 * i + 8 * t < out_dim)
       {
-        v = *reinterpret_cast<const float4 *>(h + (row0 + g + 8 * half) * ld + kk);
+        const float4 *src =
+            reinterpret_cast<const float4 *>(frozen + static_cast<int64_t>(row_of[half]) * out_dim + col0 + 32 * i + 8 * t);
+        f[i][half][0] = src[0];
+        f[i][half][1] = src[1];
       }
-      const float e[4] = {v.x, v.y, v.z, v.w};
+    }
+  }
+  uint32_t top[KS][2][2], rest[KS][2][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+  {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      const float e[4] = {v[ks][half].x, v[ks][half].y, v[ks][half].z, v[ks][half].w};
 #pragma unroll
       for (int i = 0; i < 2; ++i)
       {
-        const uint32_t top = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+        const uint32_t high = pack_bf16x2(e[2 * i], e[2 * i + 1]);
         // (an infinity has no second term)
-        const float r0 = isfinite(e[2 * i]) ? e[2 * i] - __uint_as_float(top << 16) : 0.0f;
-        const float r1 = isfinite(e[2 * i + 1]) ? e[2 * i + 1] - __uint_as_float(top & 0xFFFF0000u) : 0.0f;
-        o.top[half][i] = top;
-        o.rest[half][i] = pack_bf16x2(r0, r1);
+        const float r0 = isfinite(e[2 * i]) ? e[2 * i] - __uint_as_float(high << 16) : 0.0f;
+        const float r1 = isfinite(e[2 * i + 1]) ? e[2 * i + 1] - __uint_as_float(high & 0xFFFF0000u) : 0.0f;
+        top[ks][half][i] = high;
+        rest[ks][half][i] = pack_bf16x2(r0, r1);
       }
     }
-    return o;
-  };
-  auto multiply = [](float(&c)[4][4], const UpOperands &o) {
+  }
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i)
+  {
+    float c[4][4];
 #pragma unroll
     for (int nt = 0; nt < 4; ++nt)
     {
-      mma_16816(c[nt], o.top[0][0], o.top[1][0], o.top[0][1], o.top[1][1], o.w[nt].x, o.w[nt].y);
-      mma_16816(c[nt], o.rest[0][0], o.rest[1][0], o.rest[0][1], o.rest[1][1], o.w[nt].x, o.w[nt].y);
+      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+      if (rank > 0)   // (rows without an adapter: zeros, whatever the other rows hold)
+      {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+        {
+          mma_16816(c[nt], top[ks][0][0], top[ks][1][0], top[ks][0][1], top[ks][1][1], w[i][ks][nt].x, w[i][ks][nt].y);
+          mma_16816(c[nt], rest[ks][0][0], rest[ks][1][0], rest[ks][0][1], rest[ks][1][1], w[i][ks][nt].x, w[i][ks][nt].y);
+        }
+      }
     }
-  };
-  auto add = [&](const float(&c)[4][4], int at) {
-    const float scale = entry[at].scale;
 #pragma unroll
     for (int half = 0; half < 2; ++half)
     {
-      if (id_of[half] == ids[at] && stores)
+      if (row_of[half] >= 0 && col0 + 32 * i + 8 * t < out_dim)
       {
+        const float4 *q = f[i][half];
+        const int e = 2 * half;
         uint4 o;
-        o.x = pack_bf16x2(fmaf(c[0][2 * half], scale, f[half][0].x), fmaf(c[0][2 * half + 1], scale, f[half][0].y));
-        o.y = pack_bf16x2(fmaf(c[1][2 * half], scale, f[half][0].z), fmaf(c[1][2 * half + 1], scale, f[half][0].w));
-        o.z = pack_bf16x2(fmaf(c[2][2 * half], scale, f[half][1].x), fmaf(c[2][2 * half + 1], scale, f[half][1].y));
-        o.w = pack_bf16x2(fmaf(c[3][2 * half], scale, f[half][1].z), fmaf(c[3][2 * half + 1], scale, f[half][1].w));
-        *reinterpret_cast<uint4 *>(y + (row0 + g + 8 * half) * out_dim + col0 + 8 * t) = o;
-      }
-    }
-  };
-  // this block's share of the tile's adapters, two at a time so that the loads of one hide behind the other's
-  int turn = 0;
-  auto next = [&]() {
-    while (firsts != 0u)
-    {
-      const int at = __ffs(static_cast<int>(firsts)) - 1;
-      firsts &= firsts - 1u;
-      if (turn++ % static_cast<int>(gridDim.z) == static_cast<int>(blockIdx.z))
-      {
-        return at;
-      }
-    }
-    return -1;
-  };
-  for (int a = next(); a >= 0; a = next())
-  {
-    const int b = next();
-    UpOperands oa = operands(a, 0);
-    UpOperands ob = oa;
-    if (b >= 0)
-    {
-      ob = operands(b, 0);
-    }
-    float ca[4][4] = {}, cb[4][4] = {};
-    multiply(ca, oa);
-#pragma unroll 1
-    for (int k = 16; k < entry[a].rank; k += 16)
-    {
-      multiply(ca, operands(a, k));
-    }
-    add(ca, a);
-    if (b >= 0)
-    {
-      multiply(cb, ob);
-#pragma unroll 1
-      for (int k = 16; k < entry[b].rank; k += 16)
-      {
-        multiply(cb, operands(b, k));
-      }
-      add(cb, b);
-    }
-  }
-  if (blockIdx.z == 0 && stores)
-  {
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-    {
-      const int64_t row = row0 + g + 8 * half;
-      if (row < m && id_of[half] < 0)
-      {
-        *reinterpret_cast<uint4 *>(y + row * out_dim + col0 + 8 * t) =
-            make_uint4(pack_bf16x2(f[half][0].x, f[half][0].y), pack_bf16x2(f[half][0].z, f[half][0].w),
-                       pack_bf16x2(f[half][1].x, f[half][1].y), pack_bf16x2(f[half][1].z, f[half][1].w));
+        o.x = pack_bf16x2(fmaf(c[0][e], entry.scale, q[0].x), fmaf(c[0][e + 1], entry.scale, q[0].y));
+        o.y = pack_bf16x2(fmaf(c[1][e], entry.scale, q[0].z), fmaf(c[1][e + 1], entry.scale, q[0].w));
+        o.z = pack_bf16x2(fmaf(c[2][e], entry.scale, q[1].x), fmaf(c[2][e + 1], entry.scale, q[1].y));
+        o.w = pack_bf16x2(fmaf(c[3][e], entry.scale, q[1].z), fmaf(c[3][e + 1], entry.scale, q[1].w));
+        *reinterpret_cast<uint4 *>(y + static_cast<int64_t>(row_of[half]) * out_dim + col0 + 32 * i + 8 * t) = o;
       }
     }
   }
 }
 
-// blocks that share a tile's adapters, no more than there can be: as many as keep the launch near `most` blocks.  (Most of
-// them find nothing to do where a tile's rows are one prompt's, and leave at once.)
-int bank_shares(int64_t blocks, int64_t most, int64_t m, int count)
+size_t round_256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
+
+// the plan in `scratch`, of lora_bank_scratch_bytes
+BankPlan plan_in(void *scratch, int64_t tiles)
 {
-  int64_t n = most / blocks;
-  n = n > 16 ? 16 : n;
-  n = n > m ? m : n;
-  n = n > count ? count : n;
-  return static_cast<int>(n < 1 ? 1 : n);
+  char *p = static_cast<char *>(scratch);
+  BankPlan plan;
+  plan.entry = reinterpret_cast<caifq_lora_entry *>(p);
+  p += round_256(static_cast<size_t>(tiles) * sizeof(caifq_lora_entry));
+  plan.rows = reinterpret_cast<int32_t *>(p);
+  p += round_256(static_cast<size_t>(tiles) * kTileRows * sizeof(int32_t));
+  plan.h = reinterpret_cast<float *>(p);
+  return plan;
 }
 
-int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h, cudaStream_t s)
+int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, void *scratch, cudaStream_t s)
 {
-  const int64_t tiles = (m + 15) / 16;
-  // blocks of a cluster: as in the adapter's own thin product, with at least two steps of 32 columns for every warp
+  const int64_t tiles = most_tiles(m, bank.count);
+  const BankPlan plan = plan_in(scratch, tiles);
+  const bool small = m <= kSmallCall;
+  if (!small)
+  {
+    CAIFQ_CHECK_CUDA(launch_dependent(bank_plan_kernel, dim3(1), dim3(1024), static_cast<size_t>(bank.count + 1) * 2 * sizeof(int), s,
+                                      adapter_of_row, bank.entries, bank.count, plan, m, static_cast<int>(tiles)));
+  }
+  // clusters that split the columns where the tiles leave SMs without work, with at least two steps of 32 columns for every warp
   int cluster = 1;
   while (cluster < 8 && tiles * cluster < 4 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
   {
     cluster *= 2;
   }
-  const int shares = bank_shares(tiles * cluster, 32 * 148, m, bank.count);
-  void (*down)(const __nv_bfloat16 *, const int32_t *, const caifq_lora_entry *, int, float *, int, int64_t, int, int) =
-      bank.max_rank <= 8 ? bank_down_mma_kernel<1>
-                         : (bank.max_rank <= 16 ? bank_down_mma_kernel<2>
-                                                : (bank.max_rank <= 32 ? bank_down_mma_kernel<4> : bank_down_mma_kernel<8>));
+  void (*down)(const __nv_bfloat16 *, const int32_t *, const caifq_lora_entry *, int, BankPlan, int, int64_t, int, int) = nullptr;
+  if (bank.max_rank <= 8)
+  {
+    down = small ? bank_down_mma_kernel<1, true> : bank_down_mma_kernel<1, false>;
+  }
+  else if (bank.max_rank <= 16)
+  {
+    down = small ? bank_down_mma_kernel<2, true> : bank_down_mma_kernel<2, false>;
+  }
+  else if (bank.max_rank <= 32)
+  {
+    down = small ? bank_down_mma_kernel<4, true> : bank_down_mma_kernel<4, false>;
+  }
+  else
+  {
+    down = small ? bank_down_mma_kernel<8, true> : bank_down_mma_kernel<8, false>;
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * cluster), static_cast<unsigned>(shares));
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * cluster));
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -489,21 +667,32 @@ int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
   cfg.attrs = attr;
   cfg.numAttrs = dependent_launches() ? 2 : 1;
   CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, down, static_cast<const __nv_bfloat16 *>(x), adapter_of_row, bank.entries,
-                                      bank.count, h, bank.max_rank, m, bank.in_dim, cluster));
+                                      bank.count, plan, bank.max_rank, m, bank.in_dim, cluster));
   return CAIFQ_OK;
 }
 
-int up_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h, int64_t m, void *y,
-           cudaStream_t s)
+template <int KS, int GROUPS>
+int up_mma_inst(const caifq_lora_bank &bank, const BankPlan &plan, int64_t tiles, const float *frozen, void *y, cudaStream_t s)
 {
-  const int64_t tiles = (m + 15) / 16;
-  const int64_t columns = (bank.out_dim + 127) / 128;
-  CAIFQ_CHECK_CUDA(launch_dependent(bank_up_mma_kernel,
-                                    dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(columns),
-                                         static_cast<unsigned>(bank_shares(tiles * columns, 16 * 148, m, bank.count))),
-                                    dim3(128), 0, s, frozen, h, adapter_of_row, bank.entries, bank.count,
-                                    static_cast<__nv_bfloat16 *>(y), bank.max_rank, m, bank.out_dim));
+  const unsigned columns = static_cast<unsigned>((bank.out_dim + 128 * GROUPS - 1) / (128 * GROUPS));
+  CAIFQ_CHECK_CUDA(launch_dependent(bank_up_mma_kernel<KS, GROUPS>, dim3(static_cast<unsigned>(tiles), columns), dim3(128), 0, s, frozen,
+                                    plan, static_cast<__nv_bfloat16 *>(y), bank.max_rank, bank.out_dim));
   return CAIFQ_OK;
+}
+
+int up_mma(const caifq_lora_bank &bank, const float *frozen, int64_t m, void *y, void *scratch, cudaStream_t s)
+{
+  const int64_t tiles = most_tiles(m, bank.count);
+  const BankPlan plan = plan_in(scratch, tiles);
+  if (bank.max_rank <= 16)
+  {
+    return up_mma_inst<1, 2>(bank, plan, tiles, frozen, y, s);
+  }
+  if (bank.max_rank <= 32)
+  {
+    return up_mma_inst<2, 2>(bank, plan, tiles, frozen, y, s);
+  }
+  return up_mma_inst<4, 1>(bank, plan, tiles, frozen, y, s);
 }
 
 template <typename T>
@@ -528,16 +717,36 @@ int up_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const
 
 bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// whether a call runs on the tensor core.  (out_dim: the grid's second dimension; the tiles with their clusters fit the first)
+bool tiled(const caifq_lora_bank &bank, const void *x, const void *y, const float *frozen, int64_t m)
+{
+  return bank.vectors != 0 && (bank.in_dim % 32) == 0 && (bank.out_dim % 8) == 0 && bank.out_dim <= 65535 * 128 && on_16(x) &&
+         on_16(y) && on_16(frozen) && (m <= kSmallCall || bank.count <= kTableMost);
+}
+
 }  // namespace
 
-// h[m, max_rank] (fp32, 16-byte aligned) = x . A^T of each row's adapter; rows without one are left as they are.  m >= 1
-int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h,
-                          cudaStream_t s)
+// x . A^T of every row, and where the rows of each adapter are
+size_t lora_bank_scratch_bytes(const caifq_lora_bank &bank, int64_t m)
 {
-  if (bank.vectors != 0 && (bank.in_dim % 32) == 0 && on_16(x))
+  const size_t tiles = static_cast<size_t>(most_tiles(m, bank.count));
+  const size_t rank = static_cast<size_t>(bank.max_rank);
+  const size_t by_tile = round_256(tiles * sizeof(caifq_lora_entry)) + round_256(tiles * kTileRows * sizeof(int32_t)) +
+                         tiles * kTileRows * rank * sizeof(float);
+  const size_t by_row = static_cast<size_t>(m) * rank * sizeof(float);
+  return round_256(bank.vectors != 0 && by_tile > by_row ? by_tile : by_row);
+}
+
+// The two launches around the frozen product, with the same arguments: x . A^T into the scratch (256-byte aligned), and
+// y[m, out] = frozen[m, out] + the adapters' part; frozen (fp32) may be y itself.  m >= 1
+int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m,
+                          const void *y, void *scratch, cudaStream_t s)
+{
+  if (tiled(bank, x, y, frozen, m))
   {
-    return down_mma(bank, adapter_of_row, x, m, h, s);
+    return down_mma(bank, adapter_of_row, x, m, scratch, s);
   }
+  float *h = static_cast<float *>(scratch);
   switch (bank.dtype)
   {
     case CAIFQ_F32:
@@ -549,14 +758,14 @@ int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of
   }
 }
 
-// y[m, out] = frozen[m, out] + the adapters' part; frozen (fp32) may be y itself.  m >= 1
-int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, const float *h,
-                        int64_t m, void *y, cudaStream_t s)
+int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m,
+                        void *y, void *scratch, cudaStream_t s)
 {
-  if (bank.vectors != 0 && (bank.out_dim % 8) == 0 && bank.out_dim <= 65535 * 128 && on_16(y) && on_16(frozen))
+  if (tiled(bank, x, y, frozen, m))
   {
-    return up_mma(bank, adapter_of_row, frozen, h, m, y, s);
+    return up_mma(bank, frozen, m, y, scratch, s);
   }
+  const float *h = static_cast<const float *>(scratch);
   switch (bank.dtype)
   {
     case CAIFQ_F32:
