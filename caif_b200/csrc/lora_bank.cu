@@ -176,10 +176,9 @@ bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_en
     rows_of[i] = 0;
   }
   __syncthreads();
-  // one addition for the lanes of a warp that have one adapter; the row's place in it, where `deal`
-  auto place = [&](int64_t row) {
-    const bool live = row < m;
-    const int id = live ? group_of(adapter_of_row, row, count) : -1;
+  // one addition for the lanes of a warp that have one adapter; the row's place in it
+  auto place = [&](int id) {
+    const bool live = id >= 0;
     const uint32_t same = __match_any_sync(0xFFFFFFFFu, id);
     const int leader = __ffs(static_cast<int>(same)) - 1;
     int at = 0;
@@ -187,13 +186,26 @@ bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_en
     {
       at = atomicAdd(&rows_of[id], __popc(same));
     }
-    at = __shfl_sync(0xFFFFFFFFu, at, leader) + __popc(same & ((1u << lane) - 1u));
-    return make_int2(id, at);
+    return __shfl_sync(0xFFFFFFFFu, at, leader) + __popc(same & ((1u << lane) - 1u));
   };
-  const int64_t trips = (m + 1023) / 1024;
-  for (int64_t i = 0; i < trips; ++i)
+  // four rows a thread a trip, so that their indices come together
+  auto groups = [&](int (&id)[4], int64_t base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+      const int64_t row = base + i * 1024 + threadIdx.x;
+      id[i] = row < m ? group_of(adapter_of_row, row, count) : -1;
+    }
+  };
+  for (int64_t base = 0; base < m; base += 4096)
   {
-    place(i * 1024 + threadIdx.x);
+    int id[4];
+    groups(id, base);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+      place(id[i]);
+    }
   }
   __syncthreads();
   // first tiles: an exclusive sum over the adapters, a run of them for each thread
@@ -253,13 +265,18 @@ bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_en
     rows_of[i] = 0;
   }
   __syncthreads();
-  for (int64_t i = 0; i < trips; ++i)
+  for (int64_t base = 0; base < m; base += 4096)
   {
-    const int64_t row = i * 1024 + threadIdx.x;
-    const int2 p = place(row);
-    if (row < m)
+    int id[4];
+    groups(id, base);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
     {
-      plan.rows[static_cast<int64_t>(first[p.x]) * kTileRows + p.y] = static_cast<int32_t>(row);
+      const int at = place(id[i]);
+      if (id[i] >= 0)
+      {
+        plan.rows[static_cast<int64_t>(first[id[i]]) * kTileRows + at] = static_cast<int32_t>(base + i * 1024 + threadIdx.x);
+      }
     }
   }
 }
@@ -632,7 +649,7 @@ int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
   }
   // clusters that split the columns where the tiles leave SMs without work, with at least two steps of 32 columns for every warp
   int cluster = 1;
-  while (cluster < 8 && tiles * cluster < 4 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
+  while (cluster < 8 && tiles * cluster < 2 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
   {
     cluster *= 2;
   }
