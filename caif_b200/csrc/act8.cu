@@ -6,7 +6,7 @@
 // Why a power of two, which costs up to one of the code's eight bits against max|x| / 127: code * s is exact in bf16 and
 // fp32 (7 bits of significand), so x / s and the value need no rounding beyond the code's own and the backward pass
 // multiplies the very rows that caifq_act_unpack gives; and a block's scale is one byte.
-#include "common.cuh"
+#include "umma.cuh"
 
 namespace caifq
 {
@@ -336,35 +336,43 @@ int act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int64_t rows
 }
 
 
-// ---- reductions over tokens, any type: C[p, q] = factor * sum_m U[m, p] * V[m, q] ----
-// V may be packed rows.  gridDim.z slices the tokens; a slice's sums go to part[slice][p][q] and tn_finish_kernel adds the
-// slices in order and rounds once.
+// ---- reductions over tokens: both gradients of an adapter in one launch, and their sums over slices of tokens in a second ----
+//   dB[out, r] = factor * sum_m dy[m, out] * h[m, r]        dA[r, in] = factor * sum_m dH[m, r] * x[m, in], x packed
+// A slice's sums go to part[slice], dB's [out][r] and then dA's as [in][r]; gradients_kernel adds the slices in order and rounds
+// once, so that equal calls give equal bits.
 
+struct Gradients
+{
+  const void *dy;          // [m, out]
+  const void *h;           // [m, r]
+  const void *dh;          // [m, r]
+  const int8_t *x;         // [m, in]
+  const uint8_t *scales;   // [m, ceil(in / 32)]
+  float *part;
+  int dtype;               // of dy and h
+  int dh_dtype;
+  int out, in, r;
+};
+
+// any type and width: 32 x 32 tiles of the result, fp32 multiply-adds
 constexpr int kTnTile = 32;
 constexpr int kTnRows = 32;
 
-struct TnJob
-{
-  const void *u;           // [m, p]
-  const void *v;           // [m, q], or codes
-  const uint8_t *v_scales; // null: v holds floats
-  float *part;
-  int u_dtype, v_dtype;
-  int p, q;
-};
-
-__global__ void __launch_bounds__(256) act_tn_kernel(const TnJob j, int64_t m)
+__global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t m)
 {
   __shared__ float su[kTnRows][kTnTile + 1];
   __shared__ float sv[kTnRows][kTnTile + 1];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x;
-  const int p0 = blockIdx.y * kTnTile;
-  const int q0 = blockIdx.x * kTnTile;
+  const int tiles_b = (j.out + kTnTile - 1) / kTnTile;
+  const bool is_a = static_cast<int>(blockIdx.x) >= tiles_b;
+  const int wide = is_a ? j.in : j.out;   // the dimension that is not the rank
+  const int c0 = (static_cast<int>(blockIdx.x) - (is_a ? tiles_b : 0)) * kTnTile;
+  const int r0 = blockIdx.y * kTnTile;
   const int64_t begin = m * blockIdx.z / gridDim.z;
   const int64_t end = m * (blockIdx.z + 1) / gridDim.z;
-  const int blocks = (j.q + kActBlock - 1) / kActBlock;
+  const int blocks = (j.in + kActBlock - 1) / kActBlock;
   const int tq = tid % 16;
   const int tp = tid / 16;
   float c[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
@@ -375,16 +383,15 @@ __global__ void __launch_bounds__(256) act_tn_kernel(const TnJob j, int64_t m)
       const int col = e % kTnTile;
       const int64_t row = mb + e / kTnTile;
       float u = 0.0f, v = 0.0f;
-      if (row < end && p0 + col < j.p)
+      if (row < end && c0 + col < wide)
       {
-        u = load_as_float(j.u, row * j.p + p0 + col, j.u_dtype);
+        const int64_t at = row * wide + c0 + col;
+        u = is_a ? static_cast<float>(j.x[at]) * scale_of(j.scales[row * blocks + (c0 + col) / kActBlock])
+                 : load_as_float(j.dy, at, j.dtype);
       }
-      if (row < end && q0 + col < j.q)
+      if (row < end && r0 + col < j.r)
       {
-        const int64_t at = row * j.q + q0 + col;
-        v = j.v_scales != nullptr
-                ? static_cast<float>(static_cast<const int8_t *>(j.v)[at]) * scale_of(j.v_scales[row * blocks + (q0 + col) / kActBlock])
-                : load_as_float(j.v, at, j.v_dtype);
+        v = is_a ? load_as_float(j.dh, row * j.r + r0 + col, j.dh_dtype) : load_as_float(j.h, row * j.r + r0 + col, j.dtype);
       }
       su[e / kTnTile][col] = u;
       sv[e / kTnTile][col] = v;
@@ -404,49 +411,339 @@ __global__ void __launch_bounds__(256) act_tn_kernel(const TnJob j, int64_t m)
     }
     __syncthreads();
   }
-  float *part = j.part + static_cast<int64_t>(blockIdx.z) * j.p * j.q;
+  float *part = j.part + static_cast<int64_t>(blockIdx.z) * (static_cast<int64_t>(j.out) + j.in) * j.r +
+                (is_a ? static_cast<int64_t>(j.out) * j.r : 0);
 #pragma unroll
   for (int a = 0; a < 2; ++a)
   {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
     {
-      const int gp = p0 + tp * 2 + a;
-      const int gq = q0 + tq * 2 + b;
-      if (gp < j.p && gq < j.q)
+      const int col = c0 + tp * 2 + a;
+      const int rr = r0 + tq * 2 + b;
+      if (col < wide && rr < j.r)
       {
-        part[static_cast<int64_t>(gp) * j.q + gq] = c[a][b];
+        part[static_cast<int64_t>(col) * j.r + rr] = c[a][b];
       }
     }
   }
 }
 
-__global__ void __launch_bounds__(256)
-tn_finish_kernel(const float *part, void *out, int dtype, float factor, int slices, int64_t n)
+// bf16, ranks 8, 16, 32, 64, widths of whole 128-column tiles: the tensor core, as the adapter's reductions on full rows run it (both
+// operands have the token as their slow axis: tiles lie in shared memory as they come, fragments are read transposed).  A tile of
+// 64 tokens x 128 columns is 16 KB of dy, or 8 KB of codes, which become bf16 numbers on the way to shared memory: code * s has
+// seven bits of significand, so the products are those of the expanded rows.  Bound by HBM: dy and the codes once.
+constexpr int kTnColumns = 128;
+constexpr int kTnTokens = 64;
+constexpr int kTnPitch = kTnColumns + 8;   // bf16 elements: 272-byte rows keep the transposed reads free of conflicts
+
+__device__ __forceinline__ void tn_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
 {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// sixteen codes and their scale byte as bf16 numbers, exactly
+__device__ __forceinline__ void codes_to_bf16(const uint4 c, uint32_t byte, uint4 (&out)[2])
+{
+  const uint32_t s = (byte << 7) | (byte << 23);   // bf16 numbers of that exponent; infinite for 255: NaN with codes of 0
+  const uint4 p = expand_int8x8(make_uint2(c.x, c.y));
+  const uint4 q = expand_int8x8(make_uint2(c.z, c.w));
+  out[0] = make_uint4(mul_bf16x2(p.x, s), mul_bf16x2(p.y, s), mul_bf16x2(p.z, s), mul_bf16x2(p.w, s));
+  out[1] = make_uint4(mul_bf16x2(q.x, s), mul_bf16x2(q.y, s), mul_bf16x2(q.z, s), mul_bf16x2(q.w, s));
+}
+
+template <int NT>   // rank / 8
+__global__ void __launch_bounds__(256) act_tn_mma_kernel(const Gradients j, int64_t m)
+{
+  constexpr int R = 8 * NT;
+  __shared__ __align__(16) __nv_bfloat16 su[kTnTokens][kTnPitch];
+  __shared__ __align__(16) __nv_bfloat16 sv[kTnTokens][R + 8];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i < n)
+  const int tid = threadIdx.x;
+  const int warp = tid >> 5;
+  const int lane = tid & 31;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int tiles_b = j.out / kTnColumns;
+  const bool is_a = static_cast<int>(blockIdx.x) >= tiles_b;
+  const int c0 = (static_cast<int>(blockIdx.x) - (is_a ? tiles_b : 0)) * kTnColumns;
+  const int wide = is_a ? j.in : j.out;
+  const int64_t per = ((m + gridDim.y - 1) / gridDim.y + kTnTokens - 1) / kTnTokens * kTnTokens;
+  const int64_t begin = per * blockIdx.y;
+  const int64_t end = begin + per < m ? begin + per : m;
+  const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(is_a ? j.dh : j.h);
+  float c[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
   {
-    float s = 0.0f;
-#pragma unroll 4
-    for (int z = 0; z < slices; ++z)
+    c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+  }
+  // the next tile's loads are issued before this one's products: 16-byte pieces of dy (four a thread) or of codes (two, with
+  // their scale bytes), and of the thin operand
+  uint4 ru[4];
+  uint32_t rs[2];
+  uint4 rv[2];
+  auto fetch = [&](int64_t mb) {
+    if (is_a)
     {
-      s += part[static_cast<int64_t>(z) * n + i];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+      {
+        const int e = tid + i * 256;
+        const int64_t row = mb + (e >> 3);
+        const int col = c0 + (e & 7) * 16;
+        ru[i] = make_uint4(0u, 0u, 0u, 0u);
+        rs[i] = 1u;
+        if (row < end)
+        {
+          ru[i] = *reinterpret_cast<const uint4 *>(j.x + row * wide + col);
+          rs[i] = j.scales[row * (wide / kActBlock) + col / kActBlock];
+        }
+      }
     }
-    store_from_float(out, i, dtype, s * factor);
+    else
+    {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+      {
+        const int e = tid + i * 256;
+        const int64_t row = mb + (e >> 4);
+        ru[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < end)
+        {
+          ru[i] = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(j.dy) + row * wide + c0 + (e & 15) * 8);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+      const int e = tid + i * 256;
+      rv[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (e < kTnTokens * NT && mb + e / NT < end)
+      {
+        rv[i] = *reinterpret_cast<const uint4 *>(v + (mb + e / NT) * R + (e % NT) * 8);
+      }
+    }
+  };
+  if (begin < end)
+  {
+    fetch(begin);
+  }
+  for (int64_t mb = begin; mb < end; mb += kTnTokens)
+  {
+    if (is_a)
+    {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+      {
+        const int e = tid + i * 256;
+        uint4 o[2];
+        codes_to_bf16(ru[i], rs[i], o);
+        uint4 *dst = reinterpret_cast<uint4 *>(&su[e >> 3][(e & 7) * 16]);
+        dst[0] = o[0];
+        dst[1] = o[1];
+      }
+    }
+    else
+    {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+      {
+        const int e = tid + i * 256;
+        *reinterpret_cast<uint4 *>(&su[e >> 4][(e & 15) * 8]) = ru[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+      const int e = tid + i * 256;
+      if (e < kTnTokens * NT)
+      {
+        *reinterpret_cast<uint4 *>(&sv[e / NT][(e % NT) * 8]) = rv[i];
+      }
+    }
+    __syncthreads();
+    if (mb + kTnTokens < end)
+    {
+      fetch(mb + kTnTokens);
+    }
+#pragma unroll
+    for (int k16 = 0; k16 < kTnTokens / 16; ++k16)
+    {
+      // rows of the product: this warp's 16 columns; lane l addresses row (l & 7) of 8 x 8 tile (l >> 3)
+      const int tile = lane >> 3;
+      uint32_t a0, a1, a2, a3;
+      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                   : "r"(smem_u32(&su[k16 * 16 + (tile >> 1) * 8 + (lane & 7)][warp * 16 + (tile & 1) * 8])));
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+      {
+        uint32_t b0, b1;
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                     : "=r"(b0), "=r"(b1)
+                     : "r"(smem_u32(&sv[k16 * 16 + (lane & 15)][nt * 8])));
+        tn_mma(c[nt], a0, a1, a2, a3, b0, b1);
+      }
+    }
+    __syncthreads();
+  }
+  float *part = j.part + static_cast<int64_t>(blockIdx.y) * (static_cast<int64_t>(j.out) + j.in) * R +
+                (is_a ? static_cast<int64_t>(j.out) * R : 0);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+  {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      const int64_t col = c0 + warp * 16 + g + 8 * half;
+      *reinterpret_cast<float2 *>(part + col * R + nt * 8 + 2 * t) = make_float2(c[nt][2 * half], c[nt][2 * half + 1]);
+    }
   }
 }
 
-int tn_slices(int64_t m, int p, int q)
+// the slices' sums, rounded once: [out][r] as it lies, [in][r] turned to [r, in]
+__global__ void __launch_bounds__(256)
+gradients_kernel(const float *part, void *d_b, void *d_a, int dtype, float factor, int slices, int64_t n_b, int in, int r)
 {
-  const int64_t tiles = static_cast<int64_t>((p + kTnTile - 1) / kTnTile) * ((q + kTnTile - 1) / kTnTile);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t n = n_b + static_cast<int64_t>(in) * r;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n)
+  {
+    return;
+  }
+  float s = 0.0f;
+#pragma unroll 4
+  for (int z = 0; z < slices; ++z)
+  {
+    s += part[static_cast<int64_t>(z) * n + i];
+  }
+  if (i < n_b)
+  {
+    store_from_float(d_b, i, dtype, s * factor);
+  }
+  else
+  {
+    const int64_t e = i - n_b;
+    store_from_float(d_a, (e % r) * in + e / r, dtype, s * factor);
+  }
+}
+
+// ---- what the general form of the backward pass multiplies by itself ----
+
+constexpr int kDhChunk = 1024;
+
+// dH[m, r] = dy . B, fp32: a block a row.  B's rows lie one behind the other, so the block reads it as one run of numbers and a
+// thread always meets the same column of it; the row of dy waits in shared memory.
+__global__ void __launch_bounds__(256)
+dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r)
+{
+  __shared__ float row[kDhChunk];
+  __shared__ float sums[256];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tid = threadIdx.x;
+  const int64_t at = blockIdx.x;
+  for (int j0 = 0; j0 < r; j0 += 256)
+  {
+    const int width = r - j0 < 256 ? r - j0 : 256;   // columns of this trip
+    const int groups = 256 / width;                  // rows of B at a time
+    const int j = tid % width;
+    const int group = tid / width;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = 0; c0 < out; c0 += kDhChunk)
+    {
+      const int n = out - c0 < kDhChunk ? out - c0 : kDhChunk;
+      __syncthreads();   // the chunk before has been read
+      for (int i = tid; i < n; i += 256)
+      {
+        row[i] = load_as_float(dy, at * out + c0 + i, dtype);
+      }
+      __syncthreads();
+      if (group < groups)
+      {
+        int o = group;
+        for (; o + 3 * groups < n; o += 4 * groups)
+        {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+          {
+            s[u] = fmaf(row[o + u * groups], load_as_float(b, static_cast<int64_t>(c0 + o + u * groups) * r + j0 + j, dtype), s[u]);
+          }
+        }
+        for (; o < n; o += groups)
+        {
+          s[0] = fmaf(row[o], load_as_float(b, static_cast<int64_t>(c0 + o) * r + j0 + j, dtype), s[0]);
+        }
+      }
+    }
+    __syncthreads();
+    sums[tid] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (tid < width)
+    {
+      float v = 0.0f;
+      for (int i = 0; i < groups; ++i)
+      {
+        v += sums[i * width + tid];
+      }
+      dh[at * r + j0 + tid] = v;
+    }
+  }
+}
+
+// dx[m, in] = factor * dH . A: a thread a column
+__global__ void __launch_bounds__(256)
+dx_adapter_kernel(const float *dh, const void *a, void *dx, int dtype, float factor, int in, int r)
+{
+  __shared__ float row[256];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t at = blockIdx.x;
+  const int c = blockIdx.y * 256 + static_cast<int>(threadIdx.x);
+  float s = 0.0f;
+  for (int j0 = 0; j0 < r; j0 += 256)
+  {
+    __syncthreads();
+    if (j0 + static_cast<int>(threadIdx.x) < r)
+    {
+      row[threadIdx.x] = dh[at * r + j0 + threadIdx.x];
+    }
+    __syncthreads();
+    const int n = r - j0 < 256 ? r - j0 : 256;
+    if (c < in)
+    {
+#pragma unroll 8
+      for (int j = 0; j < n; ++j)
+      {
+        s = fmaf(row[j], load_as_float(a, static_cast<int64_t>(j0 + j) * in + c, dtype), s);
+      }
+    }
+  }
+  if (c < in)
+  {
+    store_from_float(dx, at * in + c, dtype, s * factor);
+  }
+}
+
+// slices of tokens: four blocks an SM, no slice without tokens
+int tn_slices(int64_t m, int64_t tiles, int tokens)
+{
   int64_t n = (148 * 4 + tiles - 1) / tiles;
-  const int64_t most = (m + kTnRows - 1) / kTnRows;
+  const int64_t most = (m + tokens - 1) / tokens;
   n = n > most ? most : n;
-  n = n > 64 ? 64 : n;
   return static_cast<int>(n < 1 ? 1 : n);
+}
+
+int64_t general_tiles(int out, int in, int r)
+{
+  return static_cast<int64_t>((out + kTnTile - 1) / kTnTile + (in + kTnTile - 1) / kTnTile) * ((r + kTnTile - 1) / kTnTile);
 }
 
 }  // namespace
@@ -485,23 +782,57 @@ int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int d
   }
 }
 
-// fp32 scratch of launch_act_tn
-size_t act_tn_scratch_bytes(int64_t m, int p, int q)
+// fp32 scratch of launch_act_gradients; never less for more rows
+size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r)
 {
-  return static_cast<size_t>(tn_slices(m, p, q)) * static_cast<size_t>(p) * static_cast<size_t>(q) * sizeof(float);
+  const int64_t general = tn_slices(m, general_tiles(out, in, r), kTnRows);
+  const int64_t tiled = tn_slices(m, (out + in + kTnColumns - 1) / kTnColumns, kTnTokens);
+  return static_cast<size_t>(general > tiled ? general : tiled) * (static_cast<size_t>(out) + in) * r * sizeof(float);
 }
 
-// out[p, q] = factor * sum over tokens of u[m, p] * v[m, q]; v_scales != null: v is packed rows.  m >= 1
-int launch_act_tn(const void *u, int u_dtype, const void *v, int v_dtype, const uint8_t *v_scales, void *out, int out_dtype,
-                  float factor, float *scratch, int64_t m, int p, int q, cudaStream_t s)
+// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * dh^T . x, x packed.  m >= 1; dy, h, d_a, d_b in dtype
+int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
+                         void *d_b, void *d_a, int dtype, float factor, float *scratch, int64_t m, int out, int in, int r,
+                         cudaStream_t s)
 {
-  const int slices = tn_slices(m, p, q);
-  const TnJob job{u, v, v_scales, scratch, u_dtype, v_dtype, p, q};
-  const dim3 grid((q + kTnTile - 1) / kTnTile, (p + kTnTile - 1) / kTnTile, static_cast<unsigned>(slices));
-  CAIFQ_CHECK_CUDA(launch_dependent(act_tn_kernel, grid, dim3(256), 0, s, job, m));
-  const int64_t n = static_cast<int64_t>(p) * q;
-  CAIFQ_CHECK_CUDA(launch_dependent(tn_finish_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s,
-                                    static_cast<const float *>(scratch), out, out_dtype, factor, slices, n));
+  const Gradients j{dy, h, dh, x, scales, scratch, dtype, dh_dtype, out, in, r};
+  auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  int slices = 0;
+  if (dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
+      (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(x))
+  {
+    const int tiles = (out + in) / kTnColumns;
+    slices = tn_slices(m, tiles, kTnTokens);
+    auto kernel = r == 8 ? act_tn_mma_kernel<1>
+                         : (r == 16 ? act_tn_mma_kernel<2> : (r == 32 ? act_tn_mma_kernel<4> : act_tn_mma_kernel<8>));
+    CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(slices)), dim3(256), 0, s, j, m));
+  }
+  else
+  {
+    slices = tn_slices(m, general_tiles(out, in, r), kTnRows);
+    const dim3 grid((out + kTnTile - 1) / kTnTile + (in + kTnTile - 1) / kTnTile, (r + kTnTile - 1) / kTnTile,
+                    static_cast<unsigned>(slices));
+    CAIFQ_CHECK_CUDA(launch_dependent(act_tn_kernel, grid, dim3(256), 0, s, j, m));
+  }
+  const int64_t n = (static_cast<int64_t>(out) + in) * r;
+  CAIFQ_CHECK_CUDA(launch_dependent(gradients_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s,
+                                    static_cast<const float *>(scratch), d_b, d_a, dtype, factor, slices,
+                                    static_cast<int64_t>(out) * r, in, r));
+  return CAIFQ_OK;
+}
+
+// dh[m, r] (fp32) = dy . b, dy and b in dtype
+int launch_dh(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r, cudaStream_t s)
+{
+  CAIFQ_CHECK_CUDA(launch_dependent(dh_kernel, dim3(static_cast<unsigned>(m)), dim3(256), 0, s, dy, b, dh, dtype, m, out, r));
+  return CAIFQ_OK;
+}
+
+// dx[m, in] = factor * dh . a, dx and a in dtype
+int launch_dx_adapter(const float *dh, const void *a, void *dx, int dtype, float factor, int64_t m, int in, int r, cudaStream_t s)
+{
+  CAIFQ_CHECK_CUDA(launch_dependent(dx_adapter_kernel, dim3(static_cast<unsigned>(m), (in + 255) / 256), dim3(256), 0, s, dh, a, dx,
+                                    dtype, factor, in, r));
   return CAIFQ_OK;
 }
 

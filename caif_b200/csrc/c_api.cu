@@ -138,9 +138,12 @@ int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_r
 // act8.cu
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
-size_t act_tn_scratch_bytes(int64_t m, int p, int q);
-int launch_act_tn(const void *u, int u_dtype, const void *v, int v_dtype, const uint8_t *v_scales, void *out, int out_dtype,
-                  float factor, float *scratch, int64_t m, int p, int q, cudaStream_t s);
+size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r);
+int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
+                         void *d_b, void *d_a, int dtype, float factor, float *scratch, int64_t m, int out, int in, int r,
+                         cudaStream_t s);
+int launch_dh(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r, cudaStream_t s);
+int launch_dx_adapter(const float *dh, const void *a, void *dx, int dtype, float factor, int64_t m, int in, int r, cudaStream_t s);
 // layernorm.cu
 size_t layernorm_bwd_workspace_bytes(int rows, int dim);
 int launch_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
@@ -1243,7 +1246,7 @@ struct PackedBwdWs
 {
   LoraBwdWs lora;
   size_t weight;   // the expanded weight, where there is one
-  size_t sums;     // fp32, of one reduction over tokens at a time
+  size_t sums;     // fp32, of the reductions over tokens
   size_t total;
 };
 
@@ -1253,9 +1256,7 @@ PackedBwdWs packed_bwd_ws(const caifq_weight *w, const caifq_lora *l, int64_t m,
   o.lora = lora_bwd_ws(w, l, m);
   o.weight = o.lora.total;
   o.sums = o.weight + (expand_ok(w, l, kAlignedProbe, m, compute_dtype) ? expanded_weight_bytes(w) : 0);
-  const size_t b = act_tn_scratch_bytes(m, w->out_dim, l->rank);
-  const size_t a = act_tn_scratch_bytes(m, l->rank, w->in_dim);
-  o.total = o.sums + align256(a > b ? a : b);
+  o.total = o.sums + align256(act_gradients_scratch_bytes(m, w->out_dim, w->in_dim, l->rank));
   return o;
 }
 }  // namespace
@@ -1280,6 +1281,7 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
     return rc;
   }
   CAIFQ_CHECK_ARG(m >= 0, "%s: negative m", who);
+  CAIFQ_CHECK_ARG(m <= 0x7FFFFFFF, "%s: %lld rows", who, static_cast<long long>(m));
   CAIFQ_CHECK_ARG(is_float_dtype(compute_dtype), "%s: the compute dtype must be F32, F16 or BF16", who);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sd = lora->dtype;
@@ -1316,11 +1318,8 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
     }
     if (r == CAIFQ_OK)
     {
-      r = launch_act_tn(dy, sd, hidden, sd, nullptr, d_b, sd, scale, sums, m, w->out_dim, lora->rank, s);
-    }
-    if (r == CAIFQ_OK)
-    {
-      r = launch_act_tn(d_hidden, sd, x_codes, CAIFQ_I8, x_scales, d_a, sd, scale, sums, m, lora->rank, w->in_dim, s);
+      r = launch_act_gradients(dy, hidden, d_hidden, sd, x_codes, x_scales, d_b, d_a, sd, scale, sums, m, w->out_dim, w->in_dim,
+                               lora->rank, s);
     }
     if (r != CAIFQ_OK)
     {
@@ -1330,26 +1329,18 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
     return linear_any(expand ? &wbf : w, true, dy, sd, 1.0f, m, dx, sd, false, compute_dtype, s, who, base + ws.lora.dhs,
                       base + ws.lora.ap, expand ? epilogue_scale_ptr(w) : nullptr);
   }
-  // dH = dy . B stays in fp32, and with it the adapter's products
-  int r = launch_act_tn(dy, sd, hidden, sd, nullptr, d_b, sd, scale, sums, m, w->out_dim, lora->rank, s);
-  if (r != CAIFQ_OK)
+  // dH = dy . B stays in fp32, and with it the adapter's products: both gradients, then dx = (scale dH) . A and the frozen base on
+  // top
+  int r = launch_dh(dy, lora->b, static_cast<float *>(d_hidden), sd, m, w->out_dim, lora->rank, s);
+  if (r == CAIFQ_OK)
   {
-    return r;
+    r = launch_act_gradients(dy, hidden, d_hidden, CAIFQ_F32, x_codes, x_scales, d_b, d_a, sd, scale, sums, m, w->out_dim,
+                             w->in_dim, lora->rank, s);
   }
-  const caifq_weight fb = float_weight(lora->b, sd, w->out_dim, lora->rank);
-  r = linear_any(&fb, true, dy, sd, 1.0f, m, d_hidden, CAIFQ_F32, false, CAIFQ_F32, s, who);
-  if (r != CAIFQ_OK)
+  if (r == CAIFQ_OK)
   {
-    return r;
+    r = launch_dx_adapter(static_cast<const float *>(d_hidden), lora->a, dx, sd, scale, m, w->in_dim, lora->rank, s);
   }
-  r = launch_act_tn(d_hidden, CAIFQ_F32, x_codes, CAIFQ_I8, x_scales, d_a, sd, scale, sums, m, lora->rank, w->in_dim, s);
-  if (r != CAIFQ_OK)
-  {
-    return r;
-  }
-  // dx = (scale dH) . A, then the frozen base on top
-  const caifq_weight fa = float_weight(lora->a, sd, lora->rank, w->in_dim);
-  r = linear_any(&fa, true, d_hidden, CAIFQ_F32, scale, m, dx, sd, false, CAIFQ_F32, s, who);
   if (r != CAIFQ_OK)
   {
     return r;
