@@ -357,6 +357,7 @@ struct Gradients
 // any type and width: 32 x 32 tiles of the result, fp32 multiply-adds
 constexpr int kTnTile = 32;
 constexpr int kTnRows = 32;
+constexpr int kTnGeneralBlocks = 6;   // an SM
 
 __global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t m)
 {
@@ -454,8 +455,12 @@ __device__ __forceinline__ void codes_to_bf16(const uint4 c, uint32_t byte, uint
   out[1] = make_uint4(mul_bf16x2(q.x, s), mul_bf16x2(q.y, s), mul_bf16x2(q.z, s), mul_bf16x2(q.w, s));
 }
 
+// blocks an SM: the accumulators of large ranks leave room for two
+template <int NT>
+constexpr int kTnBlocks = NT <= 2 ? 4 : 2;
+
 template <int NT>   // rank / 8
-__global__ void __launch_bounds__(256) act_tn_mma_kernel(const Gradients j, int64_t m)
+__global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gradients j, int64_t m)
 {
   constexpr int R = 8 * NT;
   __shared__ __align__(16) __nv_bfloat16 su[kTnTokens][kTnPitch];
@@ -606,6 +611,106 @@ __global__ void __launch_bounds__(256) act_tn_mma_kernel(const Gradients j, int6
   }
 }
 
+// dH[m, r] = dy . B for the same adapters, with the transposed copy bt[r, out] of B: bf16, and times `mul` / *div, padded to 64 columns, as the
+// extra k-block of the product that gives dx.  A block takes 32 rows, so that bt crosses the SM's cache once for 32 rows and not once for
+// 16 (8192 x 4096, rank 16: it is as many bytes as 16 rows of dy); eight warps split the columns, in 16-byte pieces straight into
+// fragments (the order of the columns inside a fragment is the same for both operands).
+template <int NT>
+__global__ void __launch_bounds__(256, NT <= 2 ? 3 : 2)
+act_nt_mma_kernel(const __nv_bfloat16 *dy, const __nv_bfloat16 *bt, __nv_bfloat16 *dh, __nv_bfloat16 *padded, float mul,
+                  const float *div, int64_t m, int out)
+{
+  constexpr int R = 8 * NT;
+  __shared__ float part[8][16][R + 1];
+  asm volatile("griddepcontrol.wait;" : "+l"(dy), "+l"(bt), "+l"(div)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 32;
+  const int steps = out / 32;
+  const int begin = steps * warp / 8;
+  const int end = steps * (warp + 1) / 8;
+  const uint4 *src[4];
+  bool live[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+  {
+    live[i] = row0 + g + 8 * i < m;
+    src[i] = reinterpret_cast<const uint4 *>(dy + (live[i] ? row0 + g + 8 * i : 0) * out) + t;
+  }
+  const uint4 *b_row = reinterpret_cast<const uint4 *>(bt + static_cast<int64_t>(g) * out) + t;
+  float c[2][NT][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+  {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+    {
+      c[i][nt][0] = c[i][nt][1] = c[i][nt][2] = c[i][nt][3] = 0.0f;
+    }
+  }
+#pragma unroll 2
+  for (int st = begin; st < end; ++st)
+  {
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+      v[i] = live[i] ? __ldg(src[i] + st * 4) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+    {
+      const uint4 w = __ldg(b_row + static_cast<int64_t>(nt) * out + st * 4);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+      {
+        tn_mma(c[i][nt], v[2 * i].x, v[2 * i + 1].x, v[2 * i].y, v[2 * i + 1].y, w.x, w.y);
+        tn_mma(c[i][nt], v[2 * i].z, v[2 * i + 1].z, v[2 * i].w, v[2 * i + 1].w, w.z, w.w);
+      }
+    }
+  }
+  const float factor = div != nullptr ? mul / __ldg(div) : mul;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)   // sixteen rows at a time
+  {
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+    {
+      part[warp][g][nt * 8 + 2 * t] = c[i][nt][0];
+      part[warp][g][nt * 8 + 2 * t + 1] = c[i][nt][1];
+      part[warp][g + 8][nt * 8 + 2 * t] = c[i][nt][2];
+      part[warp][g + 8][nt * 8 + 2 * t + 1] = c[i][nt][3];
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * 32; e += 256)
+    {
+      const int64_t row = row0 + 16 * i + (e >> 5);
+      const int col = (e & 31) * 2;
+      if (row < m)
+      {
+        uint32_t pad = 0u;
+        if (col < R)
+        {
+          float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int w = 0; w < 8; ++w)
+          {
+            sum.x += part[w][e >> 5][col];
+            sum.y += part[w][e >> 5][col + 1];
+          }
+          *reinterpret_cast<uint32_t *>(dh + row * R + col) = pack_bf16x2(sum.x, sum.y);
+          pad = pack_bf16x2(sum.x * factor, sum.y * factor);
+        }
+        *reinterpret_cast<uint32_t *>(padded + row * 64 + col) = pad;
+      }
+    }
+  }
+}
+
 // the slices' sums, rounded once: [out][r] as it lies, [in][r] turned to [r, in]
 __global__ void __launch_bounds__(256)
 gradients_kernel(const float *part, void *d_b, void *d_a, int dtype, float factor, int slices, int64_t n_b, int in, int r)
@@ -656,7 +761,7 @@ dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int ou
     const int groups = 256 / width;                  // rows of B at a time
     const int j = tid % width;
     const int group = tid / width;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // (sixteen loads on their way, four chains of additions)
     for (int c0 = 0; c0 < out; c0 += kDhChunk)
     {
       const int n = out - c0 < kDhChunk ? out - c0 : kDhChunk;
@@ -669,12 +774,18 @@ dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int ou
       if (group < groups)
       {
         int o = group;
-        for (; o + 3 * groups < n; o += 4 * groups)
+        for (; o + 15 * groups < n; o += 16 * groups)
         {
+          float w[16];
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
+          for (int u = 0; u < 16; ++u)
           {
-            s[u] = fmaf(row[o + u * groups], load_as_float(b, static_cast<int64_t>(c0 + o + u * groups) * r + j0 + j, dtype), s[u]);
+            w[u] = load_as_float(b, static_cast<int64_t>(c0 + o + u * groups) * r + j0 + j, dtype);
+          }
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+          {
+            s[u & 3] = fmaf(row[o + u * groups], w[u], s[u & 3]);
           }
         }
         for (; o < n; o += groups)
@@ -732,10 +843,10 @@ dx_adapter_kernel(const float *dh, const void *a, void *dx, int dtype, float fac
   }
 }
 
-// slices of tokens: four blocks an SM, no slice without tokens
-int tn_slices(int64_t m, int64_t tiles, int tokens)
+// slices of tokens: as many as one wave of `blocks` an SM holds, no slice without tokens
+int tn_slices(int64_t m, int64_t tiles, int tokens, int blocks)
 {
-  int64_t n = (148 * 4 + tiles - 1) / tiles;
+  int64_t n = 148 * blocks / tiles;
   const int64_t most = (m + tokens - 1) / tokens;
   n = n > most ? most : n;
   return static_cast<int>(n < 1 ? 1 : n);
@@ -785,8 +896,8 @@ int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int d
 // fp32 scratch of launch_act_gradients; never less for more rows
 size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r)
 {
-  const int64_t general = tn_slices(m, general_tiles(out, in, r), kTnRows);
-  const int64_t tiled = tn_slices(m, (out + in + kTnColumns - 1) / kTnColumns, kTnTokens);
+  const int64_t general = tn_slices(m, general_tiles(out, in, r), kTnRows, kTnGeneralBlocks);
+  const int64_t tiled = tn_slices(m, (out + in + kTnColumns - 1) / kTnColumns, kTnTokens, r <= 16 ? kTnBlocks<2> : kTnBlocks<8>);
   return static_cast<size_t>(general > tiled ? general : tiled) * (static_cast<size_t>(out) + in) * r * sizeof(float);
 }
 
@@ -802,14 +913,14 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
       (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(x))
   {
     const int tiles = (out + in) / kTnColumns;
-    slices = tn_slices(m, tiles, kTnTokens);
+    slices = tn_slices(m, tiles, kTnTokens, r <= 16 ? kTnBlocks<2> : kTnBlocks<8>);
     auto kernel = r == 8 ? act_tn_mma_kernel<1>
                          : (r == 16 ? act_tn_mma_kernel<2> : (r == 32 ? act_tn_mma_kernel<4> : act_tn_mma_kernel<8>));
     CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(slices)), dim3(256), 0, s, j, m));
   }
   else
   {
-    slices = tn_slices(m, general_tiles(out, in, r), kTnRows);
+    slices = tn_slices(m, general_tiles(out, in, r), kTnRows, kTnGeneralBlocks);
     const dim3 grid((out + kTnTile - 1) / kTnTile + (in + kTnTile - 1) / kTnTile, (r + kTnTile - 1) / kTnTile,
                     static_cast<unsigned>(slices));
     CAIFQ_CHECK_CUDA(launch_dependent(act_tn_kernel, grid, dim3(256), 0, s, j, m));
@@ -818,6 +929,19 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
   CAIFQ_CHECK_CUDA(launch_dependent(gradients_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s,
                                     static_cast<const float *>(scratch), d_b, d_a, dtype, factor, slices,
                                     static_cast<int64_t>(out) * r, in, r));
+  return CAIFQ_OK;
+}
+
+// dh[m, r] = dy . bt^T in bf16 and padded[m, 64] = bf16(dh * mul / *div): bf16 operands on 16-byte boundaries, r 8, 16, 32 or 64, out a
+// multiple of 32, m >= 1
+int launch_act_nt(const void *dy, const void *bt, void *dh, void *padded, float mul, const float *div, int64_t m, int out, int r,
+                  cudaStream_t s)
+{
+  auto kernel = r == 8 ? act_nt_mma_kernel<1>
+                       : (r == 16 ? act_nt_mma_kernel<2> : (r == 32 ? act_nt_mma_kernel<4> : act_nt_mma_kernel<8>));
+  CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>((m + 31) / 32)), dim3(256), 0, s,
+                                    static_cast<const __nv_bfloat16 *>(dy), static_cast<const __nv_bfloat16 *>(bt),
+                                    static_cast<__nv_bfloat16 *>(dh), static_cast<__nv_bfloat16 *>(padded), mul, div, m, out));
   return CAIFQ_OK;
 }
 

@@ -142,6 +142,8 @@ size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r);
 int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
                          void *d_b, void *d_a, int dtype, float factor, float *scratch, int64_t m, int out, int in, int r,
                          cudaStream_t s);
+int launch_act_nt(const void *dy, const void *bt, void *dh, void *padded, float mul, const float *div, int64_t m, int out, int r,
+                  cudaStream_t s);
 int launch_dh(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r, cudaStream_t s);
 int launch_dx_adapter(const float *dh, const void *a, void *dx, int dtype, float factor, int64_t m, int in, int r, cudaStream_t s);
 // layernorm.cu
@@ -1250,6 +1252,8 @@ struct PackedBwdWs
   size_t total;
 };
 
+constexpr int64_t kActNtLeast = 2048;
+
 PackedBwdWs packed_bwd_ws(const caifq_weight *w, const caifq_lora *l, int64_t m, int compute_dtype)
 {
   PackedBwdWs o{};
@@ -1313,8 +1317,11 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
                                   nullptr, 0, lora->rank, s);
     if (r == CAIFQ_OK)
     {
-      r = launch_skinny_nt(dy, base + ws.lora.bt, d_hidden, base + ws.lora.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
-                           w->out_dim, lora->rank, false, s);
+      // (few rows: the columns want more blocks than there are 32 rows)
+      r = m > kActNtLeast ? launch_act_nt(dy, base + ws.lora.bt, d_hidden, base + ws.lora.dhs, scale, epilogue_scale_ptr(w), m, w->out_dim,
+                                          lora->rank, s)
+                          : launch_skinny_nt(dy, base + ws.lora.bt, d_hidden, base + ws.lora.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
+                                             w->out_dim, lora->rank, false, s);
     }
     if (r == CAIFQ_OK)
     {
