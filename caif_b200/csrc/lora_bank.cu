@@ -128,13 +128,13 @@ bank_up_kernel(const float *frozen, const float *h, const int32_t *__restrict__ 
 
 // ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on tiles of up to 16 rows of one adapter ----
 // Rows are dealt to tiles by adapter first, wherever they stand in the batch (those without one make tiles of their own, which
-// `up` copies).  A call of up to 256 rows does that inside every block of `down`, longer ones in a launch ahead of it.  Tiles
+// `up` copies).  In a call of up to 128 rows every block does that by itself, longer ones have a launch for it.  Tiles
 // of neighbouring rows as they lie, with a turn for every adapter that they name, need neither; but 200 decoding sequences of
 // 24 adapters are then 13 tiles of 14 turns, which held up `up` for 28 us beside 131 tiles of prompts, and here they are 24.
 // Which tile and slot a row gets does not change its arithmetic, so results do not depend on the rows' order.
 
 constexpr int kTileRows = 16;
-constexpr int kSmallCall = 256;     // rows that a block of `down` sorts by itself
+constexpr int kSmallCall = 128;     // rows that a block sorts by itself
 constexpr int kTableMost = 4096;    // adapters that the launch ahead counts in shared memory
 
 // what `down` leaves for `up`, in the workspace
@@ -289,7 +289,8 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// the rows and adapter of tile `tile` of a call of m <= kSmallCall rows; false: there is no such tile.  All 256 threads.
+// the rows and adapter of tile `tile` of a call of m <= kSmallCall rows; false: there is no such tile.  All threads of the block
+// (kSmallCall or more).
 __device__ __forceinline__ bool small_tile(const int32_t *adapter_of_row, const caifq_lora_entry *entries, int count, int m, int tile,
                                            int (&rows)[kTileRows], caifq_lora_entry &entry)
 {
@@ -298,32 +299,35 @@ __device__ __forceinline__ bool small_tile(const int32_t *adapter_of_row, const 
   __shared__ int lead[2];   // the row that begins the tile, and how many of its adapter come before it
   const int i = threadIdx.x;
   const int id = i < m ? group_of(adapter_of_row, i, count) : -1;
-  id_of[i] = id;
+  if (i < kSmallCall)
+  {
+    id_of[i] = id;
+  }
   if (i < kTileRows)
   {
     rows[i] = -1;
   }
   __syncthreads();
   int before = 0;
-  for (int k = 0; k < m; ++k)
+  for (int k = 0; k < (i < m ? i : 0); ++k)
   {
-    before += k < i && id_of[k] == id ? 1 : 0;
+    before += id_of[k] == id ? 1 : 0;
   }
   const bool begins = i < m && before % kTileRows == 0;
   const uint32_t mask = __ballot_sync(0xFFFFFFFFu, begins);
-  if ((i & 31) == 0)
+  if ((i & 31) == 0 && i < kSmallCall)
   {
     warp_tiles[i >> 5] = __popc(mask);
   }
   __syncthreads();
-  int tiles = 0, mine = __popc(mask & ((1u << (i & 31)) - 1u));
+  int tiles = 0, earlier = 0;
 #pragma unroll
   for (int w = 0; w < kSmallCall / 32; ++w)
   {
-    mine += w < (i >> 5) ? warp_tiles[w] : 0;
+    earlier += w < (i >> 5) ? warp_tiles[w] : 0;
     tiles += warp_tiles[w];
   }
-  if (begins && mine == tile)
+  if (begins && earlier + __popc(mask & ((1u << (i & 31)) - 1u)) == tile)
   {
     lead[0] = i;
     lead[1] = before;
@@ -358,7 +362,8 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
   __shared__ float part[8][kTileRows][NT * 8 + 1];
   __shared__ int rows[kTileRows];
   __shared__ caifq_lora_entry entry;
-  // (what invariant loads read is addressed out of the wait, so that they stay behind it)
+  // (what invariant loads read is addressed out of the wait, so that they stay behind it.  The wait comes before the next launch is
+  // let in: `up` relies on it)
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5;
@@ -370,26 +375,7 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
   if constexpr (SMALL)
   {
     // (every block of a cluster finds the same)
-    const bool any = small_tile(adapter_of_row, entries, count, static_cast<int>(m), static_cast<int>(tile), rows, entry);
-    if (rank_in_cluster == 0)
-    {
-      if (threadIdx.x == 0)
-      {
-        if (any)
-        {
-          plan.entry[tile] = entry;
-        }
-        else
-        {
-          plan.entry[tile].rank = -1;
-        }
-      }
-      if (any && threadIdx.x < kTileRows)
-      {
-        plan.rows[tile * kTileRows + threadIdx.x] = rows[threadIdx.x];
-      }
-    }
-    if (!any)
+    if (!small_tile(adapter_of_row, entries, count, static_cast<int>(m), static_cast<int>(tile), rows, entry))
     {
       return;
     }
@@ -501,20 +487,44 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
 // y of a tile's rows and 128 * GROUPS columns: a warp GROUPS times 32.  h enters as two bf16 terms (2^-16 relative).  The columns
 // of a group of 32 are dealt out to its four 8-wide tiles so that a lane ends with eight neighbouring ones of a row.  Bound by
 // latency (tile, then operands, then results) at few rows and by the frozen product's 4 bytes and y's 2 at many.
-template <int KS, int GROUPS>   // KS: sixteens of the largest rank
+//
+// A short call's block finds its rows and fetches its rows of B before it waits for the frozen product: what it reads for that was
+// complete before `down`, which waited for it, let the frozen product's launch in, and with it this one.
+template <int KS, int GROUPS, bool SMALL>   // KS: sixteens of the largest rank
 __global__ void __launch_bounds__(128)
-bank_up_mma_kernel(const float *frozen, const BankPlan plan, __nv_bfloat16 *y, int ld, int out_dim)
+bank_up_mma_kernel(const float *frozen, const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries,
+                   int count, int64_t m, const BankPlan plan, __nv_bfloat16 *y, int ld, int out_dim)
 {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int rows[kTileRows];
+  __shared__ caifq_lora_entry entry_of_tile;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2;
   const int t = lane & 3;
   const int64_t tile = blockIdx.x;
   const int col0 = (static_cast<int>(blockIdx.y) * 4 + warp) * 32 * GROUPS;
-  const caifq_lora_entry entry = plan.entry[tile];
-  const int32_t row_of[2] = {plan.rows[tile * kTileRows + g], plan.rows[tile * kTileRows + g + 8]};
+  caifq_lora_entry entry;
+  int32_t row_of[2];
+  if constexpr (SMALL)
+  {
+    if (!small_tile(adapter_of_row, entries, count, static_cast<int>(m), static_cast<int>(tile), rows, entry_of_tile))
+    {
+      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+      asm volatile("griddepcontrol.wait;" ::: "memory");   // (whoever follows relies on it)
+      return;
+    }
+    entry = entry_of_tile;
+    row_of[0] = rows[g];
+    row_of[1] = rows[g + 8];
+  }
+  else
+  {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    entry = plan.entry[tile];
+    row_of[0] = plan.rows[tile * kTileRows + g];
+    row_of[1] = plan.rows[tile * kTileRows + g + 8];
+  }
   const int rank = entry.rank;
   if (rank < 0)
   {
@@ -522,21 +532,6 @@ bank_up_mma_kernel(const float *frozen, const BankPlan plan, __nv_bfloat16 *y, i
   }
   const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entry.b);
   uint2 w[GROUPS][KS][4];
-  float4 f[GROUPS][2][2];
-  float4 v[KS][2];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks)
-  {
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-    {
-      v[ks][half] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (row_of[half] >= 0 && 16 * ks + 4 * t < rank)
-      {
-        v[ks][half] = *reinterpret_cast<const float4 *>(plan.h + (tile * kTileRows + g + 8 * half) * ld + 16 * ks + 4 * t);
-      }
-    }
-  }
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i)
   {
@@ -554,6 +549,30 @@ bank_up_mma_kernel(const float *frozen, const BankPlan plan, __nv_bfloat16 *y, i
         }
       }
     }
+  }
+  if constexpr (SMALL)
+  {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+  }
+  float4 v[KS][2];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+  {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      v[ks][half] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (row_of[half] >= 0 && 16 * ks + 4 * t < rank)
+      {
+        v[ks][half] = *reinterpret_cast<const float4 *>(plan.h + (tile * kTileRows + g + 8 * half) * ld + 16 * ks + 4 * t);
+      }
+    }
+  }
+  float4 f[GROUPS][2][2];
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i)
+  {
 #pragma unroll
     for (int half = 0; half < 2; ++half)
     {
@@ -689,27 +708,30 @@ int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
 }
 
 template <int KS, int GROUPS>
-int up_mma_inst(const caifq_lora_bank &bank, const BankPlan &plan, int64_t tiles, const float *frozen, void *y, cudaStream_t s)
+int up_mma_inst(const caifq_lora_bank &bank, const int32_t *adapter_of_row, int64_t m, const BankPlan &plan, int64_t tiles,
+                const float *frozen, void *y, cudaStream_t s)
 {
+  auto kernel = m <= kSmallCall ? bank_up_mma_kernel<KS, GROUPS, true> : bank_up_mma_kernel<KS, GROUPS, false>;
   const unsigned columns = static_cast<unsigned>((bank.out_dim + 128 * GROUPS - 1) / (128 * GROUPS));
-  CAIFQ_CHECK_CUDA(launch_dependent(bank_up_mma_kernel<KS, GROUPS>, dim3(static_cast<unsigned>(tiles), columns), dim3(128), 0, s, frozen,
-                                    plan, static_cast<__nv_bfloat16 *>(y), bank.max_rank, bank.out_dim));
+  CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(tiles), columns), dim3(128), 0, s, frozen, adapter_of_row,
+                                    bank.entries, bank.count, m, plan, static_cast<__nv_bfloat16 *>(y), bank.max_rank, bank.out_dim));
   return CAIFQ_OK;
 }
 
-int up_mma(const caifq_lora_bank &bank, const float *frozen, int64_t m, void *y, void *scratch, cudaStream_t s)
+int up_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const float *frozen, int64_t m, void *y, void *scratch,
+           cudaStream_t s)
 {
   const int64_t tiles = most_tiles(m, bank.count);
   const BankPlan plan = plan_in(scratch, tiles);
   if (bank.max_rank <= 16)
   {
-    return up_mma_inst<1, 2>(bank, plan, tiles, frozen, y, s);
+    return up_mma_inst<1, 2>(bank, adapter_of_row, m, plan, tiles, frozen, y, s);
   }
   if (bank.max_rank <= 32)
   {
-    return up_mma_inst<2, 2>(bank, plan, tiles, frozen, y, s);
+    return up_mma_inst<2, 2>(bank, adapter_of_row, m, plan, tiles, frozen, y, s);
   }
-  return up_mma_inst<4, 1>(bank, plan, tiles, frozen, y, s);
+  return up_mma_inst<4, 1>(bank, adapter_of_row, m, plan, tiles, frozen, y, s);
 }
 
 template <typename T>
@@ -780,7 +802,7 @@ int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_r
 {
   if (tiled(bank, x, y, frozen, m))
   {
-    return up_mma(bank, frozen, m, y, scratch, s);
+    return up_mma(bank, adapter_of_row, frozen, m, y, scratch, s);
   }
   const float *h = static_cast<const float *>(scratch);
   switch (bank.dtype)
