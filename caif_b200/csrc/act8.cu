@@ -31,6 +31,9 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t most)
   return b < 1 ? 1u : static_cast<uint32_t>(b);
 }
 
+// rint(v / s) in the low byte: adding 1.5 * 2^23 rounds to the nearest even integer
+__device__ __forceinline__ uint32_t code_of(float v, float inverse) { return __float_as_uint(fmaf(v, inverse, 12582912.0f)); }
+
 // 1 / s; 0 for a block that stands for NaN (finite values give codes of 0, the others NaN, which converts to 0)
 __device__ __forceinline__ float inverse_of(uint32_t byte) { return byte == 255u ? 0.0f : __uint_as_float((254u - byte) << 23); }
 
@@ -55,7 +58,26 @@ __device__ __forceinline__ __half act_t<__half>(float v) { return __float2half(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 act_t<__nv_bfloat16>(float v) { return __float2bfloat16(v); }
 
-// ---- any width, any alignment: a warp a block, a lane an element ----
+// ---- any width, any alignment: a lane an element ----
+// A warp takes sixteen neighbouring blocks of a row at a time, all on their way together (bound by latency: one after the other, 67000
+// rows of 1000 bf16 took 210 us, four at a time 125).
+
+constexpr int kActTrain = 16;
+
+// trips of a warp over all rows; the same for every lane
+struct ActTrips
+{
+  int blocks;       // of a row
+  int trips;        // of a row
+  int64_t total;
+
+  __device__ __forceinline__ ActTrips(int64_t rows, int dim)
+  {
+    blocks = (dim + kActBlock - 1) / kActBlock;
+    trips = (blocks + kActTrain - 1) / kActTrain;
+    total = rows * trips;
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kActThreads)
@@ -64,23 +86,37 @@ act_pack_kernel(const T *x, int8_t *codes, uint8_t *scales, int64_t rows, int di
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int blocks = (dim + kActBlock - 1) / kActBlock;
-  const int64_t total = rows * blocks;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * (kActThreads / 32);
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * (kActThreads / 32) + (threadIdx.x >> 5); b < total; b += stride)
+  const ActTrips k(rows, dim);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kActThreads / 32);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kActThreads / 32) + (threadIdx.x >> 5); i < k.total; i += step)
   {
-    const int64_t row = b / blocks;
-    const int c = static_cast<int>(b - row * blocks) * kActBlock + lane;
-    const bool live = c < dim;
-    const float v = live ? act_f<T>(x[row * dim + c]) : 0.0f;
-    const uint32_t byte = scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v) & 0x7FFFFFFFu));
-    if (live)
+    const int64_t row = k.trips == 1 ? i : i / k.trips;
+    const int b0 = static_cast<int>(i - row * k.trips) * kActTrain;
+    const int c0 = b0 * kActBlock + lane;
+    const T *src = x + row * dim + c0;
+    int8_t *dst = codes + row * dim + c0;
+    const int left = dim - c0;   // this lane's columns from here on, every 32nd of them
+    T v[kActTrain];
+#pragma unroll
+    for (int u = 0; u < kActTrain; ++u)
     {
-      codes[row * dim + c] = static_cast<int8_t>(__float2int_rn(v * inverse_of(byte)));
+      v[u] = u * kActBlock < left ? src[u * kActBlock] : act_t<T>(0.0f);
     }
-    if (lane == 0)
+    uint32_t mine = 0u;   // the scale byte of block `lane`
+#pragma unroll
+    for (int u = 0; u < kActTrain; ++u)
     {
-      scales[b] = static_cast<uint8_t>(byte);
+      const float f = act_f<T>(v[u]);
+      const uint32_t byte = scale_byte(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(f) & 0x7FFFFFFFu));
+      mine = lane == u ? byte : mine;
+      if (u * kActBlock < left)
+      {
+        dst[u * kActBlock] = static_cast<int8_t>(byte == 255u ? 0u : code_of(f, inverse_of(byte)));
+      }
+    }
+    if (lane < kActTrain && b0 + lane < k.blocks)
+    {
+      scales[row * k.blocks + b0 + lane] = static_cast<uint8_t>(mine);
     }
   }
 }
@@ -92,31 +128,47 @@ act_unpack_kernel(const int8_t *codes, const uint8_t *scales, T *x, int64_t rows
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
-  const int blocks = (dim + kActBlock - 1) / kActBlock;
-  const int64_t total = rows * blocks;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * (kActThreads / 32);
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * (kActThreads / 32) + (threadIdx.x >> 5); b < total; b += stride)
+  const ActTrips k(rows, dim);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (kActThreads / 32);
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kActThreads / 32) + (threadIdx.x >> 5); i < k.total; i += step)
   {
-    const int64_t row = b / blocks;
-    const int c = static_cast<int>(b - row * blocks) * kActBlock + lane;
-    if (c < dim)
+    const int64_t row = k.trips == 1 ? i : i / k.trips;
+    const int b0 = static_cast<int>(i - row * k.trips) * kActTrain;
+    const int c0 = b0 * kActBlock + lane;
+    const int8_t *src = codes + row * dim + c0;
+    T *dst = x + row * dim + c0;
+    const int left = dim - c0;
+    const uint32_t mine = lane < kActTrain && b0 + lane < k.blocks ? scales[row * k.blocks + b0 + lane] : 1u;
+    int8_t q[kActTrain];
+#pragma unroll
+    for (int u = 0; u < kActTrain; ++u)
     {
-      x[row * dim + c] = act_t<T>(static_cast<float>(codes[row * dim + c]) * scale_of(scales[b]));
+      q[u] = u * kActBlock < left ? src[u * kActBlock] : static_cast<int8_t>(0);
+    }
+#pragma unroll
+    for (int u = 0; u < kActTrain; ++u)
+    {
+      const float s = scale_of(__shfl_sync(0xFFFFFFFFu, mine, u));
+      if (u * kActBlock < left)
+      {
+        dst[u * kActBlock] = act_t<T>(static_cast<float>(q[u]) * s);
+      }
     }
   }
 }
 
-unsigned act_grid(int64_t blocks)
+unsigned act_grid(int64_t rows, int dim)
 {
-  const int64_t ctas = (blocks + kActThreads / 32 - 1) / (kActThreads / 32);
+  const int64_t blocks = (static_cast<int64_t>(dim) + kActBlock - 1) / kActBlock;
+  const int64_t warps = rows * ((blocks + kActTrain - 1) / kActTrain);
+  const int64_t ctas = (warps + kActThreads / 32 - 1) / (kActThreads / 32);
   return static_cast<unsigned>(ctas < 148 * 64 ? ctas : 148 * 64);
 }
 
 // ---- rows of whole blocks on 16-byte boundaries: a thread 16 bytes of the row ----
 // HBM-bound (8192 x 4096 bf16: 102 MB each way).  A thread holds kActTrip pieces so that all its loads are in flight before
-// the first is used; the lanes of a block (4, or 8 of fp32) meet in two or three shuffles.  A code is the low byte of
-// x / s + 1.5 * 2^23, which rounds to the nearest even integer: one fused multiply-add instead of a conversion, whose unit
-// takes a sixteenth of a warp a cycle.
+// the first is used; the lanes of a block (4, or 8 of fp32) meet in two or three shuffles.  A code takes one fused multiply-add
+// instead of a conversion, whose unit serves a sixteenth of a warp a cycle.
 
 constexpr int kActTrip = 4;
 
@@ -167,12 +219,11 @@ __device__ __forceinline__ float piece_get(const uint32_t (&w)[4], int i)
 template <typename T>
 __device__ __forceinline__ uint32_t codes_of(const uint32_t (&w)[4], int first, float inverse)
 {
-  constexpr float kRound = 12582912.0f;   // 1.5 * 2^23
   uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
   {
-    b[i] = __float_as_uint(fmaf(piece_get<T>(w, first + i), inverse, kRound));
+    b[i] = code_of(piece_get<T>(w, first + i), inverse);
   }
   return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
@@ -315,7 +366,7 @@ int act_pack(const void *x, int8_t *codes, uint8_t *scales, int64_t rows, int di
                                       static_cast<const uint4 *>(x), static_cast<void *>(codes), scales, pieces));
     return CAIFQ_OK;
   }
-  CAIFQ_CHECK_CUDA(launch_dependent(act_pack_kernel<T>, dim3(act_grid(rows * ((dim + kActBlock - 1) / kActBlock))),
+  CAIFQ_CHECK_CUDA(launch_dependent(act_pack_kernel<T>, dim3(act_grid(rows, dim)),
                                     dim3(kActThreads), 0, s, static_cast<const T *>(x), codes, scales, rows, dim));
   return CAIFQ_OK;
 }
@@ -330,7 +381,7 @@ int act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int64_t rows
                                       static_cast<const void *>(codes), scales, static_cast<uint4 *>(x), pieces));
     return CAIFQ_OK;
   }
-  CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_kernel<T>, dim3(act_grid(rows * ((dim + kActBlock - 1) / kActBlock))),
+  CAIFQ_CHECK_CUDA(launch_dependent(act_unpack_kernel<T>, dim3(act_grid(rows, dim)),
                                     dim3(kActThreads), 0, s, codes, scales, static_cast<T *>(x), rows, dim));
   return CAIFQ_OK;
 }

@@ -63,7 +63,7 @@ __device__ __forceinline__ float sum_of(float v, float *slots)
   return v;
 }
 
-// ---- any width, any alignment: a CTA a row, the row read from memory (the cache) in every pass ----
+// ---- any width, any alignment (tensors off a 16-byte boundary, rows wider than 128 KB): a block a row, read in every pass ----
 
 template <typename T>
 __global__ void __launch_bounds__(kLnThreads)
@@ -134,45 +134,6 @@ layernorm_dx_kernel(const T *dy, const T *x, const float *__restrict__ gamma, co
   }
 }
 
-// partial sums over slice blockIdx.y of the rows: part[slice][0][c] = sum dy * xh, part[slice][1][c] = sum dy
-template <typename T>
-__global__ void __launch_bounds__(kLnThreads)
-layernorm_columns_kernel(const T *dy, const T *x, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
-                         float *__restrict__ part, int rows, int64_t dim)
-{
-  __shared__ float2 tile[8][33];
-  asm volatile("griddepcontrol.wait;" : "+l"(mean_in), "+l"(rstd_in)::"memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int lane = threadIdx.x & 31;
-  const int group = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  const int64_t begin = static_cast<int64_t>(rows) * blockIdx.y / gridDim.y;
-  const int64_t end = static_cast<int64_t>(rows) * (blockIdx.y + 1) / gridDim.y;
-  float2 s = make_float2(0.0f, 0.0f);
-  if (c < dim)
-  {
-    for (int64_t r = begin + group; r < end; r += 8)
-    {
-      const float g = to_f<T>(dy[r * dim + c]);
-      s.x = fmaf(g, (to_f<T>(x[r * dim + c]) - mean_in[r]) * rstd_in[r], s.x);
-      s.y += g;
-    }
-  }
-  tile[group][lane] = s;
-  __syncthreads();
-  if (group == 0 && c < dim)
-  {
-    for (int i = 1; i < 8; ++i)
-    {
-      s.x += tile[i][lane].x;
-      s.y += tile[i][lane].y;
-    }
-    float *dst = part + static_cast<int64_t>(blockIdx.y) * 2 * dim + c;
-    dst[0] = s.x;
-    dst[dim] = s.y;
-  }
-}
-
 // the slices' sums, in a fixed order: 32 threads a column take every 32nd slice each (with eight, 296 slices of 4096 columns
 // took 10 us)
 __global__ void __launch_bounds__(1024)
@@ -215,8 +176,9 @@ layernorm_finish_kernel(const float *part, float *grad_gamma, float *grad_beta, 
 }
 
 // ---- rows in registers ----
-// WARPS warps own a row; a thread holds P pieces of V columns, 16 bytes each where the rows allow it (V = 1: rows off a
-// 16-byte boundary or of odd length, element by element).  The row comes in once and all its loads are in flight together.
+// WARPS warps own a row; a thread holds P pieces of V columns, 16 bytes each.  The row comes in once and all its loads are in flight
+// together.  A row that does not begin with a piece begins
+// `shift` columns into one, and its first and last piece are read and written element by element.
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) LnPiece
@@ -224,8 +186,56 @@ struct alignas(sizeof(T) * V) LnPiece
   T e[V];
 };
 
-template <typename T, int V>
-__device__ __forceinline__ void load_floats(float (&out)[V], const float *p, float other)
+// threads of a block: several short rows, or one long one
+template <int WARPS>
+constexpr int kLnSlots = WARPS < 8 ? 8 / WARPS : 1;
+template <int WARPS>
+constexpr int kLnBlock = WARPS * 32 * kLnSlots<WARPS>;
+
+// a piece of a row from column c on, and back; its elements that are not the row's are zeros, or left alone
+template <typename T, int V, bool SHIFT>
+__device__ __forceinline__ LnPiece<T, V> load_piece(const T *row, int c, int dim)
+{
+  LnPiece<T, V> p;
+  if (!SHIFT || (c >= 0 && c + V <= dim))
+  {
+    p = *reinterpret_cast<const LnPiece<T, V> *>(row + c);
+  }
+  else
+  {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      p.e[i] = c + i >= 0 && c + i < dim ? row[c + i] : from_f<T>(0.0f);
+    }
+  }
+  return p;
+}
+
+template <typename T, int V, bool SHIFT>
+__device__ __forceinline__ void store_piece(T *row, int c, int dim, const LnPiece<T, V> &p)
+{
+  if (!SHIFT || (c >= 0 && c + V <= dim))
+  {
+    *reinterpret_cast<LnPiece<T, V> *>(row + c) = p;
+  }
+  else
+  {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      if (c + i >= 0 && c + i < dim)
+      {
+        row[c + i] = p.e[i];
+      }
+    }
+  }
+}
+
+// fp32 values of a piece's columns; `other` without a vector.  `vector`: p on a 16-byte boundary.  Columns that do not begin on one
+// are taken out of the 16-byte pieces around them.
+template <int V, bool SHIFT>
+__device__ __forceinline__ void load_columns(float (&out)[V], const float *p, int c, int dim, bool vector, float other)
 {
   if (p == nullptr)
   {
@@ -234,64 +244,87 @@ __device__ __forceinline__ void load_floats(float (&out)[V], const float *p, flo
     {
       out[i] = other;
     }
+    return;
   }
-  else if constexpr (V >= 4)
+  const int skip = SHIFT ? c & 3 : 0;
+  if (vector && c >= 0 && c - skip + V + (SHIFT ? 4 : 0) <= dim)
   {
+    float f[V + 4];
 #pragma unroll
-    for (int i = 0; i < V; i += 4)
+    for (int i = 0; i < V + (SHIFT ? 4 : 0); i += 4)
     {
-      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + i));
-      out[i] = v.x;
-      out[i + 1] = v.y;
-      out[i + 2] = v.z;
-      out[i + 3] = v.w;
+      const float4 v = __ldg(reinterpret_cast<const float4 *>(p + c - skip + i));
+      f[i] = v.x;
+      f[i + 1] = v.y;
+      f[i + 2] = v.z;
+      f[i + 3] = v.w;
     }
-  }
-  else
-  {
+    if constexpr (SHIFT)
+    {
+#pragma unroll
+      for (int i = 0; i < V + 2; ++i)
+      {
+        f[i] = (skip & 2) != 0 ? f[i + 2] : f[i];
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        f[i] = (skip & 1) != 0 ? f[i + 1] : f[i];
+      }
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i)
     {
-      out[i] = __ldg(p + i);
+      out[i] = f[i];
     }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+  {
+    out[i] = c + i >= 0 && c + i < dim ? __ldg(p + c + i) : 0.0f;
   }
 }
 
-// threads of a block: several short rows, or one long one
-template <int WARPS, int LEAST>
-constexpr int kLnBlock = WARPS * 32 > LEAST ? WARPS * 32 : LEAST;
+__device__ __forceinline__ bool on_16_dev(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <typename T, int V, int P, int WARPS>
-__global__ void __launch_bounds__(kLnBlock<WARPS, 128>)
-layernorm_fwd_rows_kernel(const T *x, const float *__restrict__ gamma, const float *__restrict__ beta, T *y,
-                          float *__restrict__ mean_out, float *__restrict__ rstd_out, float epsilon, int rows, int dim)
+// columns of the first piece that belong to the row before
+template <int V>
+__device__ __forceinline__ int shift_of(int64_t row, int dim)
 {
-  constexpr int SLOTS = kLnBlock<WARPS, 128> / (WARPS * 32);
-  constexpr int THREADS = WARPS * 32;   // of a row
-  __shared__ float sums[SLOTS][WARPS];
+  return static_cast<int>(row * dim % V);
+}
+
+// rows too wide for the form below, which keeps gamma and beta: one row a block
+template <typename T, int V, int P, int WARPS, bool SHIFT>
+__global__ void __launch_bounds__(WARPS * 32)
+layernorm_fwd_rows_kernel(const T *x, const float *__restrict__ gamma, const float *__restrict__ beta, T *y,
+                          float *__restrict__ mean_out, float *__restrict__ rstd_out, float epsilon, int dim)
+{
+  constexpr int THREADS = WARPS * 32;
+  __shared__ float sums[WARPS];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(beta)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int slot = threadIdx.x / THREADS;
-  const int t = threadIdx.x % THREADS;
-  const int r = blockIdx.x * SLOTS + slot;
-  const bool live = r < rows;
+  const int64_t r = blockIdx.x;
+  const bool vector = on_16_dev(gamma) && on_16_dev(beta);
+  const int c0 = static_cast<int>(threadIdx.x) * V - (SHIFT ? shift_of<V>(r, dim) : 0);
   using Piece = LnPiece<T, V>;
   Piece v[P];
-  const T *src = x + static_cast<int64_t>(live ? r : 0) * dim;
+  const T *src = x + r * dim;
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = c0 + j * THREADS * V;
+    if (c < dim)
+    {
+      v[j] = load_piece<T, V, SHIFT>(src, c, dim);
+    }
+  }
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < P; ++j)
   {
-    const int c = (t + j * THREADS) * V;
-    if (live && c < dim)
-    {
-      v[j] = *reinterpret_cast<const Piece *>(src + c);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < P; ++j)
-  {
-    if (live && (t + j * THREADS) * V < dim)
+    if (c0 + j * THREADS * V < dim)
     {
 #pragma unroll
       for (int i = 0; i < V; ++i)
@@ -300,64 +333,223 @@ layernorm_fwd_rows_kernel(const T *x, const float *__restrict__ gamma, const flo
       }
     }
   }
-  const float mean = sum_of<WARPS>(s, sums[slot]) / static_cast<float>(dim);
+  const float mean = sum_of<WARPS>(s, sums) / static_cast<float>(dim);
   s = 0.0f;
 #pragma unroll
   for (int j = 0; j < P; ++j)
   {
-    if (live && (t + j * THREADS) * V < dim)
+    const int c = c0 + j * THREADS * V;
+    if (c < dim)
     {
 #pragma unroll
       for (int i = 0; i < V; ++i)
       {
-        const float d = to_f<T>(v[j].e[i]) - mean;
+        const float d = !SHIFT || (c + i >= 0 && c + i < dim) ? to_f<T>(v[j].e[i]) - mean : 0.0f;
         s = fmaf(d, d, s);
       }
     }
   }
-  const float rstd = 1.0f / sqrtf(sum_of<WARPS>(s, sums[slot]) / static_cast<float>(dim) + epsilon);
-  if (!live)
-  {
-    return;
-  }
-  T *dst = y + static_cast<int64_t>(r) * dim;
+  const float rstd = 1.0f / sqrtf(sum_of<WARPS>(s, sums) / static_cast<float>(dim) + epsilon);
+  T *dst = y + r * dim;
 #pragma unroll
   for (int j = 0; j < P; ++j)
   {
-    const int c = (t + j * THREADS) * V;
+    const int c = c0 + j * THREADS * V;
     if (c < dim)
     {
       float g[V], b[V];
-      load_floats<T, V>(g, gamma != nullptr ? gamma + c : nullptr, 1.0f);
-      load_floats<T, V>(b, beta != nullptr ? beta + c : nullptr, 0.0f);
+      load_columns<V, SHIFT>(g, gamma, c, dim, vector, 1.0f);
+      load_columns<V, SHIFT>(b, beta, c, dim, vector, 0.0f);
       Piece o;
 #pragma unroll
       for (int i = 0; i < V; ++i)
       {
         o.e[i] = from_f<T>(fmaf((to_f<T>(v[j].e[i]) - mean) * rstd, g[i], b[i]));
       }
-      *reinterpret_cast<Piece *>(dst + c) = o;
+      store_piece<T, V, SHIFT>(dst, c, dim, o);
     }
   }
-  if (t == 0)
+  if (threadIdx.x == 0)
   {
     mean_out[r] = mean;
     rstd_out[r] = rstd;
   }
 }
 
+// the same rows' dx.  (A thread's columns' sums beside two pieces of the row would not fit the registers: they come from
+// layernorm_columns_kernel, which reads dy and x once more.)
+template <typename T, int V, int P, int WARPS, bool SHIFT>
+__global__ void __launch_bounds__(WARPS * 32)
+layernorm_dx_rows_kernel(const T *dy, const T *x, const float *__restrict__ gamma, const float *__restrict__ mean_in,
+                         const float *__restrict__ rstd_in, T *dx, int dim)
+{
+  constexpr int THREADS = WARPS * 32;
+  __shared__ float sums[2][WARPS];
+  asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(mean_in), "+l"(rstd_in)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t r = blockIdx.x;
+  const bool vector = on_16_dev(gamma);
+  const int c0 = static_cast<int>(threadIdx.x) * V - (SHIFT ? shift_of<V>(r, dim) : 0);
+  using Piece = LnPiece<T, V>;
+  Piece vx[P], vd[P];
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = c0 + j * THREADS * V;
+    if (c < dim)
+    {
+      vx[j] = load_piece<T, V, SHIFT>(x + r * dim, c, dim);
+      vd[j] = load_piece<T, V, SHIFT>(dy + r * dim, c, dim);
+    }
+  }
+  const float mean = mean_in[r];
+  const float rstd = rstd_in[r];
+  float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = c0 + j * THREADS * V;
+    if (c < dim)
+    {
+      float g[V];
+      load_columns<V, SHIFT>(g, gamma, c, dim, vector, 1.0f);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        // (dy is zero outside the row, and x there too)
+        const float w = to_f<T>(vd[j].e[i]) * g[i];
+        s1 += w;
+        s2 = fmaf(w, (to_f<T>(vx[j].e[i]) - mean) * rstd, s2);
+      }
+    }
+  }
+  s1 = sum_of<WARPS>(s1, sums[0]) / static_cast<float>(dim);
+  s2 = sum_of<WARPS>(s2, sums[1]) / static_cast<float>(dim);
+#pragma unroll
+  for (int j = 0; j < P; ++j)
+  {
+    const int c = c0 + j * THREADS * V;
+    if (c < dim)
+    {
+      float g[V];
+      load_columns<V, SHIFT>(g, gamma, c, dim, vector, 1.0f);
+      Piece o;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+      {
+        const float xh = (to_f<T>(vx[j].e[i]) - mean) * rstd;
+        o.e[i] = from_f<T>(rstd * (to_f<T>(vd[j].e[i]) * g[i] - s1 - xh * s2));
+      }
+      store_piece<T, V, SHIFT>(dx + r * dim, c, dim, o);
+    }
+  }
+}
+
+// part[slice][0][c] = sum of dy * xh, part[slice][1][c] = sum of dy over slice blockIdx.y of the rows: a warp every eighth row of it, a
+// lane V neighbouring columns (V = 1, rows that are not whole pieces: eight columns, 32 apart); the eight warps' sums meet in shared
+// memory.  HBM-bound: dy and x once.
+template <typename T, int V>
+__global__ void __launch_bounds__(kLnThreads)
+layernorm_columns_kernel(const T *dy, const T *x, const float *__restrict__ mean_in, const float *__restrict__ rstd_in,
+                         float *__restrict__ part, int rows, int64_t dim)
+{
+  constexpr int N = V == 1 ? 8 : V;   // columns of a thread
+  __shared__ float2 tile[kLnThreads / 32][32 * N + 1];
+  asm volatile("griddepcontrol.wait;" : "+l"(mean_in), "+l"(rstd_in)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int64_t begin = static_cast<int64_t>(rows) * blockIdx.y / gridDim.y;
+  const int64_t end = static_cast<int64_t>(rows) * (blockIdx.y + 1) / gridDim.y;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 32 * N;
+  float sg[N], sb[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+  {
+    sg[i] = sb[i] = 0.0f;
+  }
+#pragma unroll 2
+  for (int64_t r = begin + warp; r < end; r += kLnThreads / 32)
+  {
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    T d[N], v[N];
+    if constexpr (V > 1)
+    {
+      const int64_t c = first + lane * V;
+      if (c < dim)
+      {
+        *reinterpret_cast<LnPiece<T, V> *>(d) = *reinterpret_cast<const LnPiece<T, V> *>(dy + r * dim + c);
+        *reinterpret_cast<LnPiece<T, V> *>(v) = *reinterpret_cast<const LnPiece<T, V> *>(x + r * dim + c);
+      }
+    }
+    else
+    {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+      {
+        const int64_t c = first + lane + 32 * i;
+        if (c < dim)
+        {
+          d[i] = dy[r * dim + c];
+          v[i] = x[r * dim + c];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)   // (sums of columns that are not there are not stored)
+    {
+      const float g = to_f<T>(d[i]);
+      sg[i] = fmaf(g, (to_f<T>(v[i]) - mean) * rstd, sg[i]);
+      sb[i] += g;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+  {
+    tile[warp][V > 1 ? lane * V + i : lane + 32 * i] = make_float2(sg[i], sb[i]);
+  }
+  __syncthreads();
+  float *dst = part + static_cast<int64_t>(blockIdx.y) * 2 * dim;
+  for (int i = threadIdx.x; i < 32 * N; i += kLnThreads)
+  {
+    if (first + i < dim)
+    {
+      float2 s = tile[0][i];
+#pragma unroll
+      for (int w = 1; w < kLnThreads / 32; ++w)
+      {
+        s.x += tile[w][i].x;
+        s.y += tile[w][i].y;
+      }
+      dst[first + i] = s.x;
+      dst[dim + first + i] = s.y;
+    }
+  }
+}
+
 // ---- many rows: a block takes rows one after the other ----
 // gamma and beta (or the columns' sums of the backward pass) stay in registers from row to row, and the next rows are on their
 // way: 16-byte pieces come by asynchronous copies through a ring of RING rows in shared memory, of which every thread reads
-// back exactly what it copied, so that no barrier belongs to the copies.  Rows that no 16-byte piece fits are fetched one row
-// ahead into registers.  A sum's slots alternate from row to row: one barrier a sum.
+// back exactly what it copied, so that no barrier belongs to the copies.  A sum's slots alternate from row to row: one barrier a
+// sum.
+// Rows that are not whole pieces begin anywhere in one.  A block's rows are a multiple of V apart then, so that all of them begin
+// `shift` columns into a piece and a thread's columns stay the same from row to row; the pieces that reach into a neighbouring row
+// are masked, and stored element by element.
+
+// blocks an SM
+template <int WARPS, bool SHIFT>
+constexpr int kFwdBlocks = WARPS <= 8 ? (SHIFT ? 2 : 3) : (WARPS <= 12 ? 2 : 1);
+template <int WARPS>
+constexpr int kBwdBlocks = WARPS <= 8 ? 2 : 1;
 
 template <typename T>
 constexpr int kLnRing = sizeof(T) == 4 ? 3 : 4;
 
-__device__ __forceinline__ void copy_16(void *to, const void *from)
+// 16 bytes, of which the first `bytes` are read and the others zero
+__device__ __forceinline__ void copy_16(void *to, const void *from, int bytes)
 {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from),
+               "r"(bytes)
                : "memory");
 }
 
@@ -418,7 +610,7 @@ __device__ __forceinline__ void sums_of(float (&v)[N], float (*slots)[WARPS])
 #pragma unroll
     for (int n = 0; n < N; ++n)
     {
-      if constexpr (WARPS >= 4)
+      if constexpr (WARPS % 4 == 0)
       {
         const float4 *p = reinterpret_cast<const float4 *>(slots[n]);
         float4 s = p[0];
@@ -435,7 +627,12 @@ __device__ __forceinline__ void sums_of(float (&v)[N], float (*slots)[WARPS])
       }
       else
       {
-        v[n] = slots[n][0] + slots[n][1];
+        v[n] = slots[n][0];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w)
+        {
+          v[n] += slots[n][w];
+        }
       }
     }
   }
@@ -450,61 +647,48 @@ __device__ __forceinline__ float inverse_root(float v)
 }
 
 // the rows of N tensors that a block walks over: start() once, then next() for each row in turn gives this thread's pieces
-template <typename T, int V, int P, int THREADS, int BLOCK, int N>
+template <typename T, int V, int P, int THREADS, int BLOCK, int N, bool SHIFT>
 struct RowsAhead
 {
   using Piece = LnPiece<T, V>;
   static constexpr int RING = kLnRing<T>;
-  static constexpr size_t kBytes = V > 1 ? static_cast<size_t>(RING) * N * P * BLOCK * 16 : 0;
+  static constexpr size_t kBytes = static_cast<size_t>(RING) * N * P * BLOCK * 16;
   const T *src[N];
   int64_t row;     // the next row to fetch
   int64_t step;
   int rows, dim, t;
+  int shift;       // columns of the first piece that belong to the row before
   uint4 *ring;
   int at;          // ring row that next() reads
-  Piece ahead[V > 1 ? 1 : N][V > 1 ? 1 : P];
+
+  // first column of piece j; below 0 or past the row where the piece reaches into a neighbouring one
+  __device__ __forceinline__ int column(int j) const { return (t + j * THREADS) * V - (SHIFT ? shift : 0); }
+
+  // whether all of piece j, or nothing of it, is the row's
+  __device__ __forceinline__ bool whole(int j) const { return !SHIFT || (column(j) >= 0 && column(j) + V <= dim) || column(j) >= dim; }
 
   __device__ __forceinline__ void fetch(int stage)
   {
-    if constexpr (V > 1)
+    if (row < rows)
     {
-      if (row < rows)
+      const int64_t left = (rows - row) * dim;   // elements from the row's first on
+#pragma unroll
+      for (int n = 0; n < N; ++n)
       {
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int j = 0; j < P; ++j)
         {
-#pragma unroll
-          for (int j = 0; j < P; ++j)
+          const int c = column(j);
+          if (c < dim)
           {
-            const int c = (t + j * THREADS) * V;
-            if (c < dim)
-            {
-              copy_16(ring + ((stage * N + n) * P + j) * BLOCK + threadIdx.x, src[n] + row * dim + c);
-            }
-          }
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    else
-    {
-      if (row < rows)
-      {
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-        {
-#pragma unroll
-          for (int j = 0; j < P; ++j)
-          {
-            const int c = (t + j * THREADS) * V;
-            if (c < dim)
-            {
-              ahead[n][j] = *reinterpret_cast<const Piece *>(src[n] + row * dim + c);
-            }
+            // (of the tensor's last piece only what belongs to it)
+            const int bytes = SHIFT && left - c < V ? static_cast<int>(left - c) * static_cast<int>(sizeof(T)) : 16;
+            copy_16(ring + ((stage * N + n) * P + j) * BLOCK + threadIdx.x, src[n] + row * dim + c, bytes);
           }
         }
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
     row += step;
   }
 
@@ -512,7 +696,7 @@ struct RowsAhead
   {
     at = 0;
 #pragma unroll
-    for (int i = 0; i < (V > 1 ? RING - 1 : 1); ++i)
+    for (int i = 0; i < RING - 1; ++i)
     {
       fetch(i);
     }
@@ -521,42 +705,44 @@ struct RowsAhead
   // the row's values of this thread in pairs; zeros where the thread has no column, or the block no row
   __device__ __forceinline__ void next(Two (&out)[N][P * V / 2], bool live)
   {
-    Piece piece[N][P];
-    if constexpr (V > 1)
+    // (the ring row before this one, which this thread has read, is filled again)
+    fetch(at == 0 ? RING - 1 : at - 1);
+    asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
+#pragma unroll
+    for (int n = 0; n < N; ++n)
     {
-      // (the ring row before this one, which this thread has read, is filled again)
-      fetch(at == 0 ? RING - 1 : at - 1);
-      asm volatile("cp.async.wait_group %0;" ::"n"(RING - 1) : "memory");
 #pragma unroll
-      for (int n = 0; n < N; ++n)
+      for (int j = 0; j < P; ++j)
       {
-#pragma unroll
-        for (int j = 0; j < P; ++j)
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        const int c = column(j);
+        if (live && c < dim)
         {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (live && (t + j * THREADS) * V < dim)
+          v = ring[((at * N + n) * P + j) * BLOCK + threadIdx.x];
+          if (!whole(j))
           {
-            v = ring[((at * N + n) * P + j) * BLOCK + threadIdx.x];
+            mask(v, c);
           }
-          pairs_of(out[n] + j * (V / 2), v);
         }
+        pairs_of(out[n] + j * (V / 2), v);
       }
-      at = at == RING - 1 ? 0 : at + 1;
     }
-    else
+    at = at == RING - 1 ? 0 : at + 1;
+  }
+
+  // zeros for the elements of a piece that are not the row's
+  __device__ __forceinline__ void mask(uint4 &v, int c) const
+  {
+    Piece p = *reinterpret_cast<const Piece *>(&v);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
     {
-#pragma unroll
-      for (int n = 0; n < N; ++n)
+      if (c + i < 0 || c + i >= dim)
       {
-#pragma unroll
-        for (int j = 0; j < P; j += 2)
-        {
-          out[n][j / 2] = two(live && t + j * THREADS < dim ? to_f<T>(ahead[n][j].e[0]) : 0.0f,
-                              live && t + (j + 1) * THREADS < dim ? to_f<T>(ahead[n][j + 1].e[0]) : 0.0f);
-        }
+        p.e[i] = from_f<T>(0.0f);
       }
-      fetch(0);
     }
+    v = *reinterpret_cast<const uint4 *>(&p);
   }
 
   static __device__ __forceinline__ void pairs_of(Two *out, const uint4 &v)
@@ -584,7 +770,7 @@ struct RowsAhead
 #pragma unroll
     for (int j = 0; j < P; ++j)
     {
-      const int c = (t + j * THREADS) * V;
+      const int c = column(j);
       if (c < dim)
       {
         Piece o;
@@ -594,47 +780,73 @@ struct RowsAhead
           const int e = j * V + i;
           o.e[i] = from_f<T>((e & 1) != 0 ? second_of(v[e / 2]) : first_of(v[e / 2]));
         }
-        *reinterpret_cast<Piece *>(row_out + c) = o;
+        if (whole(j))
+        {
+          *reinterpret_cast<Piece *>(row_out + c) = o;
+        }
+        else
+        {
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+          {
+            if (c + i >= 0 && c + i < dim)
+            {
+              row_out[c + i] = o.e[i];
+            }
+          }
+        }
       }
     }
   }
 
+  // column of element e of the thread, and whether the row has it
+  __device__ __forceinline__ int column_of(int e) const { return column(e / V) + e % V; }
+  __device__ __forceinline__ bool has(int e) const { return column_of(e) >= 0 && column_of(e) < dim; }
+
   // fp32 values of this thread's columns; `other` without a vector, zeros where the thread has no column
   __device__ __forceinline__ void columns(Two (&out)[P * V / 2], const float *p, float other) const
   {
-    float f[P][V];
+    float f[P * V];
 #pragma unroll
     for (int j = 0; j < P; ++j)
     {
-      const int c = (t + j * THREADS) * V;
+      if (!SHIFT && column(j) < dim && p != nullptr && on_16_dev(p))
+      {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-      {
-        f[j][i] = 0.0f;
+        for (int i = 0; i < V; i += 4)
+        {
+          const float4 v = __ldg(reinterpret_cast<const float4 *>(p + column(j) + i));
+          f[j * V + i] = v.x;
+          f[(j * V + i + 1) % (P * V)] = v.y;
+          f[(j * V + i + 2) % (P * V)] = v.z;
+          f[(j * V + i + 3) % (P * V)] = v.w;
+        }
       }
-      if (c < dim)
+      else
       {
-        load_floats<T, V>(f[j], p != nullptr ? p + c : nullptr, other);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+        {
+          const int e = j * V + i;
+          f[e] = !has(e) ? 0.0f : (p != nullptr ? __ldg(p + column_of(e)) : other);
+        }
       }
     }
 #pragma unroll
     for (int e = 0; e < P * V; e += 2)
     {
-      out[e / 2] = two(f[e / V][e % V], f[(e + 1) / V][(e + 1) % V]);
+      out[e / 2] = two(f[e], f[e + 1]);
     }
   }
-
-  // whether element e of the thread is a column
-  __device__ __forceinline__ bool has(int e) const { return (t + (e / V) * THREADS) * V < dim; }
 };
 
-template <typename T, int V, int P, int WARPS>
-__global__ void __launch_bounds__(kLnBlock<WARPS, 256>, WARPS <= 8 ? 3 : 1)
+template <typename T, int V, int P, int WARPS, bool SHIFT>
+__global__ void __launch_bounds__(kLnBlock<WARPS>, kFwdBlocks<WARPS, SHIFT>)
 layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const float *__restrict__ beta, T *y,
                           float *__restrict__ mean_out, float *__restrict__ rstd_out, float epsilon, int rows, int dim)
 {
-  constexpr int BLOCK = kLnBlock<WARPS, 256>;
-  constexpr int SLOTS = BLOCK / (WARPS * 32);
+  constexpr int BLOCK = kLnBlock<WARPS>;
+  constexpr int SLOTS = kLnSlots<WARPS>;
   constexpr int THREADS = WARPS * 32;
   constexpr int PAIRS = P * V / 2;
   extern __shared__ uint4 ln_ring[];
@@ -645,19 +857,19 @@ layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const flo
   const int t = threadIdx.x % THREADS;
   const int first = static_cast<int>(blockIdx.x) * SLOTS;
   const int step = static_cast<int>(gridDim.x) * SLOTS;
-  RowsAhead<T, V, P, THREADS, BLOCK, 1> in;
+  RowsAhead<T, V, P, THREADS, BLOCK, 1, SHIFT> in;
   in.src[0] = x;
   in.row = first + slot;
   in.step = step;
   in.rows = rows;
   in.dim = dim;
   in.t = t;
+  in.shift = SHIFT ? static_cast<int>(static_cast<int64_t>(first + slot) * dim % V) : 0;
   in.ring = ln_ring;
   in.start();
   Two g[PAIRS], b[PAIRS];
   in.columns(g, gamma, 1.0f);
   in.columns(b, beta, 0.0f);
-  const bool ragged = dim < THREADS * P * V;
   const float inverse = 1.0f / static_cast<float>(dim);
   int turn = 0;
   for (int64_t base = first; base < rows; base += step, turn ^= 1)   // (every slot takes part in the sums' barriers)
@@ -680,10 +892,32 @@ layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const flo
     for (int i = 0; i < PAIRS; ++i)
     {
       v[0][i] = add2(v[0][i], two(-mean, -mean));
-      if (ragged)
+      if (i % (V / 2) == V / 2 - 1)   // the piece's last pair
       {
-        v[0][i] = two(in.has(2 * i) ? first_of(v[0][i]) : 0.0f, in.has(2 * i + 1) ? second_of(v[0][i]) : 0.0f);
+        constexpr int H = V / 2;
+        const int j = i / H;
+        if (in.column(j) >= dim)
+        {
+#pragma unroll
+          for (int k = 0; k < H; ++k)
+          {
+            v[0][j * H + k] = two(0.0f, 0.0f);
+          }
+        }
+        else if (!in.whole(j))
+        {
+#pragma unroll
+          for (int k = 0; k < H; ++k)
+          {
+            const int e = 2 * (j * H + k);
+            v[0][j * H + k] = two(in.has(e) ? first_of(v[0][j * H + k]) : 0.0f, in.has(e + 1) ? second_of(v[0][j * H + k]) : 0.0f);
+          }
+        }
       }
+    }
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i)
+    {
       a = fma2(v[0][i], v[0][i], a);
     }
     s[0] = first_of(a) + second_of(a);
@@ -708,20 +942,20 @@ layernorm_fwd_many_kernel(const T *x, const float *__restrict__ gamma, const flo
 
 // dx and this block's share of dgamma and dbeta in one pass: a thread keeps its columns' sums over all rows of the block.
 // part[block][0][c], part[block][1][c] as in layernorm_columns_kernel.
-template <typename T, int V, int P, int WARPS>
-__global__ void __launch_bounds__(kLnBlock<WARPS, 256>, WARPS <= 8 ? 2 : 1)
+template <typename T, int V, int P, int WARPS, bool SHIFT>
+__global__ void __launch_bounds__(kLnBlock<WARPS>, kBwdBlocks<WARPS>)
 layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gamma, const float *__restrict__ mean_in,
                           const float *__restrict__ rstd_in, T *dx, float *__restrict__ part, int rows, int dim)
 {
-  constexpr int BLOCK = kLnBlock<WARPS, 256>;
-  constexpr int SLOTS = BLOCK / (WARPS * 32);
+  constexpr int BLOCK = kLnBlock<WARPS>;
+  constexpr int SLOTS = kLnSlots<WARPS>;
   constexpr int THREADS = WARPS * 32;
   constexpr int PAIRS = P * V / 2;
   extern __shared__ uint4 ln_ring[];   // the ring; then, where SLOTS > 1, the columns' sums [2][dim]
   __shared__ __align__(16) float sums[2][SLOTS][2][WARPS];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(mean_in), "+l"(rstd_in)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  using Rows = RowsAhead<T, V, P, THREADS, BLOCK, 2>;
+  using Rows = RowsAhead<T, V, P, THREADS, BLOCK, 2, SHIFT>;
   const int slot = threadIdx.x / THREADS;
   const int t = threadIdx.x % THREADS;
   const int first = static_cast<int>(blockIdx.x) * SLOTS;
@@ -734,6 +968,7 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
   in.rows = rows;
   in.dim = dim;
   in.t = t;
+  in.shift = SHIFT ? static_cast<int>(static_cast<int64_t>(first + slot) * dim % V) : 0;
   in.ring = ln_ring;
   in.start();
   Two g[PAIRS], sg[PAIRS], sb[PAIRS];
@@ -808,8 +1043,8 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
 #pragma unroll
       for (int e = 0; e < P * V; ++e)
       {
-        const int c = (t + (e / V) * THREADS) * V + e % V;
-        if (c < dim)
+        const int c = in.column_of(e);
+        if (c >= 0 && c < dim)
         {
           const float vg = (e & 1) != 0 ? second_of(sg[e / 2]) : first_of(sg[e / 2]);
           const float vb = (e & 1) != 0 ? second_of(sb[e / 2]) : first_of(sb[e / 2]);
@@ -832,7 +1067,7 @@ layernorm_bwd_rows_kernel(const T *dy, const T *x, const float *__restrict__ gam
   }
 }
 
-// slices of rows with partial sums of their own
+// slices of rows with partial sums of their own, at most
 int ln_slices(int rows) { return rows < 148 * 2 ? rows : 148 * 2; }
 
 unsigned ln_grid(int rows) { return static_cast<unsigned>(rows < 148 * 8 ? rows : 148 * 8); }
@@ -841,15 +1076,28 @@ constexpr size_t kLnPlainSmem = 40 * 1024;   // dynamic, beside the static slots
 
 bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// columns that the threads of a row must reach: its own, and those of its first piece that are not
+template <int V>
+int64_t reach_of(int dim)
+{
+  return static_cast<int64_t>(dim) + (dim % V != 0 ? V - 1 : 0);
+}
+
+// blocks of a launch that walks over the rows: one wave.  Where rows are not whole pieces a block's rows lie a multiple of V apart.
+template <int V>
+int walk_blocks(int rows, int slots, int dim, int per_sm)
+{
+  const int blocks = (rows - 1) / slots + 1;
+  const int most = 148 * per_sm;
+  return blocks <= most ? blocks : (dim % V != 0 ? most / 8 * 8 : most);
+}
+
 template <typename T, int V, int P, int WARPS>
 int ln_fwd_rows(const T *x, const float *gamma, const float *beta, T *y, float *mean, float *rstd, float epsilon, int rows,
                 int dim, cudaStream_t s)
 {
-  constexpr int BLOCK = kLnBlock<WARPS, 128>;
-  constexpr int SLOTS = BLOCK / (WARPS * 32);
-  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_rows_kernel<T, V, P, WARPS>,
-                                    dim3(static_cast<unsigned>((static_cast<int64_t>(rows) + SLOTS - 1) / SLOTS)), dim3(BLOCK), 0, s, x,
-                                    gamma, beta, y, mean, rstd, epsilon, rows, dim));
+  auto kernel = dim % V == 0 ? layernorm_fwd_rows_kernel<T, V, P, WARPS, false> : layernorm_fwd_rows_kernel<T, V, P, WARPS, true>;
+  CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rows)), dim3(WARPS * 32), 0, s, x, gamma, beta, y, mean, rstd, epsilon, dim));
   return CAIFQ_OK;
 }
 
@@ -872,48 +1120,40 @@ cudaError_t allow_smem(K kernel, size_t bytes, std::atomic<uint64_t> &done)
   return set;
 }
 
-template <typename T, int V, int P, int WARPS>
+template <typename T, int V, int P, int WARPS, bool SHIFT>
 int ln_fwd_many(const T *x, const float *gamma, const float *beta, T *y, float *mean, float *rstd, float epsilon, int rows,
                 int dim, cudaStream_t s)
 {
-  constexpr int BLOCK = kLnBlock<WARPS, 256>;
-  constexpr int SLOTS = BLOCK / (WARPS * 32);
-  constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 1>::kBytes;
+  constexpr int BLOCK = kLnBlock<WARPS>;
+  constexpr int SLOTS = kLnSlots<WARPS>;
+  constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 1, SHIFT>::kBytes;
   static std::atomic<uint64_t> done{0};
   if (kBytes > kLnPlainSmem)
   {
-    CAIFQ_CHECK_CUDA(allow_smem(layernorm_fwd_many_kernel<T, V, P, WARPS>, kBytes, done));
+    CAIFQ_CHECK_CUDA(allow_smem(layernorm_fwd_many_kernel<T, V, P, WARPS, SHIFT>, kBytes, done));
   }
-  const int blocks = (rows - 1) / SLOTS + 1;
-  const int most = 148 * (WARPS <= 8 ? 3 : 1);
-  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_many_kernel<T, V, P, WARPS>,
-                                    dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(BLOCK), kBytes, s, x,
-                                    gamma, beta, y, mean, rstd, epsilon, rows, dim));
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_many_kernel<T, V, P, WARPS, SHIFT>,
+                                    dim3(static_cast<unsigned>(walk_blocks<V>(rows, SLOTS, dim, kFwdBlocks<WARPS, SHIFT>))), dim3(BLOCK),
+                                    kBytes, s, x, gamma, beta, y, mean, rstd, epsilon, rows, dim));
   return CAIFQ_OK;
 }
 
-// the fewest warps (a power of two) whose registers hold the row
-#define CAIFQ_LN_WARPS(CALL, ELEMENTS)  \
-  if (dim <= 32 * (ELEMENTS))           \
-  {                                     \
-    return CALL(1);                     \
-  }                                     \
-  if (dim <= 64 * (ELEMENTS))           \
-  {                                     \
-    return CALL(2);                     \
-  }                                     \
-  if (dim <= 128 * (ELEMENTS))          \
-  {                                     \
-    return CALL(4);                     \
-  }                                     \
-  if (dim <= 256 * (ELEMENTS))          \
-  {                                     \
-    return CALL(8);                     \
-  }                                     \
-  if (dim <= 512 * (ELEMENTS))          \
-  {                                     \
-    return CALL(16);                    \
+// the fewest warps whose registers hold `reach` columns, ELEMENTS of them a thread
+#define CAIFQ_LN_CASE(CALL, W, ELEMENTS) \
+  if (reach <= 32 * (W) * (ELEMENTS))    \
+  {                                      \
+    return CALL(W);                      \
   }
+#define CAIFQ_LN_WARPS(CALL, ELEMENTS) \
+  CAIFQ_LN_CASE(CALL, 1, ELEMENTS)     \
+  CAIFQ_LN_CASE(CALL, 2, ELEMENTS)     \
+  CAIFQ_LN_CASE(CALL, 3, ELEMENTS)     \
+  CAIFQ_LN_CASE(CALL, 4, ELEMENTS)     \
+  CAIFQ_LN_CASE(CALL, 6, ELEMENTS)     \
+  CAIFQ_LN_CASE(CALL, 8, ELEMENTS)     \
+  CAIFQ_LN_CASE(CALL, 10, ELEMENTS)    \
+  CAIFQ_LN_CASE(CALL, 12, ELEMENTS)    \
+  CAIFQ_LN_CASE(CALL, 16, ELEMENTS)
 
 template <typename T>
 int ln_fwd(const void *xv, const float *gamma, const float *beta, void *yv, float *mean, float *rstd, float epsilon, int rows,
@@ -922,33 +1162,33 @@ int ln_fwd(const void *xv, const float *gamma, const float *beta, void *yv, floa
   const T *x = static_cast<const T *>(xv);
   T *y = static_cast<T *>(yv);
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  // (gamma and beta of 16 columns a thread fit the registers; of eight where every column has an address of its own)
-  if ((dim % V) == 0 && on_16(x) && on_16(y) && on_16(gamma) && on_16(beta))
+  if (on_16(x) && on_16(y))
   {
-#define CAIFQ_LN_CALL(W) ln_fwd_many<T, V, 16 / V, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
-    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+    const int64_t reach = reach_of<V>(dim);
+    // (gamma and beta of 16 columns a thread fit the registers)
+    if (dim % V == 0)
+    {
+      if (dim <= 32 * V)
+      {
+        return ln_fwd_many<T, V, 1, 1, false>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
+      }
+#define CAIFQ_LN_CALL(W) ln_fwd_many<T, V, 16 / V, W, false>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
+      CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
 #undef CAIFQ_LN_CALL
-    if (sizeof(T) == 2 && dim <= 512 * 4 * V)
+    }
+    else
+    {
+#define CAIFQ_LN_CALL(W) ln_fwd_many<T, V, 16 / V, W, true>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
+      CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
+#undef CAIFQ_LN_CALL
+    }
+    if (sizeof(T) == 2 && reach <= 512 * 4 * V)
     {
       return ln_fwd_rows<T, V, 4, 16>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
     }
-    if (dim <= 1024 * 4 * V)
+    if (reach <= 1024 * 4 * V)
     {
       return ln_fwd_rows<T, V, 4, 32>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
-    }
-  }
-  else
-  {
-#define CAIFQ_LN_CALL(W) ln_fwd_many<T, 1, 8, W>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s)
-    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 8)
-#undef CAIFQ_LN_CALL
-    if (dim <= 512 * 16)
-    {
-      return ln_fwd_rows<T, 1, 16, 16>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
-    }
-    if (dim <= 1024 * 16)
-    {
-      return ln_fwd_rows<T, 1, 16, 32>(x, gamma, beta, y, mean, rstd, epsilon, rows, dim, s);
     }
   }
   CAIFQ_CHECK_CUDA(launch_dependent(layernorm_fwd_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s, x, gamma, beta, y,
@@ -956,23 +1196,21 @@ int ln_fwd(const void *xv, const float *gamma, const float *beta, void *yv, floa
   return CAIFQ_OK;
 }
 
-template <typename T, int V, int P, int WARPS>
+template <typename T, int V, int P, int WARPS, bool SHIFT>
 int ln_bwd_rows(const T *dy, const T *x, const float *gamma, const float *mean, const float *rstd, T *dx, float *part,
                 int *slices, int rows, int dim, cudaStream_t s)
 {
-  constexpr int BLOCK = kLnBlock<WARPS, 256>;
-  constexpr int SLOTS = BLOCK / (WARPS * 32);
-  constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 2>::kBytes;
+  constexpr int BLOCK = kLnBlock<WARPS>;
+  constexpr int SLOTS = kLnSlots<WARPS>;
+  constexpr size_t kBytes = RowsAhead<T, V, P, WARPS * 32, BLOCK, 2, SHIFT>::kBytes;
   constexpr size_t kColumns = SLOTS > 1 ? sizeof(float) * 2 * P * V * WARPS * 32 : 0;   // of the widest row
   static std::atomic<uint64_t> done{0};
   if (kBytes + kColumns > kLnPlainSmem)
   {
-    CAIFQ_CHECK_CUDA(allow_smem(layernorm_bwd_rows_kernel<T, V, P, WARPS>, kBytes + kColumns, done));
+    CAIFQ_CHECK_CUDA(allow_smem(layernorm_bwd_rows_kernel<T, V, P, WARPS, SHIFT>, kBytes + kColumns, done));
   }
-  const int blocks = (rows - 1) / SLOTS + 1;
-  const int most = WARPS <= 8 ? 148 * 2 : 148;
-  *slices = blocks < most ? blocks : most;
-  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_bwd_rows_kernel<T, V, P, WARPS>, dim3(static_cast<unsigned>(*slices)), dim3(BLOCK),
+  *slices = walk_blocks<V>(rows, SLOTS, dim, kBwdBlocks<WARPS>);
+  CAIFQ_CHECK_CUDA(launch_dependent(layernorm_bwd_rows_kernel<T, V, P, WARPS, SHIFT>, dim3(static_cast<unsigned>(*slices)), dim3(BLOCK),
                                     kBytes + (SLOTS > 1 ? sizeof(float) * 2 * static_cast<size_t>(dim) : 0), s, dy, x, gamma,
                                     mean, rstd, dx, part, rows, dim));
   return CAIFQ_OK;
@@ -987,28 +1225,44 @@ int ln_bwd(const void *dyv, const void *xv, const float *gamma, const float *mea
   const T *x = static_cast<const T *>(xv);
   T *dx = static_cast<T *>(dxv);
   constexpr int V = 16 / static_cast<int>(sizeof(T));
-  if ((dim % V) == 0 && on_16(dy) && on_16(x) && on_16(dx) && on_16(gamma))
+  const bool pieces = on_16(dy) && on_16(x) && on_16(dx);
+  const int64_t reach = reach_of<V>(dim);
+  if (pieces && dim % V == 0)
   {
-#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, V, 16 / V, W>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
+    if (dim <= 32 * V)
+    {
+      return ln_bwd_rows<T, V, 1, 1, false>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s);
+    }
+#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, V, 16 / V, W, false>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
     CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 16)
 #undef CAIFQ_LN_CALL
   }
-  else
+  else if (pieces)
   {
-#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, 1, 8, W>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
-    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, 8)
+    constexpr int P = V == 4 ? 3 : 2;   // (four shifted pieces of two tensors in fp32 do not fit the registers)
+#define CAIFQ_LN_CALL(W) ln_bwd_rows<T, V, P, W, true>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s)
+    CAIFQ_LN_WARPS(CAIFQ_LN_CALL, P * V)
 #undef CAIFQ_LN_CALL
-    if (dim <= 512 * 16)
-    {
-      return ln_bwd_rows<T, 1, 16, 16>(dy, x, gamma, mean, rstd, dx, part, slices, rows, dim, s);
-    }
   }
-  *slices = ln_slices(rows);
+  // slices of at least 64 rows: a warp takes every eighth
+  const int most = rows / 64 < 1 ? 1 : rows / 64;
+  *slices = most < ln_slices(rows) ? most : ln_slices(rows);
   if (part != nullptr)
   {
     // (before dx, which may be written over dy)
-    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_columns_kernel<T>, dim3((dim + 31) / 32, static_cast<unsigned>(*slices)),
+    const bool whole = pieces && dim % V == 0;
+    const int wide = 32 * (whole ? V : 8);
+    CAIFQ_CHECK_CUDA(launch_dependent(whole ? layernorm_columns_kernel<T, V> : layernorm_columns_kernel<T, 1>,
+                                      dim3(static_cast<unsigned>((static_cast<int64_t>(dim) + wide - 1) / wide), static_cast<unsigned>(*slices)),
                                       dim3(kLnThreads), 0, s, dy, x, mean, rstd, part, rows, static_cast<int64_t>(dim)));
+  }
+  if (pieces && reach <= 1024 * 4 * V)
+  {
+    auto kernel = reach <= 1024 * 2 * V
+                      ? (dim % V == 0 ? layernorm_dx_rows_kernel<T, V, 2, 32, false> : layernorm_dx_rows_kernel<T, V, 2, 32, true>)
+                      : (dim % V == 0 ? layernorm_dx_rows_kernel<T, V, 4, 32, false> : layernorm_dx_rows_kernel<T, V, 4, 32, true>);
+    CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(rows)), dim3(1024), 0, s, dy, x, gamma, mean, rstd, dx, dim));
+    return CAIFQ_OK;
   }
   CAIFQ_CHECK_CUDA(launch_dependent(layernorm_dx_kernel<T>, dim3(ln_grid(rows)), dim3(kLnThreads), 0, s, dy, x, gamma, mean,
                                     rstd, dx, rows, static_cast<int64_t>(dim)));

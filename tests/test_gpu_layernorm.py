@@ -102,7 +102,8 @@ def test_layernorm(rows, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,dim", [(2100, 1024), (1500, 4096), (4000, 129), (700, 8192)])
+@pytest.mark.parametrize("rows,dim", [(2100, 1024), (1500, 4096), (4000, 129), (700, 8192), (3001, 1001), (1100, 4101), (600, 8191),
+                                      (500, 8197), (300, 16384), (40001, 5), (9000, 33), (2500, 640), (1700, 3001)])
 def test_layernorm_many_rows(rows, dim, dtype):
     x, dy, gamma, beta = make(rows, dim, dtype)
     got = nv.layernorm_fwd(x, gamma, beta, EPS)
@@ -188,31 +189,32 @@ def test_layernorm_equal_values_in_a_row():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_layernorm_in_place(dtype):
-    x, dy, gamma, beta = make(33, 2048, dtype)
+@pytest.mark.parametrize("rows,dim", [(33, 2048), (1900, 1001), (70, 8205), (3, 40000)])
+def test_layernorm_in_place(rows, dim, dtype):
+    x, dy, gamma, beta = make(rows, dim, dtype)
     y, mean, rstd = nv.layernorm_fwd(x, gamma, beta, EPS)
     dx, dg, db = nv.layernorm_bwd(dy, x, mean, rstd, gamma)
     x2, m2, r2 = x.clone(), torch.empty_like(mean), torch.empty_like(rstd)
     code = nv.dtype_code(x)
     nv._check(nv.lib().caifq_layernorm_fwd(nv._ptr(x2), nv._ptr(gamma), nv._ptr(beta), nv._ptr(x2), nv._ptr(m2), nv._ptr(r2),
-                                           EPS, code, 33, 2048, nv._stream()), "in place")
+                                           EPS, code, rows, dim, nv._stream()), "in place")
     assert torch.equal(x2, y) and torch.equal(m2, mean) and torch.equal(r2, rstd)
-    ws = torch.empty(nv.lib().caifq_layernorm_bwd_workspace_bytes(33, 2048), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(nv.lib().caifq_layernorm_bwd_workspace_bytes(rows, dim), dtype=torch.uint8, device="cuda")
     for over_dy in (True, False):
         d2, x2, g2, b2 = dy.clone(), x.clone(), torch.empty_like(dg), torch.empty_like(db)
         nv._check(nv.lib().caifq_layernorm_bwd(nv._ptr(d2), nv._ptr(x2), nv._ptr(gamma), nv._ptr(mean), nv._ptr(rstd),
-                                               nv._ptr(d2 if over_dy else x2), nv._ptr(g2), nv._ptr(b2), 0, nv._ptr(ws), code, 33, 2048,
+                                               nv._ptr(d2 if over_dy else x2), nv._ptr(g2), nv._ptr(b2), 0, nv._ptr(ws), code, rows, dim,
                                                nv._stream()), "in place")
         assert torch.equal(d2 if over_dy else x2, dx) and torch.equal(g2, dg) and torch.equal(b2, db)
     # rows alone, without a workspace
     d3 = torch.empty_like(dy)
     nv._check(nv.lib().caifq_layernorm_bwd(nv._ptr(dy), nv._ptr(x), nv._ptr(gamma), nv._ptr(mean), nv._ptr(rstd), nv._ptr(d3),
-                                           None, None, 0, None, code, 33, 2048, nv._stream()), "dx alone")
+                                           None, None, 0, None, code, rows, dim, nv._stream()), "dx alone")
     assert torch.equal(d3, dx)
     # one of the two gradients
     g3 = torch.empty_like(dg)
     nv._check(nv.lib().caifq_layernorm_bwd(nv._ptr(dy), nv._ptr(x), nv._ptr(gamma), nv._ptr(mean), nv._ptr(rstd), nv._ptr(d3),
-                                           nv._ptr(g3), None, 0, nv._ptr(ws), code, 33, 2048, nv._stream()), "dgamma alone")
+                                           nv._ptr(g3), None, 0, nv._ptr(ws), code, rows, dim, nv._stream()), "dgamma alone")
     assert torch.equal(g3, dg)
 
 
