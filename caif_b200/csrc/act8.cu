@@ -762,33 +762,47 @@ act_nt_mma_kernel(const __nv_bfloat16 *dy, const __nv_bfloat16 *bt, __nv_bfloat1
   }
 }
 
-// the slices' sums, rounded once: [out][r] as it lies, [in][r] turned to [r, in]
-__global__ void __launch_bounds__(256)
-gradients_kernel(const float *part, void *d_b, void *d_a, int dtype, float factor, int slices, int64_t n_b, int in, int r)
+// the slices' sums, rounded once: [out][r] as it lies, [in][r] turned to [r, in]; `block` of 256 sums
+struct GradientSums
 {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t n = n_b + static_cast<int64_t>(in) * r;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const float *part;
+  void *d_b;
+  void *d_a;
+  float factor;
+  int dtype, slices, in, r;
+  int64_t n_b;
+};
+
+__device__ __forceinline__ void gradient_sums(const GradientSums &j, int64_t block)
+{
+  const int64_t n = j.n_b + static_cast<int64_t>(j.in) * j.r;
+  const int64_t i = block * 256 + threadIdx.x;
   if (i >= n)
   {
     return;
   }
   float s = 0.0f;
 #pragma unroll 4
-  for (int z = 0; z < slices; ++z)
+  for (int z = 0; z < j.slices; ++z)
   {
-    s += part[static_cast<int64_t>(z) * n + i];
+    s += j.part[static_cast<int64_t>(z) * n + i];
   }
-  if (i < n_b)
+  if (i < j.n_b)
   {
-    store_from_float(d_b, i, dtype, s * factor);
+    store_from_float(j.d_b, i, j.dtype, s * j.factor);
   }
   else
   {
-    const int64_t e = i - n_b;
-    store_from_float(d_a, (e % r) * in + e / r, dtype, s * factor);
+    const int64_t e = i - j.n_b;
+    store_from_float(j.d_a, (e % j.r) * j.in + e / j.r, j.dtype, s * j.factor);
   }
+}
+
+__global__ void __launch_bounds__(256) gradients_kernel(const GradientSums j)
+{
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  gradient_sums(j, blockIdx.x);
 }
 
 // ---- what the general form of the backward pass multiplies by itself ----
@@ -797,8 +811,9 @@ constexpr int kDhChunk = 1024;
 
 // dH[m, r] = dy . B, fp32: a block a row.  B's rows lie one behind the other, so the block reads it as one run of numbers and a
 // thread always meets the same column of it; the row of dy waits in shared memory.
+template <typename T>
 __global__ void __launch_bounds__(256)
-dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r)
+dh_row_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r)
 {
   __shared__ float row[kDhChunk];
   __shared__ float sums[256];
@@ -819,7 +834,7 @@ dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int ou
       __syncthreads();   // the chunk before has been read
       for (int i = tid; i < n; i += 256)
       {
-        row[i] = load_as_float(dy, at * out + c0 + i, dtype);
+        row[i] = act_f<T>(dy[at * out + c0 + i]);
       }
       __syncthreads();
       if (group < groups)
@@ -831,7 +846,7 @@ dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int ou
 #pragma unroll
           for (int u = 0; u < 16; ++u)
           {
-            w[u] = load_as_float(b, static_cast<int64_t>(c0 + o + u * groups) * r + j0 + j, dtype);
+            w[u] = act_f<T>(b[static_cast<int64_t>(c0 + o + u * groups) * r + j0 + j]);
           }
 #pragma unroll
           for (int u = 0; u < 16; ++u)
@@ -841,7 +856,7 @@ dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int ou
         }
         for (; o < n; o += groups)
         {
-          s[0] = fmaf(row[o], load_as_float(b, static_cast<int64_t>(c0 + o) * r + j0 + j, dtype), s[0]);
+          s[0] = fmaf(row[o], act_f<T>(b[static_cast<int64_t>(c0 + o) * r + j0 + j]), s[0]);
         }
       }
     }
@@ -860,37 +875,157 @@ dh_kernel(const void *dy, const void *b, float *dh, int dtype, int64_t m, int ou
   }
 }
 
-// dx[m, in] = factor * dH . A: a thread a column
+// The same where B is large: a cluster four rows, its blocks a share of the columns each; a number of B serves the four rows, and the
+// blocks' sums are added in order.
+constexpr int kDhRows = 4;
+constexpr int kDhPart = 512;
+
+template <typename T>
 __global__ void __launch_bounds__(256)
-dx_adapter_kernel(const float *dh, const void *a, void *dx, int dtype, float factor, int in, int r)
+dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int cluster)
+{
+  __shared__ float row[kDhRows][kDhPart];
+  __shared__ float sums[kDhRows][256];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tid = threadIdx.x;
+  const int rank = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x / cluster) * kDhRows;
+  const int begin = static_cast<int>(static_cast<int64_t>(out) * rank / cluster);
+  const int end = static_cast<int>(static_cast<int64_t>(out) * (rank + 1) / cluster);
+  for (int j0 = 0; j0 < r; j0 += 256)
+  {
+    const int width = r - j0 < 256 ? r - j0 : 256;   // columns of this trip
+    const int groups = 256 / width;                  // rows of B at a time
+    const int j = tid % width;
+    const int group = tid / width;
+    float s[kDhRows][4] = {};
+    for (int c0 = begin; c0 < end; c0 += kDhPart)
+    {
+      const int n = end - c0 < kDhPart ? end - c0 : kDhPart;
+      __syncthreads();   // the chunk before has been read
+      for (int i = tid; i < kDhRows * kDhPart; i += 256)
+      {
+        const int rr = i / kDhPart;
+        const int c = i % kDhPart;
+        row[rr][c] = row0 + rr < m && c < n ? act_f<T>(dy[(row0 + rr) * out + c0 + c]) : 0.0f;
+      }
+      __syncthreads();
+      if (group < groups)
+      {
+        for (int o = group; o < n; o += 16 * groups)
+        {
+          float w[16];
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+          {
+            const int at = o + u * groups;
+            w[u] = act_f<T>(b[static_cast<int64_t>(c0 + (at < n ? at : 0)) * r + j0 + j]);   // (one that is there, in any case)
+          }
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+          {
+            const int at = o + u * groups;
+#pragma unroll
+            for (int rr = 0; rr < kDhRows; ++rr)
+            {
+              s[rr][u & 3] = fmaf(at < n ? row[rr][at] : 0.0f, at < n ? w[u] : 0.0f, s[rr][u & 3]);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int rr = 0; rr < kDhRows; ++rr)
+    {
+      sums[rr][tid] = (s[rr][0] + s[rr][1]) + (s[rr][2] + s[rr][3]);
+    }
+    __syncthreads();
+    // a thread adds the groups of one row and column; in place, where its own first group lies
+    for (int e = tid; e < kDhRows * width; e += 256)
+    {
+      float v = 0.0f;
+      for (int i = 0; i < groups; ++i)
+      {
+        v += sums[e / width][i * width + e % width];
+      }
+      sums[e / width][e % width] = v;
+    }
+    if (cluster > 1)
+    {
+      cluster_sync_all();
+    }
+    else
+    {
+      __syncthreads();
+    }
+    for (int e = rank * 256 + tid; e < kDhRows * width; e += cluster * 256)
+    {
+      const int rr = e / width;
+      float v = sums[rr][e % width];
+      if (cluster > 1)
+      {
+        const uint32_t mine = smem_u32(&sums[rr][e % width]);
+        float from[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)   // (all on their way before the first is added)
+        {
+          from[k] = k < cluster ? __uint_as_float(ld_shared_cluster(map_to_cta(mine, static_cast<uint32_t>(k)))) : 0.0f;
+        }
+        v = ((from[0] + from[1]) + (from[2] + from[3])) + ((from[4] + from[5]) + (from[6] + from[7]));
+      }
+      if (row0 + rr < m)
+      {
+        dh[(row0 + rr) * r + j0 + e % width] = v;
+      }
+    }
+    if (cluster > 1)
+    {
+      cluster_sync_all();   // nobody's sums are written again, or left, while they are read
+    }
+  }
+}
+
+// The sums (the first blocks) and dx[m, in] = factor * dH . A, a thread a column, which needs none of them, in one launch
+template <typename T>
+__global__ void __launch_bounds__(256)
+gradients_dx_kernel(const GradientSums j, int sum_blocks, const float *dh, const T *a, T *dx)
 {
   __shared__ float row[256];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t at = blockIdx.x;
-  const int c = blockIdx.y * 256 + static_cast<int>(threadIdx.x);
+  if (static_cast<int>(blockIdx.x) < sum_blocks)
+  {
+    gradient_sums(j, blockIdx.x);
+    return;
+  }
+  const int parts = (j.in + 255) / 256;   // blocks of a row
+  const int64_t block = static_cast<int64_t>(blockIdx.x) - sum_blocks;
+  const int64_t at = block / parts;
+  const int c = static_cast<int>(block % parts) * 256 + static_cast<int>(threadIdx.x);
   float s = 0.0f;
-  for (int j0 = 0; j0 < r; j0 += 256)
+  for (int j0 = 0; j0 < j.r; j0 += 256)
   {
     __syncthreads();
-    if (j0 + static_cast<int>(threadIdx.x) < r)
+    if (j0 + static_cast<int>(threadIdx.x) < j.r)
     {
-      row[threadIdx.x] = dh[at * r + j0 + threadIdx.x];
+      row[threadIdx.x] = dh[at * j.r + j0 + threadIdx.x];
     }
     __syncthreads();
-    const int n = r - j0 < 256 ? r - j0 : 256;
-    if (c < in)
+    const int n = j.r - j0 < 256 ? j.r - j0 : 256;
+    if (c < j.in)
     {
 #pragma unroll 8
-      for (int j = 0; j < n; ++j)
+      for (int k = 0; k < n; ++k)
       {
-        s = fmaf(row[j], load_as_float(a, static_cast<int64_t>(j0 + j) * in + c, dtype), s);
+        s = fmaf(row[k], act_f<T>(a[static_cast<int64_t>(j0 + k) * j.in + c]), s);
       }
     }
   }
-  if (c < in)
+  if (c < j.in)
   {
-    store_from_float(dx, at * in + c, dtype, s * factor);
+    dx[at * j.in + c] = act_t<T>(s * j.factor);
   }
 }
 
@@ -952,10 +1087,25 @@ size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r)
   return static_cast<size_t>(general > tiled ? general : tiled) * (static_cast<size_t>(out) + in) * r * sizeof(float);
 }
 
-// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * dh^T . x, x packed.  m >= 1; dy, h, d_a, d_b in dtype
+namespace
+{
+template <typename T>
+int launch_gradients_dx(const GradientSums &j, int64_t sum_blocks, const float *dh, const void *a, void *dx, int64_t m, cudaStream_t s)
+{
+  const int64_t blocks = sum_blocks + m * ((j.in + 255) / 256);
+  CAIFQ_CHECK_ARG(blocks <= 0x7FFFFFFF, "LoRA backward on packed rows: %lld rows of %d columns are too many for its general form",
+                  static_cast<long long>(m), j.in);
+  CAIFQ_CHECK_CUDA(launch_dependent(gradients_dx_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, j,
+                                    static_cast<int>(sum_blocks), dh, static_cast<const T *>(a), static_cast<T *>(dx)));
+  return CAIFQ_OK;
+}
+}  // namespace
+
+// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * dh^T . x, x packed; with dx (dh is fp32 then) dx[m, in] = factor * dh . a
+// too.  m >= 1; dy, h, a, d_b, d_a, dx in dtype
 int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
-                         void *d_b, void *d_a, int dtype, float factor, float *scratch, int64_t m, int out, int in, int r,
-                         cudaStream_t s)
+                         void *d_b, void *d_a, const void *a, void *dx, int dtype, float factor, float *scratch, int64_t m, int out,
+                         int in, int r, cudaStream_t s)
 {
   const Gradients j{dy, h, dh, x, scales, scratch, dtype, dh_dtype, out, in, r};
   auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
@@ -977,10 +1127,22 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
     CAIFQ_CHECK_CUDA(launch_dependent(act_tn_kernel, grid, dim3(256), 0, s, j, m));
   }
   const int64_t n = (static_cast<int64_t>(out) + in) * r;
-  CAIFQ_CHECK_CUDA(launch_dependent(gradients_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s,
-                                    static_cast<const float *>(scratch), d_b, d_a, dtype, factor, slices,
-                                    static_cast<int64_t>(out) * r, in, r));
-  return CAIFQ_OK;
+  const int64_t blocks = (n + 255) / 256;
+  const GradientSums sums{scratch, d_b, d_a, factor, dtype, slices, in, r, static_cast<int64_t>(out) * r};
+  if (dx == nullptr)
+  {
+    CAIFQ_CHECK_CUDA(launch_dependent(gradients_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, sums));
+    return CAIFQ_OK;
+  }
+  switch (dtype)
+  {
+    case CAIFQ_F32:
+      return launch_gradients_dx<float>(sums, blocks, static_cast<const float *>(dh), a, dx, m, s);
+    case CAIFQ_F16:
+      return launch_gradients_dx<__half>(sums, blocks, static_cast<const float *>(dh), a, dx, m, s);
+    default:
+      return launch_gradients_dx<__nv_bfloat16>(sums, blocks, static_cast<const float *>(dh), a, dx, m, s);
+  }
 }
 
 // dh[m, r] = dy . bt^T in bf16 and padded[m, 64] = bf16(dh * mul / *div): bf16 operands on 16-byte boundaries, r 8, 16, 32 or 64, out a
@@ -996,19 +1158,57 @@ int launch_act_nt(const void *dy, const void *bt, void *dh, void *padded, float 
   return CAIFQ_OK;
 }
 
+namespace
+{
+template <typename T>
+int launch_dh_of(const void *dy, const void *b, float *dh, int64_t m, int out, int r, cudaStream_t s)
+{
+  // A block a row where a thread then reads up to 64 numbers of B: four rows a block, and clusters, cost 2 us and more there (64 rows,
+  // 1024 columns, rank 16), and save 30 of 91 where it would read 480 (152 rows, 1920 columns, rank 64)
+  const bool large = static_cast<int64_t>(out) * r > 64 * 256;
+  const int64_t groups = large ? (m + 3) / 4 : m;
+  int cluster = 1;
+  while (large && cluster < 8 && groups * cluster < 4 * 148 && static_cast<int64_t>(out) * r > static_cast<int64_t>(64 * 256) * cluster)
+  {
+    cluster *= 2;
+  }
+  if (!large)
+  {
+    CAIFQ_CHECK_CUDA(launch_dependent(dh_row_kernel<T>, dim3(static_cast<unsigned>(m)), dim3(256), 0, s, static_cast<const T *>(dy),
+                                      static_cast<const T *>(b), dh, m, out, r));
+    return CAIFQ_OK;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * cluster));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent_launches() ? 2 : 1;
+  CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dh_kernel<T>, static_cast<const T *>(dy),
+                                      static_cast<const T *>(b), dh, m, out, r, cluster));
+  return CAIFQ_OK;
+}
+}  // namespace
+
 // dh[m, r] (fp32) = dy . b, dy and b in dtype
 int launch_dh(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r, cudaStream_t s)
 {
-  CAIFQ_CHECK_CUDA(launch_dependent(dh_kernel, dim3(static_cast<unsigned>(m)), dim3(256), 0, s, dy, b, dh, dtype, m, out, r));
-  return CAIFQ_OK;
-}
-
-// dx[m, in] = factor * dh . a, dx and a in dtype
-int launch_dx_adapter(const float *dh, const void *a, void *dx, int dtype, float factor, int64_t m, int in, int r, cudaStream_t s)
-{
-  CAIFQ_CHECK_CUDA(launch_dependent(dx_adapter_kernel, dim3(static_cast<unsigned>(m), (in + 255) / 256), dim3(256), 0, s, dh, a, dx,
-                                    dtype, factor, in, r));
-  return CAIFQ_OK;
+  switch (dtype)
+  {
+    case CAIFQ_F32:
+      return launch_dh_of<float>(dy, b, dh, m, out, r, s);
+    case CAIFQ_F16:
+      return launch_dh_of<__half>(dy, b, dh, m, out, r, s);
+    default:
+      return launch_dh_of<__nv_bfloat16>(dy, b, dh, m, out, r, s);
+  }
 }
 
 }  // namespace caifq

@@ -140,12 +140,11 @@ int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, in
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
 size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r);
 int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
-                         void *d_b, void *d_a, int dtype, float factor, float *scratch, int64_t m, int out, int in, int r,
-                         cudaStream_t s);
+                         void *d_b, void *d_a, const void *a, void *dx, int dtype, float factor, float *scratch, int64_t m, int out,
+                         int in, int r, cudaStream_t s);
 int launch_act_nt(const void *dy, const void *bt, void *dh, void *padded, float mul, const float *div, int64_t m, int out, int r,
                   cudaStream_t s);
 int launch_dh(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r, cudaStream_t s);
-int launch_dx_adapter(const float *dh, const void *a, void *dx, int dtype, float factor, int64_t m, int in, int r, cudaStream_t s);
 // layernorm.cu
 size_t layernorm_bwd_workspace_bytes(int rows, int dim);
 int launch_layernorm_fwd(const void *x, const float *gamma, const float *beta, void *y, float *mean, float *rstd,
@@ -1325,8 +1324,8 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
     }
     if (r == CAIFQ_OK)
     {
-      r = launch_act_gradients(dy, hidden, d_hidden, sd, x_codes, x_scales, d_b, d_a, sd, scale, sums, m, w->out_dim, w->in_dim,
-                               lora->rank, s);
+      r = launch_act_gradients(dy, hidden, d_hidden, sd, x_codes, x_scales, d_b, d_a, nullptr, nullptr, sd, scale, sums, m, w->out_dim,
+                               w->in_dim, lora->rank, s);
     }
     if (r != CAIFQ_OK)
     {
@@ -1341,12 +1340,8 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
   int r = launch_dh(dy, lora->b, static_cast<float *>(d_hidden), sd, m, w->out_dim, lora->rank, s);
   if (r == CAIFQ_OK)
   {
-    r = launch_act_gradients(dy, hidden, d_hidden, CAIFQ_F32, x_codes, x_scales, d_b, d_a, sd, scale, sums, m, w->out_dim,
+    r = launch_act_gradients(dy, hidden, d_hidden, CAIFQ_F32, x_codes, x_scales, d_b, d_a, lora->a, dx, sd, scale, sums, m, w->out_dim,
                              w->in_dim, lora->rank, s);
-  }
-  if (r == CAIFQ_OK)
-  {
-    r = launch_dx_adapter(static_cast<const float *>(d_hidden), lora->a, dx, sd, scale, m, w->in_dim, lora->rank, s);
   }
   if (r != CAIFQ_OK)
   {

@@ -64,12 +64,19 @@ bank_down_kernel(const T *x, const int32_t *__restrict__ adapter_of_row, const c
     const T *w = a + static_cast<int64_t>(j) * in_dim;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     int c = lane;
-    for (; c + 96 < in_dim; c += 128)
+    for (; c + 480 < in_dim; c += 512)   // (bound by latency: sixteen loads of each on their way)
     {
+      T u[16], v[16];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 16; ++i)
       {
-        s[i] = fmaf(bank_f<T>(src[c + 32 * i]), bank_f<T>(w[c + 32 * i]), s[i]);
+        u[i] = src[c + 32 * i];
+        v[i] = w[c + 32 * i];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+      {
+        s[i & 3] = fmaf(bank_f<T>(u[i]), bank_f<T>(v[i]), s[i & 3]);
       }
     }
     for (; c < in_dim; c += 32)
@@ -412,19 +419,45 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
   {
     c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
   }
-#pragma unroll 4
-  for (int st = begin; st < end; ++st)
+  if constexpr (NT <= 4)
   {
-    const uint4 xa = lo ? __ldg(x_lo + st * 4) : zero4;
-    const uint4 xb = hi ? __ldg(x_hi + st * 4) : zero4;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll 4
+    for (int st = begin; st < end; ++st)
     {
-      if (nt < eights)
+      const uint4 xa = lo ? __ldg(x_lo + st * 4) : zero4;
+      const uint4 xb = hi ? __ldg(x_hi + st * 4) : zero4;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
       {
-        const uint4 w = __ldg(a_row + static_cast<int64_t>(nt) * in_dim + st * 4);
-        mma_16816(c[nt], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
-        mma_16816(c[nt], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+        if (nt < eights)
+        {
+          const uint4 w = __ldg(a_row + static_cast<int64_t>(nt) * in_dim + st * 4);
+          mma_16816(c[nt], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+          mma_16816(c[nt], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+        }
+      }
+    }
+  }
+  else
+  {
+    // (all loads of two steps before the first product: 7000 rows, 50 adapters up to rank 64, 336 -> 317 us, 64 rows 38 -> 36; with
+    // fewer rows of A a step the products on zeros cost more than the branches)
+#pragma unroll 2
+    for (int st = begin; st < end; ++st)
+    {
+      const uint4 xa = lo ? __ldg(x_lo + st * 4) : zero4;
+      const uint4 xb = hi ? __ldg(x_hi + st * 4) : zero4;
+      uint4 w[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+      {
+        w[nt] = nt < eights ? __ldg(a_row + static_cast<int64_t>(nt) * in_dim + st * 4) : zero4;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+      {
+        mma_16816(c[nt], xa.x, xb.x, xa.y, xb.y, w[nt].x, w[nt].y);
+        mma_16816(c[nt], xa.z, xb.z, xa.w, xb.w, w[nt].z, w[nt].w);
       }
     }
   }
