@@ -73,7 +73,7 @@ struct ActTrips
 
   __device__ __forceinline__ ActTrips(int64_t rows, int dim)
   {
-    blocks = (dim + kActBlock - 1) / kActBlock;
+    blocks = static_cast<int>((static_cast<int64_t>(dim) + kActBlock - 1) / kActBlock);
     trips = (blocks + kActTrain - 1) / kActTrain;
     total = rows * trips;
   }

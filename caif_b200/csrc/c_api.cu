@@ -1109,6 +1109,7 @@ int check_bank(const caifq_weight *w, const caifq_lora_bank *bank, const char *w
     return rc;
   }
   CAIFQ_CHECK_ARG(bank != nullptr && bank->entries != nullptr && bank->count > 0, "%s: the bank is empty", who);
+  CAIFQ_CHECK_ARG(bank->count <= kBankMost, "%s: %d adapters, at most %d are taken", who, bank->count, kBankMost);
   CAIFQ_CHECK_ARG(is_float_dtype(bank->dtype), "%s: the bank's dtype must be F32, F16 or BF16", who);
   CAIFQ_CHECK_ARG(bank->max_rank >= 1 && bank->max_rank <= kBankMaxRank, "%s: ranks from 1 to %d, not %d", who, kBankMaxRank,
                   bank->max_rank);
@@ -1144,6 +1145,7 @@ int caifq_lora_bank_entries(const caifq_lora *loras, int32_t count, int32_t in_d
 {
   const char *who = "caifq_lora_bank_entries";
   CAIFQ_CHECK_ARG(loras != nullptr && count > 0, "%s: no adapters", who);
+  CAIFQ_CHECK_ARG(count <= kBankMost, "%s: %d adapters, at most %d are taken", who, count, kBankMost);
   CAIFQ_CHECK_ARG(entries_host != nullptr && bank != nullptr, "%s: null pointer", who);
   CAIFQ_CHECK_ARG(in_dim > 0 && out_dim > 0, "%s: bad dims in=%d out=%d", who, in_dim, out_dim);
   caifq_lora_bank b{};

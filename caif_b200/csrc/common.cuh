@@ -420,6 +420,7 @@ struct LinearArgs
 };
 
 constexpr int kMaxPeers = 8;
+constexpr int kBankMost = 1 << 24;     // adapters of a bank
 constexpr int kBankMaxRank = 1024;   // of an adapter bank: a row of x . A^T lies in shared memory
 
 // generic tiled fp32-FMA GEMM over every (storage, compute) cell

@@ -1323,7 +1323,7 @@ int launch_layernorm_bwd(const void *dy, const void *x, const float *gamma, cons
   }
   if (columns)
   {
-    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_finish_kernel, dim3((dim + 31) / 32, 2), dim3(1024), 0, s,
+    CAIFQ_CHECK_CUDA(launch_dependent(layernorm_finish_kernel, dim3(static_cast<unsigned>((static_cast<int64_t>(dim) + 31) / 32), 2), dim3(1024), 0, s,
                                       static_cast<const float *>(workspace), grad_gamma, grad_beta, slices,
                                       static_cast<int64_t>(dim), accumulate));
   }

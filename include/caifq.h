@@ -357,7 +357,7 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
  * replays of a captured call; rows need no order.  x . A^T and the frozen product are kept in fp32; the result is rounded
  * once.
  *
- * A bank is a table of `count` entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
+ * A bank is a table of `count` (up to 2^24) entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
  * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank]), fills the table's image in HOST memory and every
  * field of *bank but `entries`; the caller copies the image to the device and sets bank->entries to it.  It needs no GPU.
  * Factors stay where they are and must outlive the calls.
