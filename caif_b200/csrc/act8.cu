@@ -1178,21 +1178,8 @@ int launch_dh_of(const void *dy, const void *b, float *dh, int64_t m, int out, i
                                       static_cast<const T *>(b), dh, m, out, r));
     return CAIFQ_OK;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(groups * cluster));
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent_launches() ? 2 : 1;
-  CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, dh_kernel<T>, static_cast<const T *>(dy),
-                                      static_cast<const T *>(b), dh, m, out, r, cluster));
+  CAIFQ_CHECK_CUDA(launch_dependent_clusters(dh_kernel<T>, dim3(static_cast<unsigned>(groups * cluster)), dim3(256), 0, s, cluster,
+                                             static_cast<const T *>(dy), static_cast<const T *>(b), dh, m, out, r, cluster));
   return CAIFQ_OK;
 }
 }  // namespace

@@ -111,6 +111,25 @@ def test_layernorm_many_rows(rows, dim, dtype):
     check_bwd(dy, x, got[1], got[2], gamma, nv.layernorm_bwd(dy, x, got[1], got[2], gamma))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,dim", [(400, 10000), (350, 12288), (260, 12296), (200, 20480), (170, 24584), (120, 24577), (40, 49149),
+                                      (60, 65536), (30, 65537), (70, 70000)])
+def test_layernorm_wide_rows(rows, dim, dtype):
+    x, dy, gamma, beta = make(rows, dim, dtype)
+    got = nv.layernorm_fwd(x, gamma, beta, EPS)
+    check_fwd(x, gamma, beta, got)
+    want = nv.layernorm_bwd(dy, x, got[1], got[2], gamma)
+    check_bwd(dy, x, got[1], got[2], gamma, want)
+    for a, b in zip(nv.layernorm_bwd(dy, x, got[1], got[2], gamma), want):
+        assert torch.equal(a, b)
+    # without the columns' sums, and in place
+    lib, s = nv.lib(), torch.cuda.current_stream().cuda_stream
+    code = {torch.float32: nv.F32, torch.float16: nv.F16, torch.bfloat16: nv.BF16}[dtype]
+    assert lib.caifq_layernorm_bwd(dy.data_ptr(), x.data_ptr(), gamma.data_ptr(), got[1].data_ptr(), got[2].data_ptr(), dy.data_ptr(),
+                                   None, None, 0, None, code, rows, dim, s) == 0
+    assert torch.equal(dy, want[0])
+
+
 @pytest.mark.parametrize("dim", [40, 1001, 4096])
 def test_layernorm_without_gamma_or_beta(dim):
     x, dy, gamma, beta = make(9, dim, torch.bfloat16)
