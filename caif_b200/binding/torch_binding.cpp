@@ -618,12 +618,13 @@ at::Tensor workspace_on(const at::Tensor *given, size_t need, const at::Tensor &
   return workspace_of(given, need, like, who);
 }
 
-// (weight, bank, adapter_of_row, x, compute, out | None, workspace | None) -> y
+// (weight, bank, its table, adapter_of_row, x, compute, out | None, workspace | None) -> y
 PyObject *lora_bank_linear_fwd(Args &a)
 {
   const char *who = "lora_bank_linear_fwd";
   const caifq_weight *w = a.record<caifq_weight>();
   const caifq_lora_bank *bank = a.record<caifq_lora_bank>();
+  const at::Tensor &table = *a.tensor();
   const at::Tensor &rows = *a.tensor();
   const at::Tensor &x = *a.tensor();
   const int compute = static_cast<int>(a.integer());
@@ -635,6 +636,7 @@ PyObject *lora_bank_linear_fwd(Args &a)
   }
   const int64_t m = rows_of(x, w->in_dim);
   const OnDevice on(x, who);
+  on.same(&table, "the bank's table", at::kByte, -1);
   on.same(&rows, "adapter_of_row", at::kInt, m);
   const std::vector<int64_t> shape = shape_with_last(x, w->out_dim);
   on.same(out, "out", x.scalar_type(), m * w->out_dim);

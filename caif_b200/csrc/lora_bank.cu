@@ -141,7 +141,9 @@ bank_up_kernel(const float *frozen, const float *h, const int32_t *__restrict__ 
 // Which tile and slot a row gets does not change its arithmetic, so results do not depend on the rows' order.
 
 constexpr int kTileRows = 16;
-constexpr int kSmallCall = 128;     // rows that a block sorts by itself
+// rows that a block sorts by itself.  4096 -> 4096 int4, 48 rows of 16 adapters: 19.1 us so, 24.3 with the launch ahead; 1024 -> 1024, 128
+// rows of 16: 15.7 and 19.2; 4096 -> 14336, 128 rows of 48: 43.1 and 43.5
+constexpr int kSmallCall = 128;
 constexpr int kTableMost = 4096;    // adapters that the launch ahead counts in shared memory
 
 // what `down` leaves for `up`, in the workspace
@@ -301,7 +303,7 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 __device__ __forceinline__ bool small_tile(const int32_t *adapter_of_row, const caifq_lora_entry *entries, int count, int m, int tile,
                                            int (&rows)[kTileRows], caifq_lora_entry &entry)
 {
-  __shared__ int id_of[kSmallCall];
+  __shared__ __align__(16) int id_of[kSmallCall];
   __shared__ int warp_tiles[kSmallCall / 32];
   __shared__ int lead[2];   // the row that begins the tile, and how many of its adapter come before it
   const int i = threadIdx.x;
@@ -315,10 +317,11 @@ __device__ __forceinline__ bool small_tile(const int32_t *adapter_of_row, const 
     rows[i] = -1;
   }
   __syncthreads();
-  int before = 0;
-  for (int k = 0; k < (i < m ? i : 0); ++k)
+  int before = __popc(__match_any_sync(0xFFFFFFFFu, id) & ((1u << (i & 31)) - 1u));
+  for (int k = 0; k < (i < m ? (i & ~31) : 0); k += 4)
   {
-    before += id_of[k] == id ? 1 : 0;
+    const int4 o = *reinterpret_cast<const int4 *>(id_of + k);
+    before += (o.x == id ? 1 : 0) + (o.y == id ? 1 : 0) + (o.z == id ? 1 : 0) + (o.w == id ? 1 : 0);
   }
   const bool begins = i < m && before % kTileRows == 0;
   const uint32_t mask = __ballot_sync(0xFFFFFFFFu, begins);
@@ -699,7 +702,9 @@ int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
     CAIFQ_CHECK_CUDA(launch_dependent(bank_plan_kernel, dim3(1), dim3(1024), static_cast<size_t>(bank.count + 1) * 2 * sizeof(int), s,
                                       adapter_of_row, bank.entries, bank.count, plan, m, static_cast<int>(tiles)));
   }
-  // clusters that split the columns where the tiles leave SMs without work, with at least two steps of 32 columns for every warp
+  // clusters that split the columns where the tiles leave SMs without work, with at least two steps of 32 columns for every warp.
+  // (4096 -> 14336 int4, 8 rows of 4 adapters: 17.8 us, 28.5 with one block a tile; 14336 -> 4096, 16 rows: 34.5 and 75.9; 4096 -> 4096, 48
+  // rows of 16: 19.3 and 21.3; the least gain, 1024 -> 1024, 128 rows of 16: 16.3 and 15.6)
   int cluster = 1;
   while (cluster < 8 && tiles * cluster < 2 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
   {
@@ -722,21 +727,9 @@ int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
   {
     down = small ? bank_down_mma_kernel<8, true> : bank_down_mma_kernel<8, false>;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * cluster));
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = dependent_launches() ? 2 : 1;
-  CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, down, static_cast<const __nv_bfloat16 *>(x), adapter_of_row, bank.entries,
-                                      bank.count, plan, bank.max_rank, m, bank.in_dim, cluster));
+  CAIFQ_CHECK_CUDA(launch_dependent_clusters(down, dim3(static_cast<unsigned>(tiles * cluster)), dim3(256), 0, s, cluster,
+                                             static_cast<const __nv_bfloat16 *>(x), adapter_of_row, bank.entries, bank.count, plan,
+                                             bank.max_rank, m, bank.in_dim, cluster));
   return CAIFQ_OK;
 }
 

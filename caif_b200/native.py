@@ -482,7 +482,7 @@ def lora_bank_workspace_bytes(w, bank, m, compute=F32):
 def lora_bank_linear_fwd(w, bank, adapter_of_row, x, compute=F32, out=None, workspace=None):
     """y = W-path(x) + each row's own adapter: adapter_of_row is an int32 tensor with an index into the bank for every row of
     x, or any value outside it (-1) for a row without one.  The indices may change between replays of a captured call."""
-    return (_native or _binding()).lora_bank_linear_fwd(w, bank, adapter_of_row, x, compute, out, workspace)
+    return (_native or _binding()).lora_bank_linear_fwd(w, bank, bank.table, adapter_of_row, x, compute, out, workspace)
 
 
 # ---- activations kept in 8 bits ------------------------------------------------

@@ -1,5 +1,9 @@
 """An adapted projection behind a layer norm, as a fine-tune and a server use it: the calls one after the other, against the
 same chain in 64 bits from the same inputs."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -102,3 +106,14 @@ def test_serving_step_of_requests_with_adapters_of_their_own(m):
         x.copy_((torch.randn(m, hidden, generator=g, device="cuda") - 1.0).to(torch.bfloat16))
         idx.copy_(torch.randint(-1, 4, (m,), generator=g, device="cuda", dtype=torch.int32))
     assert nv.lib().caifq_device_status() == 0
+
+
+def test_without_dependent_launches():
+    """Launches that wait for one another as a stream's do give the same numbers (the switch is read once a process)."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, CAIFQ_PDL="0")
+    tests = [os.path.join(here, "test_gpu_adapted_block.py") + "::" + name for name in
+             ("test_training_step_with_the_input_kept_in_8_bits", "test_serving_step_of_requests_with_adapters_of_their_own")]
+    done = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-p", "no:cacheprovider"] + tests, env=env, cwd=os.path.dirname(here),
+                          capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0, done.stdout[-2000:]

@@ -167,6 +167,33 @@ def test_rows_in_any_order_give_the_same_bits(m):
     assert torch.equal(nv.lora_bank_linear_fwd(w, bank, idx, x), y)
 
 
+@pytest.mark.parametrize("m", [127, 128, 129, 5000])
+@pytest.mark.parametrize("count", [1, 4096, 4097])
+def test_many_adapters_and_the_ends_of_the_forms(m, count):
+    """Every row's adapter its own where there are so many; scratch full of NaN is not read before it is written."""
+    in_dim, out_dim, r = 64, 72, 8
+    g = torch.Generator(device="cuda").manual_seed(count + m)
+    a = (torch.randn(count, r, in_dim, generator=g, device="cuda") / 8).bfloat16()
+    b = (torch.randn(count, out_dim, r, generator=g, device="cuda") * 0.05).bfloat16()
+    bank = nv.LoraBank([nv.Lora(a[i], b[i], 16.0) for i in range(count)])
+    w = zero_weight(in_dim, out_dim)
+    x = torch.randn(m, in_dim, generator=g, device="cuda").bfloat16()
+    idx = torch.randint(-1, count + 1, (m,), generator=g, device="cuda", dtype=torch.int32)
+    idx[0], idx[-1] = count - 1, 2 ** 31 - 1
+    ws = torch.full((nv.lora_bank_workspace_bytes(w, bank, m),), 255, dtype=torch.uint8, device="cuda")
+    y = nv.lora_bank_linear_fwd(w, bank, idx, x, workspace=ws)
+    mine = (idx >= 0) & (idx < count)
+    at = idx.clamp(0, count - 1).long()
+    xd = x.double()
+    h = torch.einsum("mi,mri->mr", xd, a[at].double())
+    eh = (in_dim / 32 + 64) * S * torch.einsum("mi,mri->mr", xd.abs(), a[at].double().abs())
+    want = 2.0 * torch.einsum("mr,mor->mo", h, b[at].double()) * mine[:, None]
+    tol = 2.0 * torch.einsum("mr,mor->mo", eh + (2.0 ** -16 + (r / 32 + 70) * S) * h.abs(), b[at].double().abs())
+    tol = tol + 2 * half(torch.bfloat16) * (want.abs() + tol)
+    assert bool(((y.double() - want).abs() <= tol).all())
+    assert not bool(y[~mine].any())
+
+
 def test_operands_off_a_16_byte_boundary():
     in_dim, out_dim, m = 256, 128, 20
     bank = make_bank(7, in_dim, out_dim, [16, 8], torch.bfloat16)
