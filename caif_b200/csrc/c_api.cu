@@ -1258,12 +1258,20 @@ struct PackedBwdWs
 // launch alone takes 17 and 26.
 constexpr int64_t kActNtLeast = 2048;
 
+// whether the weight may be expanded once for the call: as expand_ok, from 32 rows on (whole pass, rank 16, 32 to 127 rows: 4096 -> 14336 int4
+// 100 us against 142 with the codes converted in the product, 4096 -> 4096 40 and 49, 1024 -> 1024 20.5 and 23.9, 1024 -> 14336 int8 69
+// and 110; where expansion_pays says no, 14336 -> 4096, 71 and 58)
+bool packed_expand_ok(const caifq_weight *w, const caifq_lora *l, const void *act, int64_t m, int compute_dtype)
+{
+  return (w->storage != CAIFQ_I4 || compute_dtype == CAIFQ_BF16) && fused_lora_ok(w, l, act, m, compute_dtype);
+}
+
 PackedBwdWs packed_bwd_ws(const caifq_weight *w, const caifq_lora *l, int64_t m, int compute_dtype)
 {
   PackedBwdWs o{};
   o.lora = lora_bwd_ws(w, l, m);
   o.weight = o.lora.total;
-  o.sums = o.weight + (expand_ok(w, l, kAlignedProbe, m, compute_dtype) ? expanded_weight_bytes(w) : 0);
+  o.sums = o.weight + (packed_expand_ok(w, l, kAlignedProbe, m, compute_dtype) ? expanded_weight_bytes(w) : 0);
   o.total = o.sums + align256(act_gradients_scratch_bytes(m, w->out_dim, w->in_dim, l->rank));
   return o;
 }
@@ -1313,7 +1321,7 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
   float *sums = reinterpret_cast<float *>(base + ws.sums);
   if (fused_lora_ok(w, lora, dy, m, compute_dtype) && aligned_to(dx, 16))
   {
-    const bool expand = expand_ok(w, lora, dy, m, compute_dtype) && expansion_pays(w, true, m);
+    const bool expand = packed_expand_ok(w, lora, dy, m, compute_dtype) && expansion_pays(w, true, m);
     void *wb = base + ws.weight;
     // transposed B, padded A and, where the call expands, the weight in one launch; dH = dy . B, and its padded copy times
     // alpha / rank for the product's extra k-block

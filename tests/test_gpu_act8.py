@@ -222,6 +222,23 @@ def test_backward_on_packed_rows_of_any_width(dtype, compute, in_dim, out_dim, m
     check_grads(*case, nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], compute), compute)
 
 
+@pytest.mark.parametrize("m", [32, 100, 127, 128, 300])
+def test_backward_rounds_an_expanded_int4_weight_once(m):
+    """Rows of one 1 pick rows of the weight: code times scale as bf16."""
+    in_dim, out_dim = 1024, 2048
+    weight, _, _ = make_weight(np.random.default_rng(m), out_dim, in_dim, orc.I4)
+    zero = nv.Lora(torch.zeros(16, in_dim, dtype=torch.bfloat16, device="cuda"),
+                   torch.zeros(out_dim, 16, dtype=torch.bfloat16, device="cuda"), 16.0)
+    g = torch.Generator(device="cuda").manual_seed(m)
+    pick = torch.randint(0, out_dim, (m,), generator=g, device="cuda")
+    dy = torch.zeros(m, out_dim, dtype=torch.bfloat16, device="cuda")
+    dy[torch.arange(m, device="cuda"), pick] = 1.0
+    x = nv.act_pack(torch.randn(m, in_dim, generator=g, device="cuda").bfloat16())
+    hidden = torch.zeros(m, 16, dtype=torch.bfloat16, device="cuda")
+    dx, _, _ = nv.lora_linear_bwd_packed(weight, zero, dy, x, hidden, nv.BF16)
+    assert torch.equal(dx, nv.weight_materialize(weight).float()[pick].bfloat16())
+
+
 def test_backward_beside_the_one_on_full_rows():
     """On rows that eight bits hold, lora_linear_bwd gives the same gradients: dx bit for bit where alpha / rank is a power of
     two, dA and dB to the rounding of sums in another order."""
