@@ -235,7 +235,8 @@ Force forced_path()
 
 int linear_any(const caifq_weight *w, bool backward, const void *a, int a_dtype, float a_prescale, int64_t m,
                void *c, int c_dtype, bool accumulate, int compute_dtype, cudaStream_t s, const char *who,
-               const void *lora_lhs = nullptr, const void *lora_rhs = nullptr, const float *c_scale = nullptr)
+               const void *lora_lhs = nullptr, const void *lora_rhs = nullptr, const float *c_scale = nullptr,
+               bool whole_scales = false)
 {
   const int rc = check_weight(w, who);
   if (rc != CAIFQ_OK)
@@ -260,6 +261,7 @@ int linear_any(const caifq_weight *w, bool backward, const void *a, int a_dtype,
   args.c = c;
   args.c_dtype = c_dtype;
   args.accumulate = accumulate;
+  args.whole_scales = whole_scales;
   args.compute_dtype = compute_dtype;
   args.lora_lhs = lora_lhs;
   args.lora_rhs = lora_rhs;
@@ -612,7 +614,8 @@ int caifq_linear_fwd(const caifq_weight *w, const void *x, int32_t x_dtype, int6
 }  // extern "C"
 
 static int linear_ws(const caifq_weight *w, bool backward, const void *a, int a_dtype, int64_t m, void *c, int c_dtype,
-                     int compute_dtype, void *workspace, size_t workspace_bytes, cudaStream_t s, const char *who)
+                     int compute_dtype, void *workspace, size_t workspace_bytes, cudaStream_t s, const char *who,
+                     bool whole_scales = false)
 {
   const int rc = check_weight(w, who);
   if (rc != CAIFQ_OK)
@@ -623,7 +626,8 @@ static int linear_ws(const caifq_weight *w, bool backward, const void *a, int a_
       (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 ||
       !expand_linear_ok(w, backward, a, a_dtype, m, c, c_dtype, compute_dtype))
   {
-    return linear_any(w, backward, a, a_dtype, 1.0f, m, c, c_dtype, false, compute_dtype, s, who);
+    return linear_any(w, backward, a, a_dtype, 1.0f, m, c, c_dtype, false, compute_dtype, s, who, nullptr, nullptr, nullptr,
+                      whole_scales);
   }
   const int r = launch_expand_prepare(*w, workspace, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, 0, 0, s);
   if (r != CAIFQ_OK)
@@ -1213,7 +1217,7 @@ int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *ban
   int r = launch_lora_bank_down(*bank, adapter_of_row, x, frozen, m, y, workspace, s);
   if (r == CAIFQ_OK)
   {
-    r = linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who);
+    r = linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who, true);
   }
   if (r == CAIFQ_OK)
   {

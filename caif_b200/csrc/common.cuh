@@ -439,6 +439,8 @@ struct LinearArgs
   // launch and their outputs follow w's in the columns of c ([m, out + sum of their out_dims]).
   const caifq_weight *more;
   int num_more;
+  // int4 under bf16 compute on the streaming kernel: round code times scale to bf16 once, as an expanded weight is, and not the scale too
+  bool whole_scales;
 };
 
 constexpr int kMaxPeers = 8;

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 linear_stream_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ StreamParams p,
                      const __grid_constant__ StreamTable<N> table)
 {
-  constexpr bool IS_I4 = (WMODE == W_I4 || WMODE == W_I4S);
+  constexpr bool IS_I4 = (WMODE == W_I4 || WMODE == W_I4S || WMODE == W_I4X);
   constexpr int PLANES = planes_of(WMODE);
   constexpr int UNIT_STAGES = IS_I4 ? 2 : 1;          // stages of one team in a unit of codes
   constexpr uint32_t STAGE_CODES = IS_I4 ? 64u : 128u;   // bytes of a row per stage
@@ -800,6 +800,13 @@ linear_stream_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_con
                   {
                     int4x8_to_bf16_split(word, sc[2 * u + c], o4, l4);
                   }
+                  else if constexpr (WMODE == W_I4X)
+                  {
+                    const float s = sc[2 * u + c];
+                    const uint32_t top = pack_bf16x2(s, s);
+                    const float rest = s - __uint_as_float(top << 16);
+                    int4x8_to_bf16_once(word, top, pack_bf16x2(rest, rest), o4);
+                  }
                   else
                   {
                     int4x8_to_bf16(word, pack_bf16x2(sc[2 * u + c], sc[2 * u + c]), o4);
@@ -1050,6 +1057,13 @@ int launch_stream(int mode, const CUtensorMap &map_b, StreamParams &p, const Str
     case W_I4:
       return p.halves ? launch_stream_inst<W_I4, N, true>(map_b, p, table, smem, dependent, s)
                       : launch_stream_inst<W_I4, N, false>(map_b, p, table, smem, dependent, s);
+    case W_I4X:
+      if constexpr (N == 1)
+      {
+        return p.halves ? launch_stream_inst<W_I4X, N, true>(map_b, p, table, smem, dependent, s)
+                        : launch_stream_inst<W_I4X, N, false>(map_b, p, table, smem, dependent, s);
+      }
+      [[fallthrough]];   // (the table's entries are never converted so)
     default:
       return launch_stream_inst<W_I4S, N, false>(map_b, p, table, smem, dependent, s);
   }
@@ -1126,7 +1140,7 @@ bool stream_supported(const LinearArgs &g)
 int launch_linear_stream(const LinearArgs &g, cudaStream_t s)
 {
   const caifq_weight &w = g.w;
-  const int mode = wmode_of(w, g.compute_dtype);
+  const int mode = g.whole_scales && wmode_of(w, g.compute_dtype) == W_I4 ? W_I4X : wmode_of(w, g.compute_dtype);
   const int m = static_cast<int>(g.m);
   StreamParams p = common_params(w, mode, g.c_dtype, g.accumulate, m, (reinterpret_cast<uintptr_t>(w.scales) & 15u) == 0, false);
   StreamTable<1> table{};

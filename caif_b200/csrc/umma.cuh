@@ -22,7 +22,9 @@ enum WMode
   W_BF16 = 2,
   // int4 for fp32 compute: scale * code (exact in fp32) goes to the tensor core as two bf16 terms,
   // hi = bf16(w) and lo = bf16(w - hi), in two operand planes; hi + lo equals w to 2^-17 relative
-  W_I4S = 3
+  W_I4S = 3,
+  // int4 codes times the whole fp16 scale, rounded to bf16 once (W_I4 rounds the scale to bf16 first); streaming kernel only
+  W_I4X = 4
 };
 
 __host__ __device__ constexpr int planes_of(int wmode) { return wmode == W_I4S ? 2 : 1; }
@@ -348,6 +350,35 @@ __device__ __forceinline__ void int4x8_to_bf16(uint32_t w, uint32_t scale2, uint
       "mul.rn.bf16x2 %3, %3, %5;\n\t}"
       : "=&r"(out[0]), "=&r"(out[1]), "=&r"(out[2]), "=&r"(out[3])
       : "r"(w), "r"(scale2), "r"(0x43084308u));
+}
+
+// the same with a scale of two bf16 terms (whose sum an fp16 scale's eleven bits are), the product rounded once
+__device__ __forceinline__ void int4x8_to_bf16_once(uint32_t w, uint32_t scale2, uint32_t rest2, uint32_t (&out)[4])
+{
+  asm("{\n\t.reg .b32 e, d, t, v;\n\t"
+      "lop3.b32 e, %4, 0x0F0F0F0F, 0x08080808, 0x6A;\n\t"
+      "shr.u32 d, %4, 4;\n\t"
+      "lop3.b32 d, d, 0x0F0F0F0F, 0x08080808, 0x6A;\n\t"
+      "prmt.b32 t, e, d, 0x5140;\n\t"
+      "prmt.b32 v, e, d, 0x7362;\n\t"
+      "prmt.b32 %0, t, 0x43434343, 0x4140;\n\t"
+      "prmt.b32 %1, t, 0x43434343, 0x4342;\n\t"
+      "prmt.b32 %2, v, 0x43434343, 0x4140;\n\t"
+      "prmt.b32 %3, v, 0x43434343, 0x4342;\n\t"
+      "sub.rn.bf16x2 %0, %0, %7;\n\t"
+      "sub.rn.bf16x2 %1, %1, %7;\n\t"
+      "sub.rn.bf16x2 %2, %2, %7;\n\t"
+      "sub.rn.bf16x2 %3, %3, %7;\n\t"
+      "mul.rn.bf16x2 e, %0, %6;\n\t"
+      "mul.rn.bf16x2 d, %1, %6;\n\t"
+      "mul.rn.bf16x2 t, %2, %6;\n\t"
+      "mul.rn.bf16x2 v, %3, %6;\n\t"
+      "fma.rn.bf16x2 %0, %0, %5, e;\n\t"
+      "fma.rn.bf16x2 %1, %1, %5, d;\n\t"
+      "fma.rn.bf16x2 %2, %2, %5, t;\n\t"
+      "fma.rn.bf16x2 %3, %3, %5, v;\n\t}"
+      : "=&r"(out[0]), "=&r"(out[1]), "=&r"(out[2]), "=&r"(out[3])
+      : "r"(w), "r"(scale2), "r"(rest2), "r"(0x43084308u));
 }
 
 // the same eight codes as two bf16 terms of scale * code: hi = bf16(w), lo = bf16(w - hi)

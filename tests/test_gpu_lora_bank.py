@@ -121,6 +121,20 @@ def test_beside_a_frozen_weight(storage, compute, m):
     assert bool(((y.double() - (base + part)).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("m", [1, 16, 17, 48, 128, 129, 500, 768, 1500])
+def test_int4_weight_is_rounded_once(m):
+    """Rows of one 1 pick columns of the weight: code times scale as bf16, with no rounding of the scale before that."""
+    in_dim, out_dim = 256, 640
+    weight, _, _ = make_weight(np.random.default_rng(m), out_dim, in_dim, orc.I4)
+    bank = make_bank(m, in_dim, out_dim, [16, 8], torch.bfloat16)
+    pick = torch.randint(0, in_dim, (m,), generator=torch.Generator(device="cuda").manual_seed(m), device="cuda")
+    x = torch.zeros(m, in_dim, dtype=torch.bfloat16, device="cuda")
+    x[torch.arange(m, device="cuda"), pick] = 1.0
+    none = torch.full((m,), -1, dtype=torch.int32, device="cuda")
+    y = nv.lora_bank_linear_fwd(weight, bank, none, x, nv.BF16)
+    assert torch.equal(y, nv.weight_materialize(weight).float().t()[pick].bfloat16())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_beside_a_frozen_weight_other_types(dtype):
     in_dim, out_dim, m = 256, 384, 30
