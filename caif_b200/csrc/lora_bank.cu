@@ -206,14 +206,15 @@ bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_en
       id[i] = row < m ? group_of(adapter_of_row, row, count) : -1;
     }
   };
+  // (a call of one trip keeps its rows' places)
+  int kept[4], kept_at[4];
   for (int64_t base = 0; base < m; base += 4096)
   {
-    int id[4];
-    groups(id, base);
+    groups(kept, base);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-      place(id[i]);
+      kept_at[i] = place(kept[i]);
     }
   }
   __syncthreads();
@@ -269,6 +270,21 @@ bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_en
     plan.entry[i].rank = -1;
   }
   __syncthreads();
+  auto deal = [&](const int (&id)[4], const int (&at)[4], int64_t base) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+      if (id[i] >= 0)
+      {
+        plan.rows[static_cast<int64_t>(first[id[i]]) * kTileRows + at[i]] = static_cast<int32_t>(base + i * 1024 + threadIdx.x);
+      }
+    }
+  };
+  if (m <= 4096)
+  {
+    deal(kept, kept_at, 0);
+    return;
+  }
   for (int i = threadIdx.x; i <= count; i += 1024)
   {
     rows_of[i] = 0;
@@ -276,17 +292,13 @@ bank_plan_kernel(const int32_t *__restrict__ adapter_of_row, const caifq_lora_en
   __syncthreads();
   for (int64_t base = 0; base < m; base += 4096)
   {
-    int id[4];
-    groups(id, base);
+    groups(kept, base);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
     {
-      const int at = place(id[i]);
-      if (id[i] >= 0)
-      {
-        plan.rows[static_cast<int64_t>(first[id[i]]) * kTileRows + at] = static_cast<int32_t>(base + i * 1024 + threadIdx.x);
-      }
+      kept_at[i] = place(kept[i]);
     }
+    deal(kept, kept_at, base);
   }
 }
 
