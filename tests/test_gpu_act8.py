@@ -222,6 +222,19 @@ def test_backward_on_packed_rows_of_any_width(dtype, compute, in_dim, out_dim, m
     check_grads(*case, nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], compute), compute)
 
 
+@pytest.mark.parametrize("storage,compute", [(orc.I8, nv.F32), (orc.I4, nv.BF16)])
+@pytest.mark.parametrize("in_dim,out_dim,m,rank", [(256, 1024, 1024, 16), (128, 1152, 1100, 8), (384, 1280, 2049, 32), (128, 2048, 2048, 8),
+                                                   (256, 1024, 4097, 32), (128, 1024, 4095, 16), (128, 1408, 8300, 16), (256, 896, 3000, 16),
+                                                   (256, 1024, 2500, 64)])
+def test_backward_of_many_rows(storage, compute, in_dim, out_dim, m, rank):
+    case = make_case(m + rank, storage, torch.bfloat16, in_dim, out_dim, m, rank)
+    ws = torch.full((nv.lora_bwd_packed_workspace_bytes(case[0], case[1], m, compute),), 255, dtype=torch.uint8, device="cuda")
+    got = nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], compute, workspace=ws)
+    check_grads(*case, got, compute)
+    for a, b in zip(nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], compute), got):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("m", [32, 100, 127, 128, 300])
 def test_backward_rounds_an_expanded_int4_weight_once(m):
     """Rows of one 1 pick rows of the weight: code times scale as bf16."""
