@@ -375,50 +375,17 @@ __device__ __forceinline__ bool small_tile(const int32_t *adapter_of_row, const 
 // h of a tile.  As in the adapter's own thin product, a lane streams 16 bytes of two rows of x and of a row of A per 32 columns
 // straight into fragments (the order of the columns inside a fragment is the same for both); the eight warps split the columns,
 // and so do the blocks of a cluster where there are few tiles.
-template <int NT, bool SMALL>   // eights of the largest rank
-__global__ void __launch_bounds__(256)
-bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter_of_row,
-                     const caifq_lora_entry *__restrict__ entries, int count, const BankPlan plan, int ld, int64_t m, int in_dim,
-                     int cluster)
+//
+// h_part: the sums of this block's share of the columns, for the rows of a tile, in `part[0]`
+template <int NT>   // eights of the largest rank
+__device__ __forceinline__ void h_part(const __nv_bfloat16 *x, const int (&rows)[kTileRows], const caifq_lora_entry &entry, int in_dim,
+                                       int cluster, int rank_in_cluster, float (&part)[8][kTileRows][NT * 8 + 1])
 {
-  __shared__ float part[8][kTileRows][NT * 8 + 1];
-  __shared__ int rows[kTileRows];
-  __shared__ caifq_lora_entry entry;
-  // (what invariant loads read is addressed out of the wait, so that they stay behind it.  The wait comes before the next launch is
-  // let in: `up` relies on it)
-  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2;
   const int t = lane & 3;
-  const int rank_in_cluster = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int64_t tile = blockIdx.x / cluster;
-  if constexpr (SMALL)
-  {
-    // (every block of a cluster finds the same)
-    if (!small_tile(adapter_of_row, entries, count, static_cast<int>(m), static_cast<int>(tile), rows, entry))
-    {
-      return;
-    }
-  }
-  else
-  {
-    if (threadIdx.x < kTileRows)
-    {
-      rows[threadIdx.x] = plan.rows[tile * kTileRows + threadIdx.x];
-    }
-    if (threadIdx.x == 0)
-    {
-      entry = plan.entry[tile];
-    }
-    __syncthreads();
-  }
   const int eights = entry.rank / 8;
-  if (eights <= 0)
-  {
-    return;
-  }
   const int steps = in_dim / 32;
   const int begin = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp) / (8 * cluster));
   const int end = static_cast<int>(static_cast<int64_t>(steps) * (rank_in_cluster * 8 + warp + 1) / (8 * cluster));
@@ -496,6 +463,49 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
     }
     part[0][e / (NT * 8)][e % (NT * 8)] = v;
   }
+}
+
+template <int NT, bool SMALL>
+__global__ void __launch_bounds__(256)
+bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter_of_row,
+                     const caifq_lora_entry *__restrict__ entries, int count, const BankPlan plan, int ld, int64_t m, int in_dim,
+                     int cluster)
+{
+  __shared__ float part[8][kTileRows][NT * 8 + 1];
+  __shared__ int rows[kTileRows];
+  __shared__ caifq_lora_entry entry;
+  // (what invariant loads read is addressed out of the wait, so that they stay behind it.  The wait comes before the next launch is
+  // let in: `up` relies on it)
+  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int rank_in_cluster = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int64_t tile = blockIdx.x / cluster;
+  if constexpr (SMALL)
+  {
+    // (every block of a cluster finds the same)
+    if (!small_tile(adapter_of_row, entries, count, static_cast<int>(m), static_cast<int>(tile), rows, entry))
+    {
+      return;
+    }
+  }
+  else
+  {
+    if (threadIdx.x < kTileRows)
+    {
+      rows[threadIdx.x] = plan.rows[tile * kTileRows + threadIdx.x];
+    }
+    if (threadIdx.x == 0)
+    {
+      entry = plan.entry[tile];
+    }
+    __syncthreads();
+  }
+  const int eights = entry.rank / 8;
+  if (eights <= 0)
+  {
+    return;
+  }
+  h_part<NT>(x, rows, entry, in_dim, cluster, rank_in_cluster, part);
   if (cluster > 1)
   {
     cluster_sync_all();
@@ -532,13 +542,119 @@ bank_down_mma_kernel(const __nv_bfloat16 *x, const int32_t *__restrict__ adapter
   }
 }
 
-// y of a tile's rows and 128 * GROUPS columns: a warp GROUPS times 32.  h enters as two bf16 terms (2^-16 relative).  The columns
-// of a group of 32 are dealt out to its four 8-wide tiles so that a lane ends with eight neighbouring ones of a row.  Bound by
-// latency (tile, then operands, then results) at few rows and by the frozen product's 4 bytes and y's 2 at many.
+// ---- y of 32 columns of a tile: a warp's work ----
+// h enters as two bf16 terms (2^-16 relative).  The columns are dealt out to the four 8-wide tiles so that a lane ends with eight
+// neighbouring ones of a row.
+
+// h of rows g and g + 8 as fragments, four neighbouring ranks a lane per sixteen
+template <int KS>   // sixteens of the largest rank
+struct HTerms
+{
+  uint32_t top[KS][2][2], rest[KS][2][2];
+
+  __device__ __forceinline__ void take(int ks, int half, const float4 &v)
+  {
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+      const uint32_t high = pack_bf16x2(e[2 * i], e[2 * i + 1]);
+      // (an infinity has no second term)
+      const float r0 = isfinite(e[2 * i]) ? e[2 * i] - __uint_as_float(high << 16) : 0.0f;
+      const float r1 = isfinite(e[2 * i + 1]) ? e[2 * i + 1] - __uint_as_float(high & 0xFFFF0000u) : 0.0f;
+      top[ks][half][i] = high;
+      rest[ks][half][i] = pack_bf16x2(r0, r1);
+    }
+  }
+};
+
+// the adapter's rows of B for 32 columns, and the frozen product there
+template <int KS>
+struct UpColumns
+{
+  uint2 w[KS][4];
+  float4 f[2][2];
+
+  __device__ __forceinline__ void fetch_b(const __nv_bfloat16 *b, int rank, int col0, int out_dim)
+  {
+    const int lane = threadIdx.x & 31;
+    const int g = lane >> 2;
+    const int t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+    {
+      const int n = col0 + 8 * (g >> 1) + 2 * nt + (g & 1);   // the column whose row of B this lane feeds
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+      {
+        w[ks][nt] = make_uint2(0u, 0u);
+        if (16 * ks + 4 * t < rank && n < out_dim)
+        {
+          w[ks][nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n) * rank + 16 * ks + 4 * t));
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void fetch_frozen(const float *frozen, const int32_t (&row_of)[2], int col0, int out_dim)
+  {
+    const int c = col0 + 8 * static_cast<int>(threadIdx.x & 3);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      if (row_of[half] >= 0 && c < out_dim)
+      {
+        const float4 *src = reinterpret_cast<const float4 *>(frozen + static_cast<int64_t>(row_of[half]) * out_dim + c);
+        f[half][0] = src[0];
+        f[half][1] = src[1];
+      }
+    }
+  }
+
+  // (rank 0, rows without an adapter: the frozen product, whatever the other rows hold)
+  __device__ __forceinline__ void store(const HTerms<KS> &h, int rank, float scale, __nv_bfloat16 *y, const int32_t (&row_of)[2], int col0,
+                                        int out_dim) const
+  {
+    float c[4][4];
+#pragma unroll
+    for (int nt = 0; nt < 4; ++nt)
+    {
+      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
+      if (rank > 0)
+      {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+        {
+          mma_16816(c[nt], h.top[ks][0][0], h.top[ks][1][0], h.top[ks][0][1], h.top[ks][1][1], w[ks][nt].x, w[ks][nt].y);
+          mma_16816(c[nt], h.rest[ks][0][0], h.rest[ks][1][0], h.rest[ks][0][1], h.rest[ks][1][1], w[ks][nt].x, w[ks][nt].y);
+        }
+      }
+    }
+    const int at = col0 + 8 * static_cast<int>(threadIdx.x & 3);
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+    {
+      if (row_of[half] >= 0 && at < out_dim)
+      {
+        const float4 *q = f[half];
+        const int e = 2 * half;
+        uint4 o;
+        o.x = pack_bf16x2(fmaf(c[0][e], scale, q[0].x), fmaf(c[0][e + 1], scale, q[0].y));
+        o.y = pack_bf16x2(fmaf(c[1][e], scale, q[0].z), fmaf(c[1][e + 1], scale, q[0].w));
+        o.z = pack_bf16x2(fmaf(c[2][e], scale, q[1].x), fmaf(c[2][e + 1], scale, q[1].y));
+        o.w = pack_bf16x2(fmaf(c[3][e], scale, q[1].z), fmaf(c[3][e + 1], scale, q[1].w));
+        *reinterpret_cast<uint4 *>(y + static_cast<int64_t>(row_of[half]) * out_dim + at) = o;
+      }
+    }
+  }
+};
+
+// y of a tile's rows and 128 * GROUPS columns, a warp GROUPS times 32.  Bound by latency (tile, then operands, then results) at few rows
+// and by the frozen product's 4 bytes and y's 2 at many.
 //
 // A short call's block finds its rows and fetches its rows of B before it waits for the frozen product: what it reads for that was
 // complete before `down`, which waited for it, let the frozen product's launch in, and with it this one.
-template <int KS, int GROUPS, bool SMALL>   // KS: sixteens of the largest rank
+template <int KS, int GROUPS, bool SMALL>
 __global__ void __launch_bounds__(128)
 bank_up_mma_kernel(const float *frozen, const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries,
                    int count, int64_t m, const BankPlan plan, __nv_bfloat16 *y, int ld, int out_dim)
@@ -578,25 +694,11 @@ bank_up_mma_kernel(const float *frozen, const int32_t *__restrict__ adapter_of_r
   {
     return;
   }
-  const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entry.b);
-  uint2 w[GROUPS][KS][4];
+  UpColumns<KS> u[GROUPS];
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i)
   {
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt)
-    {
-      const int n = col0 + 32 * i + 8 * (g >> 1) + 2 * nt + (g & 1);   // the column whose row of B this lane feeds
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-      {
-        w[i][ks][nt] = make_uint2(0u, 0u);
-        if (16 * ks + 4 * t < rank && n < out_dim)
-        {
-          w[i][ks][nt] = __ldg(reinterpret_cast<const uint2 *>(b + static_cast<int64_t>(n) * rank + 16 * ks + 4 * t));
-        }
-      }
-    }
+    u[i].fetch_b(static_cast<const __nv_bfloat16 *>(entry.b), rank, col0 + 32 * i, out_dim);
   }
   if constexpr (SMALL)
   {
@@ -617,75 +719,140 @@ bank_up_mma_kernel(const float *frozen, const int32_t *__restrict__ adapter_of_r
       }
     }
   }
-  float4 f[GROUPS][2][2];
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i)
   {
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-    {
-      if (row_of[half] >= 0 && col0 + 32 * i + 8 * t < out_dim)
-      {
-        const float4 *src =
-            reinterpret_cast<const float4 *>(frozen + static_cast<int64_t>(row_of[half]) * out_dim + col0 + 32 * i + 8 * t);
-        f[i][half][0] = src[0];
-        f[i][half][1] = src[1];
-      }
-    }
+    u[i].fetch_frozen(frozen, row_of, col0 + 32 * i, out_dim);
   }
-  uint32_t top[KS][2][2], rest[KS][2][2];
+  HTerms<KS> h;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
   {
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-    {
-      const float e[4] = {v[ks][half].x, v[ks][half].y, v[ks][half].z, v[ks][half].w};
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-      {
-        const uint32_t high = pack_bf16x2(e[2 * i], e[2 * i + 1]);
-        // (an infinity has no second term)
-        const float r0 = isfinite(e[2 * i]) ? e[2 * i] - __uint_as_float(high << 16) : 0.0f;
-        const float r1 = isfinite(e[2 * i + 1]) ? e[2 * i + 1] - __uint_as_float(high & 0xFFFF0000u) : 0.0f;
-        top[ks][half][i] = high;
-        rest[ks][half][i] = pack_bf16x2(r0, r1);
-      }
-    }
+    h.take(ks, 0, v[ks][0]);
+    h.take(ks, 1, v[ks][1]);
   }
 #pragma unroll
   for (int i = 0; i < GROUPS; ++i)
   {
-    float c[4][4];
-#pragma unroll
-    for (int nt = 0; nt < 4; ++nt)
+    u[i].store(h, rank, entry.scale, y, row_of, col0 + 32 * i, out_dim);
+  }
+}
+
+// Short calls with few columns to add to: both steps after the frozen product in one launch.  A cluster of a tile takes x . A^T, its
+// blocks a share of the columns each; they give their sums to one another, and take a share of the columns of y.  Another launch
+// less: 1024 -> 1024, one row 9.1 -> 7.7 us, 128 rows of 16 adapters 15.6 -> 13.9; 14336 -> 4096, 16 rows of 4 34.7 -> 30.3.  Many
+// tiles of many columns want `up`'s small blocks, and B before the frozen product ends: 4096 -> 14336, 16 rows of 12, 25.7 and 27.2 so.
+template <int NT>   // eights of the largest rank
+__global__ void __launch_bounds__(256, 2)
+bank_few_mma_kernel(const __nv_bfloat16 *x, const float *frozen, const int32_t *__restrict__ adapter_of_row,
+                    const caifq_lora_entry *__restrict__ entries, int count, __nv_bfloat16 *y, int m, int in_dim, int out_dim, int cluster)
+{
+  constexpr int KS = (NT + 1) / 2;
+  __shared__ float part[8][kTileRows][NT * 8 + 1];
+  __shared__ __align__(16) float h_sum[kTileRows][KS * 16 + 4];
+  __shared__ int rows[kTileRows];
+  __shared__ caifq_lora_entry entry;
+  asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries), "+l"(x)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2;
+  const int t = lane & 3;
+  const int rank_in_cluster = cluster > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int tile = static_cast<int>(blockIdx.x) / cluster;
+  // (every block of a cluster finds the same)
+  if (!small_tile(adapter_of_row, entries, count, m, tile, rows, entry))
+  {
+    return;
+  }
+  const int rank = entry.rank;
+  const int32_t row_of[2] = {rows[g], rows[g + 8]};
+  const __nv_bfloat16 *b = static_cast<const __nv_bfloat16 *>(entry.b);
+  const int groups = (out_dim + 31) / 32;   // of columns, a warp's work
+  const int shares = cluster * static_cast<int>(gridDim.y);
+  const int share = static_cast<int>(blockIdx.y) * cluster + rank_in_cluster;
+  const int first = static_cast<int>(static_cast<int64_t>(groups) * share / shares);
+  const int last = static_cast<int>(static_cast<int64_t>(groups) * (share + 1) / shares);
+  UpColumns<KS> u;
+  HTerms<KS> h{};
+  int group = first + warp;
+  if (group < last)
+  {
+    u.fetch_b(b, rank, group * 32, out_dim);
+    u.fetch_frozen(frozen, row_of, group * 32, out_dim);
+  }
+  if (rank > 0)
+  {
+    h_part<NT>(x, rows, entry, in_dim, cluster, rank_in_cluster, part);
+    if (cluster > 1)
     {
-      c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
-      if (rank > 0)   // (rows without an adapter: zeros, whatever the other rows hold)
+      cluster_sync_all();
+    }
+    else
+    {
+      __syncthreads();
+    }
+    for (int e = threadIdx.x; e < kTileRows * KS * 16; e += 256)
+    {
+      const int rr = e / (KS * 16);
+      const int col = e % (KS * 16);
+      float v = 0.0f;
+      if (col < rank)
       {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+        v = part[0][rr][col];
+        if (cluster > 1)
         {
-          mma_16816(c[nt], top[ks][0][0], top[ks][1][0], top[ks][0][1], top[ks][1][1], w[i][ks][nt].x, w[i][ks][nt].y);
-          mma_16816(c[nt], rest[ks][0][0], rest[ks][1][0], rest[ks][0][1], rest[ks][1][1], w[i][ks][nt].x, w[i][ks][nt].y);
+          const uint32_t mine = smem_u32(&part[0][rr][col]);
+          float from[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)   // (all on their way before the first is added)
+          {
+            from[k] = k < cluster ? __uint_as_float(ld_shared_cluster(map_to_cta(mine, static_cast<uint32_t>(k)))) : 0.0f;
+          }
+          v = ((from[0] + from[1]) + (from[2] + from[3])) + ((from[4] + from[5]) + (from[6] + from[7]));
         }
       }
+      h_sum[rr][col] = v;
+    }
+    if (cluster > 1)
+    {
+      cluster_sync_all();   // nobody's sums are left while they are read
+    }
+    else
+    {
+      __syncthreads();
     }
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int ks = 0; ks < KS; ++ks)
     {
-      if (row_of[half] >= 0 && col0 + 32 * i + 8 * t < out_dim)
+      h.take(ks, 0, *reinterpret_cast<const float4 *>(&h_sum[g][16 * ks + 4 * t]));
+      h.take(ks, 1, *reinterpret_cast<const float4 *>(&h_sum[g + 8][16 * ks + 4 * t]));
+    }
+  }
+  while (group < last)
+  {
+    const int next = group + 8;
+    if constexpr (KS <= 2)   // (of rank 64 two groups do not fit the registers of two blocks an SM)
+    {
+      UpColumns<KS> ahead;
+      if (next < last)
       {
-        const float4 *q = f[i][half];
-        const int e = 2 * half;
-        uint4 o;
-        o.x = pack_bf16x2(fmaf(c[0][e], entry.scale, q[0].x), fmaf(c[0][e + 1], entry.scale, q[0].y));
-        o.y = pack_bf16x2(fmaf(c[1][e], entry.scale, q[0].z), fmaf(c[1][e + 1], entry.scale, q[0].w));
-        o.z = pack_bf16x2(fmaf(c[2][e], entry.scale, q[1].x), fmaf(c[2][e + 1], entry.scale, q[1].y));
-        o.w = pack_bf16x2(fmaf(c[3][e], entry.scale, q[1].z), fmaf(c[3][e + 1], entry.scale, q[1].w));
-        *reinterpret_cast<uint4 *>(y + static_cast<int64_t>(row_of[half]) * out_dim + col0 + 32 * i + 8 * t) = o;
+        ahead.fetch_b(b, rank, next * 32, out_dim);
+        ahead.fetch_frozen(frozen, row_of, next * 32, out_dim);
+      }
+      u.store(h, rank, entry.scale, y, row_of, group * 32, out_dim);
+      u = ahead;
+    }
+    else
+    {
+      u.store(h, rank, entry.scale, y, row_of, group * 32, out_dim);
+      if (next < last)
+      {
+        u.fetch_b(b, rank, next * 32, out_dim);
+        u.fetch_frozen(frozen, row_of, next * 32, out_dim);
       }
     }
+    group = next;
   }
 }
 
@@ -715,8 +882,7 @@ int down_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const v
                                       adapter_of_row, bank.entries, bank.count, plan, m, static_cast<int>(tiles)));
   }
   // clusters that split the columns where the tiles leave SMs without work, with at least two steps of 32 columns for every warp.
-  // (4096 -> 14336 int4, 8 rows of 4 adapters: 17.8 us, 28.5 with one block a tile; 14336 -> 4096, 16 rows: 34.5 and 75.9; 4096 -> 4096, 48
-  // rows of 16: 19.3 and 21.3; the least gain, 1024 -> 1024, 128 rows of 16: 16.3 and 15.6)
+  // (4096 -> 14336 int4, 16 rows of 12 adapters: 10 us more with one block a tile; 4096 -> 4096, 48 rows of 16: 2 more)
   int cluster = 1;
   while (cluster < 8 && tiles * cluster < 2 * 148 && bank.in_dim / 32 >= 2 * cluster * 8 * 2)
   {
@@ -772,6 +938,33 @@ int up_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const flo
   return up_mma_inst<4, 1>(bank, adapter_of_row, m, plan, tiles, frozen, y, s);
 }
 
+// calls that bank_few_mma_kernel takes
+bool few(const caifq_lora_bank &bank, int64_t m)
+{
+  return m <= kSmallCall && most_tiles(m, bank.count) * bank.out_dim <= 24 * 4096;
+}
+
+int few_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m, void *y, cudaStream_t s)
+{
+  const int64_t tiles = most_tiles(m, bank.count);
+  int cluster = 1;   // (each block a share of the columns of both)
+  while (cluster < 8 && tiles * cluster < 2 * 148 && (bank.out_dim >= 256 * cluster || bank.in_dim >= 1024 * cluster))
+  {
+    cluster *= 2;
+  }
+  auto kernel = bank.max_rank <= 8
+                    ? bank_few_mma_kernel<1>
+                    : (bank.max_rank <= 16 ? bank_few_mma_kernel<2> : (bank.max_rank <= 32 ? bank_few_mma_kernel<4> : bank_few_mma_kernel<8>));
+  // several clusters of a tile where its columns are many, each with the whole x . A^T (4096 -> 14336, 8 rows of 4: 17.5 us, 21.2 with one)
+  int64_t parts = (bank.out_dim + 512 * cluster - 1) / (512 * cluster);
+  const int64_t room = 4 * 148 / (tiles * cluster);
+  parts = parts < room ? parts : (room < 1 ? 1 : room);
+  CAIFQ_CHECK_CUDA(launch_dependent_clusters(kernel, dim3(static_cast<unsigned>(tiles * cluster), static_cast<unsigned>(parts)), dim3(256), 0, s, cluster,
+                                             static_cast<const __nv_bfloat16 *>(x), frozen, adapter_of_row, bank.entries, bank.count,
+                                             static_cast<__nv_bfloat16 *>(y), static_cast<int>(m), bank.in_dim, bank.out_dim, cluster));
+  return CAIFQ_OK;
+}
+
 template <typename T>
 int down_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h, cudaStream_t s)
 {
@@ -821,7 +1014,7 @@ int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of
 {
   if (tiled(bank, x, y, frozen, m))
   {
-    return down_mma(bank, adapter_of_row, x, m, scratch, s);
+    return few(bank, m) ? CAIFQ_OK : down_mma(bank, adapter_of_row, x, m, scratch, s);
   }
   float *h = static_cast<float *>(scratch);
   switch (bank.dtype)
@@ -840,7 +1033,7 @@ int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_r
 {
   if (tiled(bank, x, y, frozen, m))
   {
-    return up_mma(bank, adapter_of_row, frozen, m, y, scratch, s);
+    return few(bank, m) ? few_mma(bank, adapter_of_row, x, frozen, m, y, s) : up_mma(bank, adapter_of_row, frozen, m, y, scratch, s);
   }
   const float *h = static_cast<const float *>(scratch);
   switch (bank.dtype)

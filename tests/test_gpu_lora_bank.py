@@ -82,6 +82,9 @@ DTYPES = [torch.bfloat16, torch.float32, torch.float16]
     (16, 256, 264, [16] * 5, "any"), (17, 512, 128, [8, 32, 16], "any"), (33, 4096, 136, [64, 24, 8, 40], "any"),
     (64, 1024, 1024, [16] * 70, "any"), (300, 256, 384, [16, 32], "runs"), (129, 160, 8, [8], "none"),
     (1000, 128, 256, [16, 8, 64, 32, 48], "runs"), (5, 14336, 128, [16, 16], "any"),
+    # few rows into many columns
+    (16, 512, 14336, [32] * 12, "any"), (100, 256, 2056, [16, 8, 64] * 30, "any"), (60, 1024, 8192, [64, 8] * 10, "any"),
+    (1, 64, 14336, [8], "one"), (128, 128, 4096, [16], "runs"), (128, 128, 4096, [16] * 16, "runs"),
     # general forms: ranks, widths and rows that no 16-byte piece fits
     (7, 100, 36, [5, 1, 17], "any"), (50, 33, 77, [3, 200], "any"), (2, 64, 64, [1024], "one"), (40, 130, 9, [16], "any"),
     (20, 1, 1, [1], "any"),
@@ -169,9 +172,9 @@ def test_bad_values_stay_with_their_rows(dtype):
     assert bool(torch.isnan(got[8]).all()) and bool(torch.isnan(got[7]).all())
 
 
-@pytest.mark.parametrize("m", [16, 50, 400])
-def test_rows_in_any_order_give_the_same_bits(m):
-    in_dim, out_dim = 1024, 384
+@pytest.mark.parametrize("m,out_dim", [(16, 384), (50, 384), (400, 384), (100, 8192), (16, 30720)])
+def test_rows_in_any_order_give_the_same_bits(m, out_dim):
+    in_dim = 1024
     bank = make_bank(6, in_dim, out_dim, [16, 32, 8, 16, 64], torch.bfloat16)
     x, idx = make_rows(6, m, in_dim, 5, torch.bfloat16)
     w = zero_weight(in_dim, out_dim)
