@@ -938,10 +938,13 @@ int up_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const flo
   return up_mma_inst<4, 1>(bank, adapter_of_row, m, plan, tiles, frozen, y, s);
 }
 
-// calls that bank_few_mma_kernel takes
+// calls that bank_few_mma_kernel takes: by the tiles' columns, and by the rank where it is above 16.  (4096 -> 4096 int4, 18 tiles: rank 8 18.8 us
+// and 20.0 with two launches around the product, 16 19.3 and 20.3, but 64 26.9 and 24.5; 64 tiles of rank 16 24.6 and 21.8; 4096 -> 8192, 9
+// tiles: 16.2 and 16.5, 16.7 and 16.6, 23.7 and 21.6)
 bool few(const caifq_lora_bank &bank, int64_t m)
 {
-  return m <= kSmallCall && most_tiles(m, bank.count) * bank.out_dim <= 24 * 4096;
+  const int64_t sixteens = (bank.max_rank + 15) / 16;
+  return m <= kSmallCall && most_tiles(m, bank.count) * bank.out_dim * sixteens <= 24 * 4096;
 }
 
 int few_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m, void *y, cudaStream_t s)
