@@ -400,7 +400,10 @@ struct Gradients
   const int8_t *x;         // [m, in]
   const uint8_t *scales;   // [m, ceil(in / 32)]
   float *part;
-  int dtype;               // of dy and h
+  void *d_b;               // with one slice: the results themselves, rounded here; else null
+  void *d_a;
+  float factor;
+  int dtype;               // of dy, h and the results
   int dh_dtype;
   int out, in, r;
 };
@@ -410,12 +413,10 @@ constexpr int kTnTile = 32;
 constexpr int kTnRows = 32;
 constexpr int kTnGeneralBlocks = 6;   // an SM
 
-__global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t m)
+__device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
 {
   __shared__ float su[kTnRows][kTnTile + 1];
   __shared__ float sv[kTnRows][kTnTile + 1];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x;
   const int tiles_b = (j.out + kTnTile - 1) / kTnTile;
   const bool is_a = static_cast<int>(blockIdx.x) >= tiles_b;
@@ -475,10 +476,28 @@ __global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t 
       const int rr = r0 + tq * 2 + b;
       if (col < wide && rr < j.r)
       {
-        part[static_cast<int64_t>(col) * j.r + rr] = c[a][b];
+        if (j.d_b == nullptr)
+        {
+          part[static_cast<int64_t>(col) * j.r + rr] = c[a][b];
+        }
+        else if (is_a)
+        {
+          store_from_float(j.d_a, static_cast<int64_t>(rr) * j.in + col, j.dtype, c[a][b] * j.factor);
+        }
+        else
+        {
+          store_from_float(j.d_b, static_cast<int64_t>(col) * j.r + rr, j.dtype, c[a][b] * j.factor);
+        }
       }
     }
   }
+}
+
+__global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t m)
+{
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  tn_general(j, m);
 }
 
 // bf16, ranks 8, 16, 32, 64, widths of whole 128-column tiles: the tensor core, as the adapter's reductions on full rows run it (both
@@ -657,7 +676,24 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
     for (int half = 0; half < 2; ++half)
     {
       const int64_t col = c0 + warp * 16 + g + 8 * half;
-      *reinterpret_cast<float2 *>(part + col * R + nt * 8 + 2 * t) = make_float2(c[nt][2 * half], c[nt][2 * half + 1]);
+      const int rr = nt * 8 + 2 * t;
+      const float lo = c[nt][2 * half], hi = c[nt][2 * half + 1];
+      if (j.d_b == nullptr)
+      {
+        *reinterpret_cast<float2 *>(part + col * R + rr) = make_float2(lo, hi);
+      }
+      else if (is_a)
+      {
+        __nv_bfloat16 *d_a = static_cast<__nv_bfloat16 *>(j.d_a) + static_cast<int64_t>(rr) * j.in + col;
+        d_a[0] = __float2bfloat16(lo * j.factor);
+        d_a[j.in] = __float2bfloat16(hi * j.factor);
+      }
+      else
+      {
+        __nv_bfloat16 *d_b = static_cast<__nv_bfloat16 *>(j.d_b) + col * R + rr;
+        d_b[0] = __float2bfloat16(lo * j.factor);
+        d_b[1] = __float2bfloat16(hi * j.factor);
+      }
     }
   }
 }
@@ -987,12 +1023,44 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
   }
 }
 
-// The sums (the first blocks) and dx[m, in] = factor * dH . A, a thread a column, which needs none of them, in one launch
+// dx[m, in] = factor * dH . A, a thread a column; `block` of a row's 256 columns
+template <typename T>
+__device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, float factor, int in, int r, int64_t block)
+{
+  __shared__ float row[256];
+  const int parts = (in + 255) / 256;   // blocks of a row
+  const int64_t at = block / parts;
+  const int c = static_cast<int>(block % parts) * 256 + static_cast<int>(threadIdx.x);
+  float s = 0.0f;
+  for (int j0 = 0; j0 < r; j0 += 256)
+  {
+    __syncthreads();
+    if (j0 + static_cast<int>(threadIdx.x) < r)
+    {
+      row[threadIdx.x] = dh[at * r + j0 + threadIdx.x];
+    }
+    __syncthreads();
+    const int n = r - j0 < 256 ? r - j0 : 256;
+    if (c < in)
+    {
+#pragma unroll 8
+      for (int k = 0; k < n; ++k)
+      {
+        s = fmaf(row[k], act_f<T>(a[static_cast<int64_t>(j0 + k) * in + c]), s);
+      }
+    }
+  }
+  if (c < in)
+  {
+    dx[at * in + c] = act_t<T>(s * factor);
+  }
+}
+
+// The sums (the first blocks), and dx, which needs none of them, in one launch
 template <typename T>
 __global__ void __launch_bounds__(256)
 gradients_dx_kernel(const GradientSums j, int sum_blocks, const float *dh, const T *a, T *dx)
 {
-  __shared__ float row[256];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < sum_blocks)
@@ -1000,32 +1068,23 @@ gradients_dx_kernel(const GradientSums j, int sum_blocks, const float *dh, const
     gradient_sums(j, blockIdx.x);
     return;
   }
-  const int parts = (j.in + 255) / 256;   // blocks of a row
-  const int64_t block = static_cast<int64_t>(blockIdx.x) - sum_blocks;
-  const int64_t at = block / parts;
-  const int c = static_cast<int>(block % parts) * 256 + static_cast<int>(threadIdx.x);
-  float s = 0.0f;
-  for (int j0 = 0; j0 < j.r; j0 += 256)
+  dx_general<T>(dh, a, dx, j.factor, j.in, j.r, static_cast<int64_t>(blockIdx.x) - sum_blocks);
+}
+
+// Few tokens: the reductions, of one slice, and dx in one launch
+template <typename T>
+__global__ void __launch_bounds__(256)
+act_tn_dx_kernel(const Gradients j, int64_t m, int tiles, const T *a, T *dx)
+{
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (static_cast<int>(blockIdx.x) < tiles)
   {
-    __syncthreads();
-    if (j0 + static_cast<int>(threadIdx.x) < j.r)
-    {
-      row[threadIdx.x] = dh[at * j.r + j0 + threadIdx.x];
-    }
-    __syncthreads();
-    const int n = j.r - j0 < 256 ? j.r - j0 : 256;
-    if (c < j.in)
-    {
-#pragma unroll 8
-      for (int k = 0; k < n; ++k)
-      {
-        s = fmaf(row[k], act_f<T>(a[static_cast<int64_t>(j0 + k) * j.in + c]), s);
-      }
-    }
+    tn_general(j, m);
   }
-  if (c < j.in)
+  else if (blockIdx.y == 0)
   {
-    dx[at * j.in + c] = act_t<T>(s * j.factor);
+    dx_general<T>(static_cast<const float *>(j.dh), a, dx, j.factor, j.in, j.r, static_cast<int64_t>(blockIdx.x) - tiles);
   }
 }
 
@@ -1037,6 +1096,12 @@ int tn_slices(int64_t m, int64_t tiles, int tokens, int blocks)
   n = n > most ? most : n;
   return static_cast<int>(n < 1 ? 1 : n);
 }
+
+// So few tokens make one slice, whose sums are rounded where they are made, a launch less.  The whole pass, tensor core: 4096 -> 4096 int8,
+// 64 rows 37.6 -> 35.4 us, 128 rows 39.0 -> 37.3, 200 rows 38.9 and 39.4 so; multiply-adds, fp32: 2048 -> 2048, rank 64, 64 rows 45.2 -> 40.6,
+// 1024 -> 1024, rank 16, 64 rows 20.5 -> 20.0, 128 rows 28.8 and 32.1 so.
+constexpr int64_t kDirectMost = 128;
+constexpr int64_t kDirectMostGeneral = 64;
 
 int64_t general_tiles(int out, int in, int r)
 {
@@ -1090,6 +1155,18 @@ size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r)
 namespace
 {
 template <typename T>
+int launch_tn_dx(const Gradients &j, const void *a, void *dx, int64_t m, cudaStream_t s)
+{
+  const int tiles = (j.out + kTnTile - 1) / kTnTile + (j.in + kTnTile - 1) / kTnTile;
+  const int64_t blocks = tiles + m * ((j.in + 255) / 256);
+  CAIFQ_CHECK_ARG(blocks <= 0x7FFFFFFF, "LoRA backward on packed rows: %lld rows of %d columns are too many for its general form",
+                  static_cast<long long>(m), j.in);
+  CAIFQ_CHECK_CUDA(launch_dependent(act_tn_dx_kernel<T>, dim3(static_cast<unsigned>(blocks), (j.r + kTnTile - 1) / kTnTile), dim3(256), 0, s,
+                                    j, m, tiles, static_cast<const T *>(a), static_cast<T *>(dx)));
+  return CAIFQ_OK;
+}
+
+template <typename T>
 int launch_gradients_dx(const GradientSums &j, int64_t sum_blocks, const float *dh, const void *a, void *dx, int64_t m, cudaStream_t s)
 {
   const int64_t blocks = sum_blocks + m * ((j.in + 255) / 256);
@@ -1107,24 +1184,42 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
                          void *d_b, void *d_a, const void *a, void *dx, int dtype, float factor, float *scratch, int64_t m, int out,
                          int in, int r, cudaStream_t s)
 {
-  const Gradients j{dy, h, dh, x, scales, scratch, dtype, dh_dtype, out, in, r};
   auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
+  const bool tensor = dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
+                      (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(x);
+  const bool direct = m <= (tensor ? kDirectMost : kDirectMostGeneral);
+  const Gradients j{dy, h, dh, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, dtype, dh_dtype, out, in, r};
   int slices = 0;
-  if (dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
-      (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(x))
+  if (tensor)
   {
     const int tiles = (out + in) / kTnColumns;
-    slices = tn_slices(m, tiles, kTnTokens, r <= 16 ? kTnBlocks<2> : kTnBlocks<8>);
+    slices = direct ? 1 : tn_slices(m, tiles, kTnTokens, r <= 16 ? kTnBlocks<2> : kTnBlocks<8>);
     auto kernel = r == 8 ? act_tn_mma_kernel<1>
                          : (r == 16 ? act_tn_mma_kernel<2> : (r == 32 ? act_tn_mma_kernel<4> : act_tn_mma_kernel<8>));
     CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(slices)), dim3(256), 0, s, j, m));
   }
+  else if (direct && dx != nullptr)
+  {
+    switch (dtype)
+    {
+      case CAIFQ_F32:
+        return launch_tn_dx<float>(j, a, dx, m, s);
+      case CAIFQ_F16:
+        return launch_tn_dx<__half>(j, a, dx, m, s);
+      default:
+        return launch_tn_dx<__nv_bfloat16>(j, a, dx, m, s);
+    }
+  }
   else
   {
-    slices = tn_slices(m, general_tiles(out, in, r), kTnRows, kTnGeneralBlocks);
+    slices = direct ? 1 : tn_slices(m, general_tiles(out, in, r), kTnRows, kTnGeneralBlocks);
     const dim3 grid((out + kTnTile - 1) / kTnTile + (in + kTnTile - 1) / kTnTile, (r + kTnTile - 1) / kTnTile,
                     static_cast<unsigned>(slices));
     CAIFQ_CHECK_CUDA(launch_dependent(act_tn_kernel, grid, dim3(256), 0, s, j, m));
+  }
+  if (direct && dx == nullptr)
+  {
+    return CAIFQ_OK;
   }
   const int64_t n = (static_cast<int64_t>(out) + in) * r;
   const int64_t blocks = (n + 255) / 256;
