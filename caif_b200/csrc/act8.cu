@@ -408,71 +408,109 @@ struct Gradients
   int out, in, r;
 };
 
-// any type and width: 32 x 32 tiles of the result, fp32 multiply-adds
+// any type and width: 64 x 32 tiles of the result, fp32 multiply-adds, eight a thread for six values from shared memory.  The next
+// tokens' loads are issued before this trip's products.  (32 x 32 tiles with four for four: 500 rows, 2048 columns each way, rank 64, 37 us)
+constexpr int kTnWide = 64;
 constexpr int kTnTile = 32;
 constexpr int kTnRows = 32;
 constexpr int kTnGeneralBlocks = 6;   // an SM
 
+template <typename T, typename H>   // dy, h and the results; dH
 __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
 {
-  __shared__ float su[kTnRows][kTnTile + 1];
-  __shared__ float sv[kTnRows][kTnTile + 1];
+  constexpr int U = kTnRows * kTnWide / 256;
+  constexpr int V = kTnRows * kTnTile / 256;
+  __shared__ __align__(16) float su[kTnRows][kTnWide + 4];
+  __shared__ __align__(16) float sv[kTnRows][kTnTile + 2];
   const int tid = threadIdx.x;
-  const int tiles_b = (j.out + kTnTile - 1) / kTnTile;
+  const int tiles_b = (j.out + kTnWide - 1) / kTnWide;
   const bool is_a = static_cast<int>(blockIdx.x) >= tiles_b;
   const int wide = is_a ? j.in : j.out;   // the dimension that is not the rank
-  const int c0 = (static_cast<int>(blockIdx.x) - (is_a ? tiles_b : 0)) * kTnTile;
+  const int c0 = (static_cast<int>(blockIdx.x) - (is_a ? tiles_b : 0)) * kTnWide;
   const int r0 = blockIdx.y * kTnTile;
   const int64_t begin = m * blockIdx.z / gridDim.z;
   const int64_t end = m * (blockIdx.z + 1) / gridDim.z;
   const int blocks = (j.in + kActBlock - 1) / kActBlock;
   const int tq = tid % 16;
   const int tp = tid / 16;
-  float c[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+  float u[U], v[V];
+  auto fetch = [&](int64_t mb) {
+    const int col = c0 + tid % kTnWide;
+    const int64_t row0 = mb + tid / kTnWide;
+    if (is_a)
+    {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+      {
+        const int64_t row = row0 + i * (256 / kTnWide);
+        u[i] = row < end && col < wide ? static_cast<float>(j.x[row * wide + col]) * scale_of(j.scales[row * blocks + col / kActBlock]) : 0.0f;
+      }
+    }
+    else
+    {
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+      {
+        const int64_t row = row0 + i * (256 / kTnWide);
+        u[i] = row < end && col < wide ? act_f<T>(static_cast<const T *>(j.dy)[row * wide + col]) : 0.0f;
+      }
+    }
+    const int rr = r0 + tid % kTnTile;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      const int64_t row = mb + tid / kTnTile + i * (256 / kTnTile);
+      v[i] = 0.0f;
+      if (row < end && rr < j.r)
+      {
+        v[i] = is_a ? act_f<H>(static_cast<const H *>(j.dh)[row * j.r + rr]) : act_f<T>(static_cast<const T *>(j.h)[row * j.r + rr]);
+      }
+    }
+  };
+  float c[4][2] = {};
+  fetch(begin);
   for (int64_t mb = begin; mb < end; mb += kTnRows)
   {
-    for (int e = tid; e < kTnRows * kTnTile; e += 256)
+#pragma unroll
+    for (int i = 0; i < U; ++i)
     {
-      const int col = e % kTnTile;
-      const int64_t row = mb + e / kTnTile;
-      float u = 0.0f, v = 0.0f;
-      if (row < end && c0 + col < wide)
-      {
-        const int64_t at = row * wide + c0 + col;
-        u = is_a ? static_cast<float>(j.x[at]) * scale_of(j.scales[row * blocks + (c0 + col) / kActBlock])
-                 : load_as_float(j.dy, at, j.dtype);
-      }
-      if (row < end && r0 + col < j.r)
-      {
-        v = is_a ? load_as_float(j.dh, row * j.r + r0 + col, j.dh_dtype) : load_as_float(j.h, row * j.r + r0 + col, j.dtype);
-      }
-      su[e / kTnTile][col] = u;
-      sv[e / kTnTile][col] = v;
+      su[tid / kTnWide + i * (256 / kTnWide)][tid % kTnWide] = u[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+    {
+      sv[tid / kTnTile + i * (256 / kTnTile)][tid % kTnTile] = v[i];
     }
     __syncthreads();
-#pragma unroll
+    if (mb + kTnRows < end)
+    {
+      fetch(mb + kTnRows);
+    }
+#pragma unroll 8
     for (int r = 0; r < kTnRows; ++r)
     {
-      const float u0 = su[r][tp * 2];
-      const float u1 = su[r][tp * 2 + 1];
-      const float v0 = sv[r][tq * 2];
-      const float v1 = sv[r][tq * 2 + 1];
-      c[0][0] = fmaf(u0, v0, c[0][0]);
-      c[0][1] = fmaf(u0, v1, c[0][1]);
-      c[1][0] = fmaf(u1, v0, c[1][0]);
-      c[1][1] = fmaf(u1, v1, c[1][1]);
+      const float4 p = *reinterpret_cast<const float4 *>(&su[r][tp * 4]);
+      const float2 q = *reinterpret_cast<const float2 *>(&sv[r][tq * 2]);
+      c[0][0] = fmaf(p.x, q.x, c[0][0]);
+      c[0][1] = fmaf(p.x, q.y, c[0][1]);
+      c[1][0] = fmaf(p.y, q.x, c[1][0]);
+      c[1][1] = fmaf(p.y, q.y, c[1][1]);
+      c[2][0] = fmaf(p.z, q.x, c[2][0]);
+      c[2][1] = fmaf(p.z, q.y, c[2][1]);
+      c[3][0] = fmaf(p.w, q.x, c[3][0]);
+      c[3][1] = fmaf(p.w, q.y, c[3][1]);
     }
     __syncthreads();
   }
   float *part = j.part + static_cast<int64_t>(blockIdx.z) * (static_cast<int64_t>(j.out) + j.in) * j.r +
                 (is_a ? static_cast<int64_t>(j.out) * j.r : 0);
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int a = 0; a < 4; ++a)
   {
 #pragma unroll
     for (int b = 0; b < 2; ++b)
     {
-      const int col = c0 + tp * 2 + a;
+      const int col = c0 + tp * 4 + a;
       const int rr = r0 + tq * 2 + b;
       if (col < wide && rr < j.r)
       {
@@ -482,22 +520,23 @@ __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
         }
         else if (is_a)
         {
-          store_from_float(j.d_a, static_cast<int64_t>(rr) * j.in + col, j.dtype, c[a][b] * j.factor);
+          static_cast<T *>(j.d_a)[static_cast<int64_t>(rr) * j.in + col] = act_t<T>(c[a][b] * j.factor);
         }
         else
         {
-          store_from_float(j.d_b, static_cast<int64_t>(col) * j.r + rr, j.dtype, c[a][b] * j.factor);
+          static_cast<T *>(j.d_b)[static_cast<int64_t>(col) * j.r + rr] = act_t<T>(c[a][b] * j.factor);
         }
       }
     }
   }
 }
 
+template <typename T, typename H>
 __global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t m)
 {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  tn_general(j, m);
+  tn_general<T, H>(j, m);
 }
 
 // bf16, ranks 8, 16, 32, 64, widths of whole 128-column tiles: the tensor core, as the adapter's reductions on full rows run it (both
@@ -911,16 +950,15 @@ dh_row_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r)
   }
 }
 
-// The same where B is large: a cluster four rows, its blocks a share of the columns each; a number of B serves the four rows, and the
-// blocks' sums are added in order.
-constexpr int kDhRows = 4;
+// The same where B is large: a cluster four or eight rows, its blocks a share of the columns each; a number of B serves those rows, and
+// the blocks' sums are added in order.
 constexpr int kDhPart = 512;
 
-template <typename T>
+template <typename T, int kDhRows>   // 4 or 8
 __global__ void __launch_bounds__(256)
 dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int cluster)
 {
-  __shared__ float row[kDhRows][kDhPart];
+  __shared__ __align__(16) float row[kDhPart][kDhRows];   // (a number of B meets four rows' with one load)
   __shared__ float sums[kDhRows][256];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -935,7 +973,7 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
     const int groups = 256 / width;                  // rows of B at a time
     const int j = tid % width;
     const int group = tid / width;
-    float s[kDhRows][4] = {};
+    float s[kDhRows][2] = {};
     for (int c0 = begin; c0 < end; c0 += kDhPart)
     {
       const int n = end - c0 < kDhPart ? end - c0 : kDhPart;
@@ -944,7 +982,7 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
       {
         const int rr = i / kDhPart;
         const int c = i % kDhPart;
-        row[rr][c] = row0 + rr < m && c < n ? act_f<T>(dy[(row0 + rr) * out + c0 + c]) : 0.0f;
+        row[c][rr] = row0 + rr < m && c < n ? act_f<T>(dy[(row0 + rr) * out + c0 + c]) : 0.0f;
       }
       __syncthreads();
       if (group < groups)
@@ -962,10 +1000,17 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
           for (int u = 0; u < 16; ++u)
           {
             const int at = o + u * groups;
-#pragma unroll
-            for (int rr = 0; rr < kDhRows; ++rr)
+            if (at < n)
             {
-              s[rr][u & 3] = fmaf(at < n ? row[rr][at] : 0.0f, at < n ? w[u] : 0.0f, s[rr][u & 3]);
+#pragma unroll
+              for (int q = 0; q < kDhRows; q += 4)
+              {
+                const float4 v = *reinterpret_cast<const float4 *>(&row[at][q]);
+                s[q][u & 1] = fmaf(v.x, w[u], s[q][u & 1]);
+                s[q + 1][u & 1] = fmaf(v.y, w[u], s[q + 1][u & 1]);
+                s[q + 2][u & 1] = fmaf(v.z, w[u], s[q + 2][u & 1]);
+                s[q + 3][u & 1] = fmaf(v.w, w[u], s[q + 3][u & 1]);
+              }
             }
           }
         }
@@ -975,7 +1020,7 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
 #pragma unroll
     for (int rr = 0; rr < kDhRows; ++rr)
     {
-      sums[rr][tid] = (s[rr][0] + s[rr][1]) + (s[rr][2] + s[rr][3]);
+      sums[rr][tid] = s[rr][0] + s[rr][1];
     }
     __syncthreads();
     // a thread adds the groups of one row and column; in place, where its own first group lies
@@ -1023,43 +1068,64 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
   }
 }
 
-// dx[m, in] = factor * dH . A, a thread a column; `block` of a row's 256 columns
-template <typename T>
-__device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, float factor, int in, int r, int64_t block)
+// dx[m, in] = factor * dH . A, a thread a column of ROWS rows, which share A's numbers; `block` of ROWS rows' 256 columns
+template <typename T, int ROWS>
+__device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, float factor, int64_t m, int in, int r, int64_t block)
 {
-  __shared__ float row[256];
-  const int parts = (in + 255) / 256;   // blocks of a row
-  const int64_t at = block / parts;
+  __shared__ __align__(16) float row[256][ROWS];
+  const int parts = (in + 255) / 256;   // blocks of ROWS rows
+  const int64_t at = block / parts * ROWS;
   const int c = static_cast<int>(block % parts) * 256 + static_cast<int>(threadIdx.x);
-  float s = 0.0f;
+  float s[ROWS] = {};
   for (int j0 = 0; j0 < r; j0 += 256)
   {
+    const int n = r - j0 < 256 ? r - j0 : 256;
     __syncthreads();
-    if (j0 + static_cast<int>(threadIdx.x) < r)
+    for (int e = threadIdx.x; e < n * ROWS; e += 256)
     {
-      row[threadIdx.x] = dh[at * r + j0 + threadIdx.x];
+      const int64_t rr = at + e / n;
+      row[e % n][e / n] = rr < m ? dh[rr * r + j0 + e % n] : 0.0f;
     }
     __syncthreads();
-    const int n = r - j0 < 256 ? r - j0 : 256;
     if (c < in)
     {
 #pragma unroll 8
       for (int k = 0; k < n; ++k)
       {
-        s = fmaf(row[k], act_f<T>(a[static_cast<int64_t>(j0 + k) * in + c]), s);
+        const float w = act_f<T>(a[static_cast<int64_t>(j0 + k) * in + c]);
+        if constexpr (ROWS == 1)
+        {
+          s[0] = fmaf(row[k][0], w, s[0]);
+        }
+        else
+        {
+#pragma unroll
+          for (int q = 0; q < ROWS; q += 4)
+          {
+            const float4 v = *reinterpret_cast<const float4 *>(&row[k][q]);
+            s[q] = fmaf(v.x, w, s[q]);
+            s[q + 1] = fmaf(v.y, w, s[q + 1]);
+            s[q + 2] = fmaf(v.z, w, s[q + 2]);
+            s[q + 3] = fmaf(v.w, w, s[q + 3]);
+          }
+        }
       }
     }
   }
-  if (c < in)
+#pragma unroll
+  for (int q = 0; q < ROWS; ++q)
   {
-    dx[at * in + c] = act_t<T>(s * factor);
+    if (c < in && at + q < m)
+    {
+      dx[(at + q) * in + c] = act_t<T>(s[q] * factor);
+    }
   }
 }
 
 // The sums (the first blocks), and dx, which needs none of them, in one launch
-template <typename T>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(256)
-gradients_dx_kernel(const GradientSums j, int sum_blocks, const float *dh, const T *a, T *dx)
+gradients_dx_kernel(const GradientSums j, int sum_blocks, const float *dh, const T *a, T *dx, int64_t m)
 {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -1068,7 +1134,7 @@ gradients_dx_kernel(const GradientSums j, int sum_blocks, const float *dh, const
     gradient_sums(j, blockIdx.x);
     return;
   }
-  dx_general<T>(dh, a, dx, j.factor, j.in, j.r, static_cast<int64_t>(blockIdx.x) - sum_blocks);
+  dx_general<T, ROWS>(dh, a, dx, j.factor, m, j.in, j.r, static_cast<int64_t>(blockIdx.x) - sum_blocks);
 }
 
 // Few tokens: the reductions, of one slice, and dx in one launch
@@ -1080,11 +1146,11 @@ act_tn_dx_kernel(const Gradients j, int64_t m, int tiles, const T *a, T *dx)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < tiles)
   {
-    tn_general(j, m);
+    tn_general<T, float>(j, m);
   }
   else if (blockIdx.y == 0)
   {
-    dx_general<T>(static_cast<const float *>(j.dh), a, dx, j.factor, j.in, j.r, static_cast<int64_t>(blockIdx.x) - tiles);
+    dx_general<T, 1>(static_cast<const float *>(j.dh), a, dx, j.factor, m, j.in, j.r, static_cast<int64_t>(blockIdx.x) - tiles);
   }
 }
 
@@ -1097,15 +1163,17 @@ int tn_slices(int64_t m, int64_t tiles, int tokens, int blocks)
   return static_cast<int>(n < 1 ? 1 : n);
 }
 
-// So few tokens make one slice, whose sums are rounded where they are made, a launch less.  The whole pass, tensor core: 4096 -> 4096 int8,
-// 64 rows 37.6 -> 35.4 us, 128 rows 39.0 -> 37.3, 200 rows 38.9 and 39.4 so; multiply-adds, fp32: 2048 -> 2048, rank 64, 64 rows 45.2 -> 40.6,
-// 1024 -> 1024, rank 16, 64 rows 20.5 -> 20.0, 128 rows 28.8 and 32.1 so.
-constexpr int64_t kDirectMost = 128;
-constexpr int64_t kDirectMostGeneral = 64;
-
 int64_t general_tiles(int out, int in, int r)
 {
-  return static_cast<int64_t>((out + kTnTile - 1) / kTnTile + (in + kTnTile - 1) / kTnTile) * ((r + kTnTile - 1) / kTnTile);
+  return static_cast<int64_t>((out + kTnWide - 1) / kTnWide + (in + kTnWide - 1) / kTnWide) * ((r + kTnTile - 1) / kTnTile);
+}
+
+// So few tokens make one slice, whose sums are rounded where they are made, a launch less.  The whole pass, tensor core: 4096 -> 4096 int8,
+// 64 rows 37.6 -> 35.4 us, 128 rows 39.0 -> 37.3, 200 rows 38.9 and 39.4 so.  Multiply-adds, fp32, where the tiles are many: 2048 -> 2048,
+// rank 64, 64 rows 37.1 -> 35.1, 128 rows the same; 1024 -> 1024, rank 16, 40 rows 18.5 and 18.6 so, 64 rows 19.7 and 20.5.
+bool one_slice(bool tensor, int64_t m, int out, int in, int r)
+{
+  return tensor ? m <= 128 : m <= (general_tiles(out, in, r) >= 64 ? 64 : 32);
 }
 
 }  // namespace
@@ -1157,7 +1225,7 @@ namespace
 template <typename T>
 int launch_tn_dx(const Gradients &j, const void *a, void *dx, int64_t m, cudaStream_t s)
 {
-  const int tiles = (j.out + kTnTile - 1) / kTnTile + (j.in + kTnTile - 1) / kTnTile;
+  const int tiles = (j.out + kTnWide - 1) / kTnWide + (j.in + kTnWide - 1) / kTnWide;
   const int64_t blocks = tiles + m * ((j.in + 255) / 256);
   CAIFQ_CHECK_ARG(blocks <= 0x7FFFFFFF, "LoRA backward on packed rows: %lld rows of %d columns are too many for its general form",
                   static_cast<long long>(m), j.in);
@@ -1169,11 +1237,15 @@ int launch_tn_dx(const Gradients &j, const void *a, void *dx, int64_t m, cudaStr
 template <typename T>
 int launch_gradients_dx(const GradientSums &j, int64_t sum_blocks, const float *dh, const void *a, void *dx, int64_t m, cudaStream_t s)
 {
-  const int64_t blocks = sum_blocks + m * ((j.in + 255) / 256);
+  // eight rows a block where that many blocks are left: A's numbers come from L2 once for eight (500 rows, 2048 columns, rank 64: 42 us by
+  // single rows)
+  const int parts = (j.in + 255) / 256;
+  const bool eight = m * parts >= 8 * 148;
+  const int64_t blocks = sum_blocks + (eight ? (m + 7) / 8 : m) * parts;
   CAIFQ_CHECK_ARG(blocks <= 0x7FFFFFFF, "LoRA backward on packed rows: %lld rows of %d columns are too many for its general form",
                   static_cast<long long>(m), j.in);
-  CAIFQ_CHECK_CUDA(launch_dependent(gradients_dx_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, j,
-                                    static_cast<int>(sum_blocks), dh, static_cast<const T *>(a), static_cast<T *>(dx)));
+  CAIFQ_CHECK_CUDA(launch_dependent(eight ? gradients_dx_kernel<T, 8> : gradients_dx_kernel<T, 1>, dim3(static_cast<unsigned>(blocks)), dim3(256),
+                                    0, s, j, static_cast<int>(sum_blocks), dh, static_cast<const T *>(a), static_cast<T *>(dx), m));
   return CAIFQ_OK;
 }
 }  // namespace
@@ -1187,7 +1259,7 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
   auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   const bool tensor = dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
                       (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(x);
-  const bool direct = m <= (tensor ? kDirectMost : kDirectMostGeneral);
+  const bool direct = one_slice(tensor, m, out, in, r);
   const Gradients j{dy, h, dh, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, dtype, dh_dtype, out, in, r};
   int slices = 0;
   if (tensor)
@@ -1213,9 +1285,13 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
   else
   {
     slices = direct ? 1 : tn_slices(m, general_tiles(out, in, r), kTnRows, kTnGeneralBlocks);
-    const dim3 grid((out + kTnTile - 1) / kTnTile + (in + kTnTile - 1) / kTnTile, (r + kTnTile - 1) / kTnTile,
+    const dim3 grid((out + kTnWide - 1) / kTnWide + (in + kTnWide - 1) / kTnWide, (r + kTnTile - 1) / kTnTile,
                     static_cast<unsigned>(slices));
-    CAIFQ_CHECK_CUDA(launch_dependent(act_tn_kernel, grid, dim3(256), 0, s, j, m));
+    auto kernel = dtype == CAIFQ_F32 ? act_tn_kernel<float, float>
+                                     : (dtype == CAIFQ_F16 ? act_tn_kernel<__half, float>
+                                                           : (dh_dtype == CAIFQ_BF16 ? act_tn_kernel<__nv_bfloat16, __nv_bfloat16>
+                                                                                     : act_tn_kernel<__nv_bfloat16, float>));
+    CAIFQ_CHECK_CUDA(launch_dependent(kernel, grid, dim3(256), 0, s, j, m));
   }
   if (direct && dx == nullptr)
   {
@@ -1261,7 +1337,9 @@ int launch_dh_of(const void *dy, const void *b, float *dh, int64_t m, int out, i
   // A block a row where a thread then reads up to 64 numbers of B: four rows a block, and clusters, cost 2 us and more there (64 rows,
   // 1024 columns, rank 16), and save 30 of 91 where it would read 480 (152 rows, 1920 columns, rank 64)
   const bool large = static_cast<int64_t>(out) * r > 64 * 256;
-  const int64_t groups = large ? (m + 3) / 4 : m;
+  // (eight rows: half the reading of B, where enough blocks are left)
+  const bool eight = large && m >= 8 * 32;
+  const int64_t groups = eight ? (m + 7) / 8 : (m + 3) / 4;
   int cluster = 1;
   while (large && cluster < 8 && groups * cluster < 4 * 148 && static_cast<int64_t>(out) * r > static_cast<int64_t>(64 * 256) * cluster)
   {
@@ -1273,7 +1351,7 @@ int launch_dh_of(const void *dy, const void *b, float *dh, int64_t m, int out, i
                                       static_cast<const T *>(b), dh, m, out, r));
     return CAIFQ_OK;
   }
-  CAIFQ_CHECK_CUDA(launch_dependent_clusters(dh_kernel<T>, dim3(static_cast<unsigned>(groups * cluster)), dim3(256), 0, s, cluster,
+  CAIFQ_CHECK_CUDA(launch_dependent_clusters(eight ? dh_kernel<T, 8> : dh_kernel<T, 4>, dim3(static_cast<unsigned>(groups * cluster)), dim3(256), 0, s, cluster,
                                              static_cast<const T *>(dy), static_cast<const T *>(b), dh, m, out, r, cluster));
   return CAIFQ_OK;
 }

@@ -222,6 +222,17 @@ def test_backward_on_packed_rows_of_any_width(dtype, compute, in_dim, out_dim, m
     check_grads(*case, nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], compute), compute)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float16])
+@pytest.mark.parametrize("in_dim,out_dim,m,rank", [(700, 130, 500, 5), (300, 600, 301, 40), (64, 100, 260, 300), (65, 63, 64, 33), (64, 64, 65, 1),
+                                                   (2048, 1024, 150, 12), (512, 1030, 30, 64)])
+def test_backward_in_general_of_more_rows(dtype, in_dim, out_dim, m, rank):
+    case = make_case(in_dim + m, orc.I8, dtype, in_dim, out_dim, m, rank)
+    got = nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], nv.F32)
+    check_grads(*case, got, nv.F32)
+    for a, b in zip(nv.lora_linear_bwd_packed(case[0], case[1], case[4], case[2], case[3], nv.F32), got):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("storage,compute", [(orc.I8, nv.F32), (orc.I4, nv.BF16)])
 @pytest.mark.parametrize("in_dim,out_dim,m,rank", [(256, 1024, 1024, 16), (128, 1152, 1100, 8), (384, 1280, 2049, 32), (128, 2048, 2048, 8),
                                                    (256, 1024, 4097, 32), (128, 1024, 4095, 16), (128, 1408, 8300, 16), (256, 896, 3000, 16),
