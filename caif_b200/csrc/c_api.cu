@@ -1117,6 +1117,7 @@ int check_bank(const caifq_weight *w, const caifq_lora_bank *bank, const char *w
   CAIFQ_CHECK_ARG(is_float_dtype(bank->dtype), "%s: the bank's dtype must be F32, F16 or BF16", who);
   CAIFQ_CHECK_ARG(bank->max_rank >= 1 && bank->max_rank <= kBankMaxRank, "%s: ranks from 1 to %d, not %d", who, kBankMaxRank,
                   bank->max_rank);
+  CAIFQ_CHECK_ARG(bank->out_dim <= kBankMostOut, "%s: %d output features, at most %d are taken", who, bank->out_dim, kBankMostOut);
   CAIFQ_CHECK_ARG(bank->in_dim == w->in_dim && bank->out_dim == w->out_dim,
                   "%s: the bank is for %d -> %d features, the weight has %d -> %d", who, bank->in_dim, bank->out_dim,
                   w->in_dim, w->out_dim);

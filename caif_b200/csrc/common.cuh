@@ -445,7 +445,8 @@ struct LinearArgs
 
 constexpr int kMaxPeers = 8;
 constexpr int kBankMost = 1 << 24;     // adapters of a bank
-constexpr int kBankMaxRank = 1024;   // of an adapter bank: a row of x . A^T lies in shared memory
+constexpr int kBankMostOut = 65535 * 64;   // their output features: the second dimension of a launch
+constexpr int kBankMaxRank = 1024;       // ranks
 
 // generic tiled fp32-FMA GEMM over every (storage, compute) cell
 int launch_linear_generic(const LinearArgs &args, cudaStream_t s);

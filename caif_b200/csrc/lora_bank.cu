@@ -40,12 +40,14 @@ __device__ __forceinline__ __nv_bfloat16 bank_t<__nv_bfloat16>(float v) { return
 
 // ---- any type, rank and width: fp32 multiply-adds ----
 
-// a CTA a row, a warp a column of h at a time
+// A block a row; `split` of its eight warps share a column of h at a time, a part of the row each.  Bound by latency: sixteen loads of
+// each operand on their way, and short parts where there are few rows (one row of 2048, rank 16: 13 us by whole rows).
 template <typename T>
 __global__ void __launch_bounds__(kBankThreads)
 bank_down_kernel(const T *x, const int32_t *__restrict__ adapter_of_row, const caifq_lora_entry *__restrict__ entries, int count,
-                 float *h, int ld, int in_dim)
+                 float *h, int ld, int in_dim, int split)
 {
+  __shared__ float sums[kBankThreads / 32];
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t row = blockIdx.x;
@@ -55,33 +57,42 @@ bank_down_kernel(const T *x, const int32_t *__restrict__ adapter_of_row, const c
     return;
   }
   const int lane = threadIdx.x & 31;
+  const int warp = static_cast<int>(threadIdx.x >> 5);
   const int rank = entries[id].rank;
   const T *a = static_cast<const T *>(entries[id].a);
   const T *src = x + row * in_dim;
-  const int step = static_cast<int>(gridDim.y) * (kBankThreads / 32);
-  for (int j = blockIdx.y * (kBankThreads / 32) + static_cast<int>(threadIdx.x >> 5); j < rank; j += step)
+  const int part = warp % split;
+  const int begin = static_cast<int>(static_cast<int64_t>(in_dim) * part / split);
+  const int end = static_cast<int>(static_cast<int64_t>(in_dim) * (part + 1) / split);
+  const int per = kBankThreads / 32 / split;   // columns of h at a time
+  for (int j0 = blockIdx.y * per; j0 < rank; j0 += static_cast<int>(gridDim.y) * per)
   {
-    const T *w = a + static_cast<int64_t>(j) * in_dim;
+    const int j = j0 + warp / split;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int c = lane;
-    for (; c + 480 < in_dim; c += 512)   // (bound by latency: sixteen loads of each on their way)
+    if (j < rank)
     {
-      T u[16], v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
+      const T *w = a + static_cast<int64_t>(j) * in_dim;
+      int c = begin + lane;
+      for (; c + 480 < end; c += 512)
       {
-        u[i] = src[c + 32 * i];
-        v[i] = w[c + 32 * i];
-      }
+        T u[16], v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-      {
-        s[i & 3] = fmaf(bank_f<T>(u[i]), bank_f<T>(v[i]), s[i & 3]);
+        for (int i = 0; i < 16; ++i)
+        {
+          u[i] = src[c + 32 * i];
+          v[i] = w[c + 32 * i];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+          s[i & 3] = fmaf(bank_f<T>(u[i]), bank_f<T>(v[i]), s[i & 3]);
+        }
       }
-    }
-    for (; c < in_dim; c += 32)
-    {
-      s[0] = fmaf(bank_f<T>(src[c]), bank_f<T>(w[c]), s[0]);
+#pragma unroll 8
+      for (; c < end; c += 32)
+      {
+        s[0] = fmaf(bank_f<T>(src[c]), bank_f<T>(w[c]), s[0]);
+      }
     }
     float v = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
@@ -89,48 +100,79 @@ bank_down_kernel(const T *x, const int32_t *__restrict__ adapter_of_row, const c
     {
       v += __shfl_xor_sync(0xFFFFFFFFu, v, off);
     }
-    if (lane == 0)
+    if (split > 1)
+    {
+      __syncthreads();   // the sums before have been read
+      if (lane == 0)
+      {
+        sums[warp] = v;
+      }
+      __syncthreads();
+      v = 0.0f;
+      for (int k = 0; k < split; ++k)
+      {
+        v += sums[warp - part + k];
+      }
+    }
+    if (lane == 0 && part == 0 && j < rank)
     {
       h[row * ld + j] = v;
     }
   }
 }
 
-// a thread a column of y
+// A block 64 columns of a row of y, four threads a column: B's rows lie one behind the other and come through shared memory, 64 ranks at a
+// time.  (A thread a column straight from memory: 64 rows of 2048 columns, rank 64, 35 us)
+constexpr int kBankColumns = 64;
+
 template <typename T>
 __global__ void __launch_bounds__(kBankThreads)
 bank_up_kernel(const float *frozen, const float *h, const int32_t *__restrict__ adapter_of_row,
                const caifq_lora_entry *__restrict__ entries, int count, T *y, int ld, int out_dim)
 {
-  __shared__ float sh[kBankMaxRank];
+  __shared__ float sh[64];
+  __shared__ float sb[kBankColumns][64 + 1];
   asm volatile("griddepcontrol.wait;" : "+l"(adapter_of_row), "+l"(entries)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t row = blockIdx.x;
   const int id = adapter_of_row[row];
   const bool mine = id >= 0 && id < count;
   const int rank = mine ? entries[id].rank : 0;
-  for (int j = threadIdx.x; j < rank; j += kBankThreads)
-  {
-    sh[j] = h[row * ld + j];
-  }
-  __syncthreads();
-  const int col = blockIdx.y * kBankThreads + static_cast<int>(threadIdx.x);
-  if (col >= out_dim)
-  {
-    return;
-  }
+  const T *b = mine ? static_cast<const T *>(entries[id].b) : nullptr;
+  const int col0 = static_cast<int>(blockIdx.y) * kBankColumns;
+  const int columns = out_dim - col0 < kBankColumns ? out_dim - col0 : kBankColumns;
+  const int col = static_cast<int>(threadIdx.x) / 4;
+  const int quarter = static_cast<int>(threadIdx.x) % 4;
   float v = 0.0f;
-  if (mine)
+  for (int j0 = 0; j0 < rank; j0 += 64)
   {
-    const T *b = static_cast<const T *>(entries[id].b) + static_cast<int64_t>(col) * rank;
-    for (int j = 0; j < rank; ++j)
+    const int n = rank - j0 < 64 ? rank - j0 : 64;
+    __syncthreads();   // the ranks before have been read
+    if (static_cast<int>(threadIdx.x) < n)
     {
-      v = fmaf(sh[j], bank_f<T>(b[j]), v);
+      sh[threadIdx.x] = h[row * ld + j0 + threadIdx.x];
     }
-    v *= entries[id].scale;
+#pragma unroll 8
+    for (int e = threadIdx.x; e < columns * n; e += kBankThreads)
+    {
+      sb[e / n][e % n] = bank_f<T>(b[static_cast<int64_t>(col0 + e / n) * rank + j0 + e % n]);
+    }
+    __syncthreads();
+    if (col < columns)
+    {
+      for (int k = quarter; k < n; k += 4)
+      {
+        v = fmaf(sh[k], sb[col][k], v);
+      }
+    }
   }
-  const float f = frozen[row * out_dim + col];
-  y[row * out_dim + col] = bank_t<T>(mine ? f + v : f);
+  v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
+  v += __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+  if (quarter == 0 && col < columns)
+  {
+    const float f = frozen[row * out_dim + col0 + col];
+    y[row * out_dim + col0 + col] = bank_t<T>(mine ? fmaf(v, entries[id].scale, f) : f);
+  }
 }
 
 // ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on tiles of up to 16 rows of one adapter ----
@@ -971,9 +1013,15 @@ int few_mma(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const vo
 template <typename T>
 int down_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, int64_t m, float *h, cudaStream_t s)
 {
-  CAIFQ_CHECK_CUDA(launch_dependent(bank_down_kernel<T>, dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.max_rank + 7) / 8)),
+  int split = 1;
+  while (split < 8 && m * bank.max_rank * split < 8 * 8 * 148 && bank.in_dim >= 256 * split)
+  {
+    split *= 2;
+  }
+  const int per = 8 / split;
+  CAIFQ_CHECK_CUDA(launch_dependent(bank_down_kernel<T>, dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.max_rank + per - 1) / per)),
                                     dim3(kBankThreads), 0, s, static_cast<const T *>(x), adapter_of_row, bank.entries, bank.count,
-                                    h, bank.max_rank, bank.in_dim));
+                                    h, bank.max_rank, bank.in_dim, split));
   return CAIFQ_OK;
 }
 
@@ -982,7 +1030,7 @@ int up_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const
                cudaStream_t s)
 {
   CAIFQ_CHECK_CUDA(launch_dependent(bank_up_kernel<T>,
-                                    dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.out_dim + kBankThreads - 1) / kBankThreads)),
+                                    dim3(static_cast<unsigned>(m), static_cast<unsigned>((bank.out_dim + kBankColumns - 1) / kBankColumns)),
                                     dim3(kBankThreads), 0, s, frozen, h, adapter_of_row, bank.entries, bank.count,
                                     static_cast<T *>(y), bank.max_rank, bank.out_dim));
   return CAIFQ_OK;
@@ -990,10 +1038,10 @@ int up_general(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const
 
 bool on_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// whether a call runs on the tensor core.  (out_dim: the grid's second dimension; the tiles with their clusters fit the first)
+// whether a call runs on the tensor core
 bool tiled(const caifq_lora_bank &bank, const void *x, const void *y, const float *frozen, int64_t m)
 {
-  return bank.vectors != 0 && (bank.in_dim % 32) == 0 && (bank.out_dim % 8) == 0 && bank.out_dim <= 65535 * 128 && on_16(x) &&
+  return bank.vectors != 0 && (bank.in_dim % 32) == 0 && (bank.out_dim % 8) == 0 && on_16(x) &&
          on_16(y) && on_16(frozen) && (m <= kSmallCall || bank.count <= kTableMost);
 }
 

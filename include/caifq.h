@@ -358,7 +358,7 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
  * once.  (Under bf16 compute code times scale of an int4 weight is rounded to bf16 first, and only that.)
  *
  * A bank is a table of `count` (up to 2^24) entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
- * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank]), fills the table's image in HOST memory and every
+ * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank], out at most 65535 * 64), fills the table's image in HOST memory and every
  * field of *bank but `entries`; the caller copies the image to the device and sets bank->entries to it.  It needs no GPU.
  * Factors stay where they are and must outlive the calls.
  */

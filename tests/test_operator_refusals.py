@@ -83,6 +83,9 @@ def test_bank_linear():
     refused(call(w=nv.CWeight(P, P, nv.I8, 0, 128, 256, 256)), "the weight has")
     refused(call(w=nv.CWeight(None, P, nv.I8, 0, 128, 128, 256)), "not loaded")
     assert call(m=0) == 0
+    bank.out_dim = w.out_dim = 65535 * 64 + 1
+    refused(call(), "output features")
+    bank.out_dim = w.out_dim = 256
     bank.count = (1 << 24) + 1
     refused(call(), "adapters")
     refused(lib.caifq_lora_bank_entries((nv.CLora * 1)(lora()), (1 << 24) + 1, 128, 256, (nv.CLoraEntry * 1)(), ctypes.byref(bank)),
