@@ -263,6 +263,26 @@ def test_backward_rounds_an_expanded_int4_weight_once(m):
     assert torch.equal(dx, nv.weight_materialize(weight).float()[pick].bfloat16())
 
 
+@pytest.mark.parametrize("m", [40, 333, 2500])
+@pytest.mark.parametrize("what", ["hidden", "codes", "dy"])
+def test_backward_off_a_16_byte_boundary(m, what):
+    weight, lora, packed, hidden, dy = make_case(m, orc.I8, torch.bfloat16, 256, 384, m, 16)
+
+    def shifted(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    if what == "hidden":
+        hidden = shifted(hidden)
+    elif what == "codes":
+        packed = nv.PackedRows(shifted(packed.codes), shifted(packed.scales))
+    else:
+        dy = shifted(dy)
+    case = (weight, lora, packed, hidden, dy)
+    check_grads(*case, nv.lora_linear_bwd_packed(weight, lora, dy, packed, hidden, nv.F32), nv.F32)
+
+
 def test_backward_beside_the_one_on_full_rows():
     """On rows that eight bits hold, lora_linear_bwd gives the same gradients: dx bit for bit where alpha / rank is a power of
     two, dA and dB to the rounding of sums in another order."""

@@ -108,6 +108,36 @@ def test_serving_step_of_requests_with_adapters_of_their_own(m):
     assert nv.lib().caifq_device_status() == 0
 
 
+def test_calls_on_two_streams_at_once():
+    """Each stream's calls have scratch of their own: the results are those of one stream."""
+    g, weight, x, gamma, beta, make = setup(5, orc.I4, 512, 384, 200)
+    bank = nv.LoraBank([make(r) for r in (16, 8, 64, 16)])
+    lora = make(16)
+    idx = torch.randint(-1, 4, (200,), generator=g, device="cuda", dtype=torch.int32)
+    dy = torch.randn(200, 384, generator=g, device="cuda").bfloat16()
+
+    def step():
+        n, mean, rstd = nv.layernorm_fwd(x, gamma, beta)
+        y = nv.lora_bank_linear_fwd(weight, bank, idx, n, nv.BF16)
+        few = nv.lora_bank_linear_fwd(weight, bank, idx[:7], n[:7], nv.BF16)
+        h = (n.float() @ lora.a.float().t()).bfloat16()
+        dn, d_a, d_b = nv.lora_linear_bwd_packed(weight, lora, dy, nv.act_pack(n), h, nv.BF16)
+        return (y, few, d_a, d_b) + nv.layernorm_bwd(dn, x, mean, rstd, gamma)
+
+    want = step()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step())
+    torch.cuda.synchronize()
+    for results in got:
+        for result in results:
+            assert all(torch.equal(a, b) for a, b in zip(result, want))
+
+
 def test_without_dependent_launches():
     """Launches that wait for one another as a stream's do give the same numbers (the switch is read once a process)."""
     here = os.path.dirname(os.path.abspath(__file__))
