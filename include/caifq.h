@@ -355,7 +355,8 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
  *   y[t] = x[t] . W_deq^T + (alpha_a / rank_a) (x[t] . A_a^T) . B_a^T,   a = adapter_of_row[t]
  * Rows whose index is outside [0, count) get the frozen product alone.  Indices, factors and rows may change between two
  * replays of a captured call; rows need no order.  x . A^T and the frozen product are kept in fp32; the result is rounded
- * once.  (Under bf16 compute code times scale of an int4 weight is rounded to bf16 first, and only that.)
+ * once.  (Under bf16 compute code times scale of an int4 weight is rounded to bf16 first; where a tensor-core kernel converts the
+ * codes itself on more than 768 rows the scale is too.)
  *
  * A bank is a table of `count` (up to 2^24) entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
  * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank], out at most 65535 * 64), fills the table's image in HOST memory and every
