@@ -135,6 +135,8 @@ int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of
                           const void *y, void *scratch, cudaStream_t s);
 int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m,
                         void *y, void *scratch, cudaStream_t s);
+bool lora_bank_frozen_supported(const caifq_weight &w, const void *x, int64_t m);
+int launch_lora_bank_frozen(const caifq_weight &w, const void *x, int dtype, int64_t m, float *frozen, cudaStream_t s);
 // act8.cu
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
@@ -1143,6 +1145,20 @@ BankWs bank_ws(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m, in
                             : 0);
   return o;
 }
+// whether only the kernel for any cell takes the product of rows in fp32 compute
+bool any_cell_only(const caifq_weight *w, const void *x, int x_dtype, int64_t m, float *y)
+{
+  LinearArgs probe{};
+  probe.w = *w;
+  probe.a = x;
+  probe.a_dtype = x_dtype;
+  probe.a_prescale = 1.0f;
+  probe.m = m;
+  probe.c = y;
+  probe.c_dtype = CAIFQ_F32;
+  probe.compute_dtype = CAIFQ_F32;
+  return !decode_supported(probe) && !rows_supported(probe) && !stream_supported(probe) && !umma_supported(probe) && !f32_supported(probe);
+}
 }  // namespace
 
 int caifq_lora_bank_entries(const caifq_lora *loras, int32_t count, int32_t in_dim, int32_t out_dim,
@@ -1218,7 +1234,10 @@ int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *ban
   int r = launch_lora_bank_down(*bank, adapter_of_row, x, frozen, m, y, workspace, s);
   if (r == CAIFQ_OK)
   {
-    r = linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who, true);
+    const bool own = compute_dtype == CAIFQ_F32 && forced_path() == Force::None && lora_bank_frozen_supported(*w, x, m) &&
+                     any_cell_only(w, x, bank->dtype, m, frozen);
+    r = own ? launch_lora_bank_frozen(*w, x, bank->dtype, m, frozen, s)
+            : linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who, true);
   }
   if (r == CAIFQ_OK)
   {

@@ -175,6 +175,83 @@ bank_up_kernel(const float *frozen, const float *h, const int32_t *__restrict__ 
   }
 }
 
+// The frozen product of few rows and a weight whose width no other kernel takes (they want whole 128s): a warp a row of codes for eight
+// rows of x, fp32 multiply-adds, code times scale in fp32 (int8: the scale at the end).  Bound by the loads of x from L1 where there are
+// many rows and by latency where there are few (1408 -> 1776 int4, 2 rows of fp32: the kernel for any cell takes 187 us).
+constexpr int kFrozenRows = 8;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) BankPiece
+{
+  T e[N];
+};
+
+template <typename T, bool I4>
+__global__ void __launch_bounds__(kBankThreads)
+bank_frozen_kernel(const T *x, const uint8_t *__restrict__ codes, const void *__restrict__ scales, float *frozen, int64_t m, int in_dim,
+                   int out_dim, int group_size)
+{
+  constexpr int N = I4 ? 8 : 4;   // codes of a lane at a time: four bytes
+  asm volatile("griddepcontrol.wait;" : "+l"(codes), "+l"(scales)::"memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int64_t o = static_cast<int64_t>(blockIdx.x) * (kBankThreads / 32) + static_cast<int>(threadIdx.x >> 5);
+  if (o >= out_dim)
+  {
+    return;
+  }
+  const int64_t row0 = static_cast<int64_t>(blockIdx.y) * kFrozenRows;
+  const int64_t flat = o * in_dim;
+  const bool whole = I4 && in_dim % group_size == 0;   // (no group in two rows)
+  const int64_t first_group = whole ? o * (in_dim / group_size) : 0;
+  float s[kFrozenRows] = {};
+#pragma unroll 2
+  for (int c = lane * N; c < in_dim; c += 32 * N)
+  {
+    const uint32_t word = *reinterpret_cast<const uint32_t *>(codes + (I4 ? (flat + c) / 2 : flat + c));
+    float scale = 1.0f;
+    if constexpr (I4)
+    {
+      const int64_t group = whole ? first_group + c / group_size : (flat + c) / group_size;
+      scale = __half2float(static_cast<const __half *>(scales)[group]);
+    }
+    float w[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+    {
+      w[i] = I4 ? static_cast<float>(static_cast<int>((word >> (4 * i)) & 15u ^ 8u) - 8) * scale
+                : static_cast<float>(static_cast<int8_t>(word >> (8 * (i & 3))));
+    }
+#pragma unroll
+    for (int k = 0; k < kFrozenRows; ++k)
+    {
+      if (row0 + k < m)
+      {
+        const BankPiece<T, N> v = *reinterpret_cast<const BankPiece<T, N> *>(x + (row0 + k) * in_dim + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+          s[k] = fmaf(bank_f<T>(v.e[i]), w[i], s[k]);
+        }
+      }
+    }
+  }
+  const float last = !I4 && scales != nullptr ? *static_cast<const float *>(scales) : 1.0f;
+#pragma unroll
+  for (int k = 0; k < kFrozenRows; ++k)
+  {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1)
+    {
+      s[k] += __shfl_xor_sync(0xFFFFFFFFu, s[k], off);
+    }
+    if (lane == k && row0 + k < m)
+    {
+      frozen[(row0 + k) * out_dim + o] = s[k] * last;
+    }
+  }
+}
+
 // ---- bf16 factors of rank 8, 16, ... 64 on 16-byte boundaries: the tensor core on tiles of up to 16 rows of one adapter ----
 // Rows are dealt to tiles by adapter first, wherever they stand in the batch (those without one make tiles of their own, which
 // `up` copies).  In a call of up to 128 rows every block does that by itself, longer ones have a launch for it.  Tiles
@@ -1076,6 +1153,41 @@ int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of
       return down_general<__half>(bank, adapter_of_row, x, m, h, s);
     default:
       return down_general<__nv_bfloat16>(bank, adapter_of_row, x, m, h, s);
+  }
+}
+
+// frozen[m, out] = x . W^T in fp32 by bank_frozen_kernel, where it takes the call: int8 with one scale or none, int4 with groups of eights,
+// rows of x on 16-byte boundaries, few of them
+bool lora_bank_frozen_supported(const caifq_weight &w, const void *x, int64_t m)
+{
+  return m <= 128 && (w.in_dim % 8) == 0 && on_16(x) && (reinterpret_cast<uintptr_t>(w.codes) & 3u) == 0 &&
+         ((w.storage == CAIFQ_I8 && (w.scales == nullptr || w.scheme == CAIFQ_PER_TENSOR)) ||
+          (w.storage == CAIFQ_I4 && w.scales != nullptr && w.group_size > 0 && (w.group_size % 8) == 0));
+}
+
+namespace
+{
+template <typename T>
+int frozen_of(const caifq_weight &w, const void *x, int64_t m, float *frozen, cudaStream_t s)
+{
+  auto kernel = w.storage == CAIFQ_I4 ? bank_frozen_kernel<T, true> : bank_frozen_kernel<T, false>;
+  const dim3 grid(static_cast<unsigned>((w.out_dim + 7) / 8), static_cast<unsigned>((m + kFrozenRows - 1) / kFrozenRows));
+  CAIFQ_CHECK_CUDA(launch_dependent(kernel, grid, dim3(kBankThreads), 0, s, static_cast<const T *>(x), static_cast<const uint8_t *>(w.codes),
+                                    w.scales, frozen, m, w.in_dim, w.out_dim, w.group_size));
+  return CAIFQ_OK;
+}
+}  // namespace
+
+int launch_lora_bank_frozen(const caifq_weight &w, const void *x, int dtype, int64_t m, float *frozen, cudaStream_t s)
+{
+  switch (dtype)
+  {
+    case CAIFQ_F32:
+      return frozen_of<float>(w, x, m, frozen, s);
+    case CAIFQ_F16:
+      return frozen_of<__half>(w, x, m, frozen, s);
+    default:
+      return frozen_of<__nv_bfloat16>(w, x, m, frozen, s);
   }
 }
 

@@ -124,6 +124,22 @@ def test_beside_a_frozen_weight(storage, compute, m):
     assert bool(((y.double() - (base + part)).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("storage", [orc.I8, orc.I4])
+@pytest.mark.parametrize("in_dim,out_dim,m", [(128, 1, 1), (384, 40, 8), (640, 880, 2), (1408, 1776, 9), (256, 136, 128), (256, 136, 129)])
+def test_beside_a_weight_of_another_width(storage, dtype, in_dim, out_dim, m):
+    weight, _, _ = make_weight(np.random.default_rng(m), out_dim, in_dim, storage)
+    w64 = nv.weight_materialize(weight).double()
+    bank = make_bank(m, in_dim, out_dim, [16, 5], dtype)
+    x, idx = make_rows(m, m, in_dim, 2, dtype)
+    y = nv.lora_bank_linear_fwd(weight, bank, idx, x, orc.F32)
+    part, tol = adapters_64(bank, idx, x, out_dim)
+    base, terms = x.double() @ w64.t(), x.double().abs() @ w64.abs().t()
+    tol = tol + (S + (in_dim / 32 + 64) * S + (2.0 ** -16 if storage == orc.I4 and dtype == torch.bfloat16 else 0.0)) * terms
+    tol = tol + half(dtype) * (base.abs() + part.abs() + (base + part).abs() + 3 * tol) + tiny(dtype)
+    assert bool(((y.double() - (base + part)).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("m", [1, 16, 17, 48, 128, 129, 500, 768, 1500])
 def test_int4_weight_is_rounded_once(m):
     """Rows of one 1 pick columns of the weight: code times scale as bf16, with no rounding of the scale before that."""
