@@ -74,7 +74,7 @@ layernorm_fwd_kernel(const T *x, const float *__restrict__ gamma, const float *_
   __shared__ float slots[kLnThreads / 32];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(beta)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
   {
     const T *src = x + r * dim;
     T *dst = y + r * dim;
@@ -112,7 +112,7 @@ layernorm_dx_kernel(const T *dy, const T *x, const float *__restrict__ gamma, co
   __shared__ float slots[kLnThreads / 32];
   asm volatile("griddepcontrol.wait;" : "+l"(gamma), "+l"(mean_in), "+l"(rstd_in)::"memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
   {
     const int64_t at = r * dim;
     const float mean = mean_in[r];

@@ -1,0 +1,42 @@
+"""The operators around an adapted projection at the ends of what their entry points take."""
+import pytest
+import torch
+
+from caif_b200 import native as nv
+
+pytestmark = pytest.mark.gpu
+
+
+def test_layernorm_of_the_most_rows():
+    """2^31 - 1 rows of one column off a 16-byte boundary: the form that walks over the rows counts them past 2^31.  One value's mean is
+    the value, its distance from it 0."""
+    rows = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    x = torch.zeros(rows + 1, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 1, 1183, 1184, rows // 2, rows - 1185, rows - 1184, rows - 2, rows - 1], device="cuda")
+    x[1:][at] = torch.arange(1.0, 10.0, device="cuda").bfloat16()
+    x = x[1:].view(rows, 1)
+    y = torch.empty(rows + 2, dtype=torch.bfloat16, device="cuda")
+    y[-1] = 7.0                                        # behind the last row
+    mean = torch.empty(rows + 1, device="cuda")
+    rstd = torch.empty(rows + 1, device="cuda")
+    mean[-1] = rstd[-1] = 7.0
+    beta = torch.full((1,), 0.5, device="cuda")
+    lib, s = nv.lib(), torch.cuda.current_stream().cuda_stream
+    out = y[1:]
+    nv._check(lib.caifq_layernorm_fwd(x.data_ptr(), None, beta.data_ptr(), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), 0.25, nv.BF16, rows, 1, s),
+              "layernorm_fwd")
+    assert float(y[-1]) == 7.0 and float(mean[-1]) == 7.0 and float(rstd[-1]) == 7.0
+    step = 1 << 28
+    for i in range(0, rows, step):
+        end = min(rows, i + step)
+        assert bool((mean[i:end] == x[i:end, 0]).all()) and bool((out[i:end] == 0.5).all()) and bool((rstd[i:end] == 2.0).all())
+    # dx over dy, without the columns' sums: a row of one value has no gradient
+    out.fill_(1.0)
+    y[-1] = 7.0
+    nv._check(lib.caifq_layernorm_bwd(out.data_ptr(), x.data_ptr(), None, mean.data_ptr(), rstd.data_ptr(), out.data_ptr(), None, None, 0, None, nv.BF16,
+                                      rows, 1, s), "layernorm_bwd")
+    assert float(y[-1]) == 7.0
+    for i in range(0, rows, step):
+        assert not bool(out[i:min(rows, i + step)].any())
