@@ -1119,6 +1119,7 @@ int check_bank(const caifq_weight *w, const caifq_lora_bank *bank, const char *w
   CAIFQ_CHECK_ARG(is_float_dtype(bank->dtype), "%s: the bank's dtype must be F32, F16 or BF16", who);
   CAIFQ_CHECK_ARG(bank->max_rank >= 1 && bank->max_rank <= kBankMaxRank, "%s: ranks from 1 to %d, not %d", who, kBankMaxRank,
                   bank->max_rank);
+  CAIFQ_CHECK_ARG(bank->in_dim <= kAdapterMostDim, "%s: %d input features, at most %d are taken", who, bank->in_dim, kAdapterMostDim);
   CAIFQ_CHECK_ARG(bank->out_dim <= kBankMostOut, "%s: %d output features, at most %d are taken", who, bank->out_dim, kBankMostOut);
   CAIFQ_CHECK_ARG(bank->in_dim == w->in_dim && bank->out_dim == w->out_dim,
                   "%s: the bank is for %d -> %d features, the weight has %d -> %d", who, bank->in_dim, bank->out_dim,
@@ -1322,6 +1323,8 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
   }
   CAIFQ_CHECK_ARG(m >= 0, "%s: negative m", who);
   CAIFQ_CHECK_ARG(m <= 0x7FFFFFFF, "%s: %lld rows", who, static_cast<long long>(m));
+  CAIFQ_CHECK_ARG(w->in_dim <= kAdapterMostDim && w->out_dim <= kAdapterMostDim, "%s: %d -> %d features, at most %d are taken", who, w->in_dim,
+                  w->out_dim, kAdapterMostDim);
   CAIFQ_CHECK_ARG(is_float_dtype(compute_dtype), "%s: the compute dtype must be F32, F16 or BF16", who);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int sd = lora->dtype;

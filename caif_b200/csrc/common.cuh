@@ -447,6 +447,7 @@ constexpr int kMaxPeers = 8;
 constexpr int kBankMost = 1 << 24;     // adapters of a bank
 constexpr int kBankMostOut = 65535 * 64;   // their output features: the second dimension of a launch
 constexpr int kBankMaxRank = 1024;       // ranks
+constexpr int kAdapterMostDim = 1 << 29;   // features beside a bank or an adapter on packed rows: a few strides past them stay within 32 bits
 
 // generic tiled fp32-FMA GEMM over every (storage, compute) cell
 int launch_linear_generic(const LinearArgs &args, cudaStream_t s);

@@ -359,7 +359,7 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
  * codes itself on more than 768 rows the scale is too.)
  *
  * A bank is a table of `count` (up to 2^24) entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
- * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank], out at most 65535 * 64), fills the table's image in HOST memory and every
+ * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank], in at most 2^29, out at most 65535 * 64), fills the table's image in HOST memory and every
  * field of *bank but `entries`; the caller copies the image to the device and sets bank->entries to it.  It needs no GPU.
  * Factors stay where they are and must outlive the calls.
  */
@@ -410,6 +410,7 @@ CAIFQ_API int caifq_act_unpack(const int8_t *codes, const uint8_t *scales, void 
  * caifq_lora_linear_bwd_expanded for an adapter whose input was kept by caifq_act_pack: the same gradients, with dA taken
  * from the codes, which are never expanded in memory.  Sums over tokens run in a fixed order (equal calls give equal bits),
  * and alpha / rank multiplies fp32 sums instead of rounded copies of dy.  With m == 0 dA and dB are zeros.  dx may not overlap dy.
+ * in and out are at most 2^29.
  */
 CAIFQ_API size_t caifq_lora_bwd_packed_workspace_bytes(const caifq_weight *w, const caifq_lora *lora, int64_t m,
                                                        int32_t compute_dtype);
