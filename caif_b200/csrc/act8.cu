@@ -410,12 +410,14 @@ struct Gradients
 
 // any type and width: 64 x 32 tiles of the result, fp32 multiply-adds, eight a thread for six values from shared memory.  The next
 // tokens' loads are issued before this trip's products.  (32 x 32 tiles with four for four: 500 rows, 2048 columns each way, rank 64, 37 us instead of 23)
+// A trip's 32 products are added up by themselves and then to the trips before (64 tokens or fewer: one chain): with one chain over a slice, 8192 tokens of a layer so wide that
+// it has three slices lost 8e-5 of a sum to small terms.
 constexpr int kTnWide = 64;
 constexpr int kTnTile = 32;
 constexpr int kTnRows = 32;
 constexpr int kTnGeneralBlocks = 6;   // an SM
 
-template <typename T, typename H>   // dy, h and the results; dH
+template <typename T, typename H, bool FEW>   // dy, h and the results; dH; so few tokens that one chain holds them
 __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
 {
   constexpr int U = kTnRows * kTnWide / 256;
@@ -467,7 +469,7 @@ __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
       }
     }
   };
-  float c[4][2] = {};
+  float c[4][2] = {}, sum[4][2] = {};
   fetch(begin);
   for (int64_t mb = begin; mb < end; mb += kTnRows)
   {
@@ -500,6 +502,15 @@ __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
       c[3][0] = fmaf(p.w, q.x, c[3][0]);
       c[3][1] = fmaf(p.w, q.y, c[3][1]);
     }
+    if constexpr (!FEW)
+    {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+      {
+        sum[i >> 1][i & 1] += c[i >> 1][i & 1];
+        c[i >> 1][i & 1] = 0.0f;
+      }
+    }
     __syncthreads();
   }
   float *part = j.part + static_cast<int64_t>(blockIdx.z) * (static_cast<int64_t>(j.out) + j.in) * j.r +
@@ -512,19 +523,20 @@ __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
     {
       const int col = c0 + tp * 4 + a;
       const int rr = r0 + tq * 2 + b;
+      const float total = FEW ? c[a][b] : sum[a][b];
       if (col < wide && rr < j.r)
       {
         if (j.d_b == nullptr)
         {
-          part[static_cast<int64_t>(col) * j.r + rr] = c[a][b];
+          part[static_cast<int64_t>(col) * j.r + rr] = total;
         }
         else if (is_a)
         {
-          static_cast<T *>(j.d_a)[static_cast<int64_t>(rr) * j.in + col] = act_t<T>(c[a][b] * j.factor);
+          static_cast<T *>(j.d_a)[static_cast<int64_t>(rr) * j.in + col] = act_t<T>(total * j.factor);
         }
         else
         {
-          static_cast<T *>(j.d_b)[static_cast<int64_t>(col) * j.r + rr] = act_t<T>(c[a][b] * j.factor);
+          static_cast<T *>(j.d_b)[static_cast<int64_t>(col) * j.r + rr] = act_t<T>(total * j.factor);
         }
       }
     }
@@ -536,7 +548,7 @@ __global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t 
 {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  tn_general<T, H>(j, m);
+  tn_general<T, H, false>(j, m);
 }
 
 // bf16, ranks 8, 16, 32, 64, widths of whole 128-column tiles: the tensor core, as the adapter's reductions on full rows run it (both
@@ -1169,7 +1181,7 @@ act_tn_dx_kernel(const Gradients j, int64_t m, int tiles, const T *a, T *dx)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (static_cast<int>(blockIdx.x) < tiles)
   {
-    tn_general<T, float>(j, m);
+    tn_general<T, float, true>(j, m);
   }
   else if (blockIdx.y == 0)
   {

@@ -1,0 +1,49 @@
+"""Long sums of the operators around an adapted projection (caif_b200/csrc/act8.cu, lora_bank.cu) in fp32, where the order of the
+additions shows.
+
+In a sum of n products the longest chain of additions is at most n / 32 + 64 long, so it is off by at most that many times
+2^-24 times the sum of the products' magnitudes, and the result is stored in fp32: one more 2^-24, and one for alpha / rank.
+The terms here are one large one and small ones that a chain which already holds the large one loses whole (2^-25 or 2^-24
+beside 1, ties to even): a chain longer than the bound loses more than the bound.  Every product is a power of two, so that nothing but the additions
+rounds.
+"""
+import pytest
+import torch
+
+from caif_b200 import native as nv
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def bound(n):
+    return (n / 32 + 64 + 2) * U
+
+
+def zeros(in_dim, out_dim):
+    return nv.Weight(torch.zeros(out_dim, in_dim, dtype=torch.int8, device="cuda"), nv.I8, in_dim, out_dim,
+                     torch.ones(1, device="cuda"))
+
+
+def near(got, n, first, rest, terms):
+    """every element of `got` is the sum of `terms` terms, `first` and as often `rest`, within the bound"""
+    want = first + (terms - 1) * rest
+    assert float((got.double() - want).abs().max()) <= bound(n) * (abs(first) + (terms - 1) * abs(rest))
+
+
+# few slices of many tokens (wide layers), one slice, many slices
+@pytest.mark.parametrize("in_dim,out_dim,rank,m", [(4096, 4096, 64, 8192), (2048, 2048, 64, 8192), (7168, 7168, 40, 3001), (1024, 512, 16, 9000),
+                                                   (2048, 2048, 64, 64)])
+def test_gradients_over_many_tokens(in_dim, out_dim, rank, m):
+    """Token 0 gives 1 to every sum, the others 2^-25."""
+    dy = torch.full((m, out_dim), 2.0 ** -25, device="cuda")
+    dy[0] = 1.0
+    b = torch.zeros(out_dim, rank, device="cuda")
+    b[0] = 1.0                                         # dH[t, :] = dy[t, 0]
+    lora = nv.Lora(torch.zeros(rank, in_dim, device="cuda"), b, float(rank))
+    packed = nv.act_pack(torch.ones(m, in_dim, device="cuda"))
+    dx, d_a, d_b = nv.lora_linear_bwd_packed(zeros(in_dim, out_dim), lora, dy, packed, torch.ones(m, rank, device="cuda"))
+    near(d_b, m, 1.0, 2.0 ** -25, m)
+    near(d_a, m, 1.0, 2.0 ** -25, m)
+    assert not bool(dx.any())
