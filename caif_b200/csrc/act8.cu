@@ -1085,7 +1085,8 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
   }
 }
 
-// dx[m, in] = factor * dH . A, a thread a column of ROWS rows, which share A's numbers; `block` of ROWS rows' 256 columns
+// dx[m, in] = factor * dH . A, a thread a column of ROWS rows, which share A's numbers; `block` of ROWS rows' 256 columns.  64 products are
+// added up by themselves and then to those before (one chain over 1024 ranks lost 3e-5 of a sum to small terms).
 template <typename T, int ROWS>
 __device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, float factor, int64_t m, int in, int r, int64_t block)
 {
@@ -1093,7 +1094,7 @@ __device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, f
   const int parts = (in + 255) / 256;   // blocks of ROWS rows
   const int64_t at = block / parts * ROWS;
   const int c = static_cast<int>(block % parts) * 256 + static_cast<int>(threadIdx.x);
-  float s[ROWS] = {};
+  float s[ROWS] = {}, sum[ROWS] = {};
   for (int j0 = 0; j0 < r; j0 += 256)
   {
     const int n = r - j0 < 256 ? r - j0 : 256;
@@ -1125,25 +1126,34 @@ __device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, f
         }
       };
       const T *src = a + static_cast<int64_t>(j0) * in + c;
-      int k = 0;
-      for (; ROWS > 1 && k + 16 <= n; k += 16, src += static_cast<int64_t>(16) * in)
+      for (int k = 0; k < n;)
       {
-        T w[16];   // (all on their way before the first is used)
-#pragma unroll
-        for (int u = 0; u < 16; ++u)
+        const int stop = n - k < 64 ? n : k + 64;
+        for (; ROWS > 1 && k + 16 <= stop; k += 16, src += static_cast<int64_t>(16) * in)
         {
-          w[u] = src[static_cast<int64_t>(u) * in];
-        }
+          T w[16];   // (all on their way before the first is used)
 #pragma unroll
-        for (int u = 0; u < 16; ++u)
-        {
-          meet(k + u, act_f<T>(w[u]));
+          for (int u = 0; u < 16; ++u)
+          {
+            w[u] = src[static_cast<int64_t>(u) * in];
+          }
+#pragma unroll
+          for (int u = 0; u < 16; ++u)
+          {
+            meet(k + u, act_f<T>(w[u]));
+          }
         }
-      }
 #pragma unroll 8
-      for (; k < n; ++k, src += in)
-      {
-        meet(k, act_f<T>(*src));
+        for (; k < stop; ++k, src += in)
+        {
+          meet(k, act_f<T>(*src));
+        }
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q)
+        {
+          sum[q] += s[q];
+          s[q] = 0.0f;
+        }
       }
     }
   }
@@ -1152,7 +1162,7 @@ __device__ __forceinline__ void dx_general(const float *dh, const T *a, T *dx, f
   {
     if (c < in && at + q < m)
     {
-      dx[(at + q) * in + c] = act_t<T>(s[q] * factor);
+      dx[(at + q) * in + c] = act_t<T>(sum[q] * factor);
     }
   }
 }

@@ -47,3 +47,17 @@ def test_gradients_over_many_tokens(in_dim, out_dim, rank, m):
     near(d_b, m, 1.0, 2.0 ** -25, m)
     near(d_a, m, 1.0, 2.0 ** -25, m)
     assert not bool(dx.any())
+
+@pytest.mark.parametrize("in_dim,m", [(64, 20), (64, 100), (300, 700), (512, 2000)])
+def test_dx_of_a_large_rank(in_dim, m):
+    """The adapter's part of dx is a sum over 1024 ranks."""
+    rank, out_dim = 1024, 64
+    dy = torch.zeros(m, out_dim, device="cuda")
+    dy[:, 3] = 1.0
+    b = torch.zeros(out_dim, rank, device="cuda")
+    b[3] = 2.0 ** -25
+    b[3, 0] = 1.0                                      # dH[t, :] = 1, 2^-25, 2^-25, ...
+    lora = nv.Lora(torch.ones(rank, in_dim, device="cuda"), b, float(rank))
+    packed = nv.act_pack(torch.ones(m, in_dim, device="cuda"))
+    dx, _, _ = nv.lora_linear_bwd_packed(zeros(in_dim, out_dim), lora, dy, packed, torch.zeros(m, rank, device="cuda"))
+    near(dx, rank, 1.0, 2.0 ** -25, rank)
