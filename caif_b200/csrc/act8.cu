@@ -953,9 +953,14 @@ dh_row_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r)
     if (tid < width)
     {
       float v = 0.0f;
-      for (int i = 0; i < groups; ++i)
+      for (int g0 = 0; g0 < groups; g0 += 16)   // (up to 256 of them, for a rank of 1: sixteen at a time by themselves)
       {
-        v += sums[i * width + tid];
+        float some = 0.0f;
+        for (int i = g0; i < groups && i < g0 + 16; ++i)
+        {
+          some += sums[i * width + tid];
+        }
+        v += some;
       }
       dh[at * r + j0 + tid] = v;
     }
@@ -963,7 +968,8 @@ dh_row_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r)
 }
 
 // The same where B is large: a cluster four or eight rows, its blocks a share of the columns each; a number of B serves those rows, and
-// the blocks' sums are added in order.
+// the blocks' sums are added in order.  64 products of a row are added up by themselves and then to those before (one chain of every other
+// product of 14336 lost 2e-4 of a sum to small terms).
 constexpr int kDhPart = 512;
 
 template <typename T, int kDhRows>   // 4 or 8
@@ -985,7 +991,16 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
     const int groups = 256 / width;                  // rows of B at a time
     const int j = tid % width;
     const int group = tid / width;
-    float s[kDhRows][2] = {};
+    constexpr int CHAINS = 8 / kDhRows;   // of a row: eight in all, so that multiply-adds follow one another
+    float s[kDhRows][CHAINS] = {}, sum[kDhRows] = {};
+    auto gather = [&]() {
+#pragma unroll
+      for (int q = 0; q < kDhRows; ++q)
+      {
+        sum[q] += CHAINS == 2 ? s[q][0] + s[q][CHAINS - 1] : s[q][0];
+        s[q][0] = s[q][CHAINS - 1] = 0.0f;
+      }
+    };
     for (int c0 = begin; c0 < end; c0 += kDhPart)
     {
       const int n = end - c0 < kDhPart ? end - c0 : kDhPart;
@@ -1013,6 +1028,7 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
         int o = group;
         const T *src = b + static_cast<int64_t>(c0 + o) * r + j0 + j;
         const int64_t step = static_cast<int64_t>(groups) * r;
+        int trip = 0;
         for (; o + 15 * groups < n; o += 16 * groups, src += 16 * step)
         {
           T w[16];   // (all on their way before the first is used)
@@ -1024,20 +1040,25 @@ dh_kernel(const T *dy, const T *b, float *dh, int64_t m, int out, int r, int clu
 #pragma unroll
           for (int u = 0; u < 16; ++u)
           {
-            meet(o + u * groups, act_f<T>(w[u]), u & 1);
+            meet(o + u * groups, act_f<T>(w[u]), u % CHAINS);
+          }
+          if ((++trip & 3) == 0)
+          {
+            gather();
           }
         }
         for (; o < n; o += groups, src += step)
         {
           meet(o, act_f<T>(*src), 0);
         }
+        gather();
       }
     }
     __syncthreads();
 #pragma unroll
     for (int rr = 0; rr < kDhRows; ++rr)
     {
-      sums[rr][tid] = s[rr][0] + s[rr][1];
+      sums[rr][tid] = sum[rr];
     }
     __syncthreads();
     // a thread adds the groups of one row and column; in place, where its own first group lies

@@ -61,3 +61,24 @@ def test_dx_of_a_large_rank(in_dim, m):
     packed = nv.act_pack(torch.ones(m, in_dim, device="cuda"))
     dx, _, _ = nv.lora_linear_bwd_packed(zeros(in_dim, out_dim), lora, dy, packed, torch.zeros(m, rank, device="cuda"))
     near(dx, rank, 1.0, 2.0 ** -25, rank)
+
+
+# a block several rows and the whole of B; a cluster; a block a row
+@pytest.mark.parametrize("out_dim,rank,m,small", [(14336, 256, 4736, 2.0 ** -25), (14336, 300, 4800, 2.0 ** -25), (14336, 256, 200, 2.0 ** -25),
+                                                  (1024, 1, 5, 2.0 ** -24), (1000, 16, 40, 2.0 ** -24), (20000, 1, 300, 2.0 ** -24)])
+def test_hidden_gradient_of_a_wide_layer(out_dim, rank, m, small):
+    """dH = dy . B, seen through dA: token 1 alone is not zero."""
+    in_dim = 64
+    b = torch.full((out_dim, rank), small, device="cuda")
+    b[0] = 1.0
+    dy = torch.zeros(m, out_dim, device="cuda")
+    dy[1] = 1.0
+    lora = nv.Lora(torch.zeros(rank, in_dim, device="cuda"), b, float(rank))
+    packed = nv.act_pack(torch.ones(m, in_dim, device="cuda"))
+    _, d_a, _ = nv.lora_linear_bwd_packed(zeros(in_dim, out_dim), lora, dy, packed, torch.zeros(m, rank, device="cuda"))
+    near(d_a, out_dim, 1.0, small, out_dim)
+    # every 32nd value of it the large one: the partial sums of threads that share a sum
+    b[:] = small / 4
+    b[0] = 1.0
+    _, d_a, _ = nv.lora_linear_bwd_packed(zeros(in_dim, out_dim), lora, dy, packed, torch.zeros(m, rank, device="cuda"))
+    near(d_a, out_dim, 1.0, small / 4, out_dim)
