@@ -82,3 +82,17 @@ def test_hidden_gradient_of_a_wide_layer(out_dim, rank, m, small):
     b[0] = 1.0
     _, d_a, _ = nv.lora_linear_bwd_packed(zeros(in_dim, out_dim), lora, dy, packed, torch.zeros(m, rank, device="cuda"))
     near(d_a, out_dim, 1.0, small / 4, out_dim)
+
+
+@pytest.mark.parametrize("rank,out_dim,m", [(1024, 100, 3), (1024, 64, 200), (520, 33, 40)])
+def test_bank_of_a_large_rank(rank, out_dim, m):
+    """h . B^T is a sum over the ranks: four large terms, one for each of the threads that share a column."""
+    in_dim = 64
+    a = torch.full((rank, in_dim), 2.0 ** -24, device="cuda")
+    a[:4] = 1.0
+    bank = nv.LoraBank([nv.Lora(a, torch.ones(out_dim, rank, device="cuda"), float(rank))])
+    x = torch.zeros(m, in_dim, device="cuda")
+    x[:, 5] = 1.0
+    y = nv.lora_bank_linear_fwd(zeros(in_dim, out_dim), bank, torch.zeros(m, dtype=torch.int32, device="cuda"), x)
+    want = 4.0 + (rank - 4) * U
+    assert float((y.double() - want).abs().max()) <= bound(rank) * want
