@@ -397,6 +397,7 @@ struct Gradients
   const void *dy;          // [m, out]
   const void *h;           // [m, r]
   const void *dh;          // [m, r]
+  const void *dh_rest;     // in bf16: what its rounding left, as another bf16 number; null where dh is fp32
   const int8_t *x;         // [m, in]
   const uint8_t *scales;   // [m, ceil(in / 32)]
   float *part;
@@ -466,6 +467,10 @@ __device__ __forceinline__ void tn_general(const Gradients &j, int64_t m)
       if (row < end && rr < j.r)
       {
         v[i] = is_a ? act_f<H>(static_cast<const H *>(j.dh)[row * j.r + rr]) : act_f<T>(static_cast<const T *>(j.h)[row * j.r + rr]);
+        if constexpr (sizeof(H) == 2)
+        {
+          v[i] += is_a ? act_f<H>(static_cast<const H *>(j.dh_rest)[row * j.r + rr]) : 0.0f;
+        }
       }
     }
   };
@@ -554,7 +559,10 @@ __global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t 
 // bf16, ranks 8, 16, 32, 64, widths of whole 128-column tiles: the tensor core, as the adapter's reductions on full rows run it (both
 // operands have the token as their slow axis: tiles lie in shared memory as they come, fragments are read transposed).  A tile of
 // 64 tokens x 128 columns is 16 KB of dy, or 8 KB of codes, which become bf16 numbers on the way to shared memory: code * s has
-// seven bits of significand, so the products are those of the expanded rows.  Bound by HBM: dy and the codes once.
+// seven bits of significand, so the products are those of the expanded rows.  dH comes as two bf16 terms, whose products with the codes meet in
+// one sum (2^-16 of dH; as one term the error of dA is 2.4e-3 instead of 1.7e-3, and a caller of fp32 compute does not expect it; the second costs
+// 4 us of 227 at 4096 -> 4096, 8192 tokens, rank 16, and 26 of 260 at rank 64, where a third of the blocks' slices for dA alone got back 8 of
+// them and cost 3 of 131 at 14336 -> 4096, 1000 tokens).  Bound by HBM: dy and the codes once.
 constexpr int kTnColumns = 128;
 constexpr int kTnTokens = 64;
 constexpr int kTnPitch = kTnColumns + 8;   // bf16 elements: 272-byte rows keep the transposed reads free of conflicts
@@ -585,11 +593,15 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
 {
   constexpr int R = 8 * NT;
   __shared__ __align__(16) __nv_bfloat16 su[kTnTokens][kTnPitch];
-  __shared__ __align__(16) __nv_bfloat16 sv[kTnTokens][R + 8];
+  __shared__ __align__(16) __nv_bfloat16 sv[2][kTnTokens][R + 8];   // (h, or dH and what its rounding left)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x;
-  const int warp = tid >> 5;
+  // a warp 16 columns and all ranks, or, of large ranks, 32 columns and half of them, so that the thin operand crosses shared memory half as often
+  constexpr int WC = NT >= 4 ? 2 : 1;
+  constexpr int NW = NT / WC;
+  const int col_w = (tid >> 5) % (8 / WC) * WC * 16;
+  const int rank_w = (tid >> 5) / (8 / WC) * NW * 8;
   const int lane = tid & 31;
   const int g = lane >> 2;
   const int t = lane & 3;
@@ -601,17 +613,16 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
   const int64_t begin = per * blockIdx.y;
   const int64_t end = begin + per < m ? begin + per : m;
   const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(is_a ? j.dh : j.h);
-  float c[NT][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-  {
-    c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.0f;
-  }
+  const __nv_bfloat16 *v_rest = static_cast<const __nv_bfloat16 *>(j.dh_rest);
+  constexpr int THIN = kTnTokens * NT;             // 16-byte pieces of a tile of the thin operand
+  constexpr int RV = (2 * THIN + 255) / 256;
+  const int thin = is_a ? 2 * THIN : THIN;
+  float c[WC][NW][4] = {};
   // the next tile's loads are issued before this one's products: 16-byte pieces of dy (four a thread) or of codes (two, with
   // their scale bytes), and of the thin operand
   uint4 ru[4];
   uint32_t rs[2];
-  uint4 rv[2];
+  uint4 rv[RV];
   auto fetch = [&](int64_t mb) {
     if (is_a)
     {
@@ -645,13 +656,13 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < RV; ++i)
     {
       const int e = tid + i * 256;
       rv[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (e < kTnTokens * NT && mb + e / NT < end)
+      if (e < thin && mb + e % THIN / NT < end)
       {
-        rv[i] = *reinterpret_cast<const uint4 *>(v + (mb + e / NT) * R + (e % NT) * 8);
+        rv[i] = *reinterpret_cast<const uint4 *>((e < THIN ? v : v_rest) + (mb + e % THIN / NT) * R + (e % NT) * 8);
       }
     }
   };
@@ -684,12 +695,12 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < RV; ++i)
     {
       const int e = tid + i * 256;
-      if (e < kTnTokens * NT)
+      if (e < thin)
       {
-        *reinterpret_cast<uint4 *>(&sv[e / NT][(e % NT) * 8]) = rv[i];
+        *reinterpret_cast<uint4 *>(&sv[e / THIN][e % THIN / NT][(e % NT) * 8]) = rv[i];
       }
     }
     __syncthreads();
@@ -700,20 +711,35 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
 #pragma unroll
     for (int k16 = 0; k16 < kTnTokens / 16; ++k16)
     {
-      // rows of the product: this warp's 16 columns; lane l addresses row (l & 7) of 8 x 8 tile (l >> 3)
+      // rows of the product: this warp's columns, 16 at a time; lane l addresses row (l & 7) of 8 x 8 tile (l >> 3)
       const int tile = lane >> 3;
-      uint32_t a0, a1, a2, a3;
-      asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
-                   : "r"(smem_u32(&su[k16 * 16 + (tile >> 1) * 8 + (lane & 7)][warp * 16 + (tile & 1) * 8])));
+      uint32_t a[WC][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i < WC; ++i)
       {
-        uint32_t b0, b1;
-        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-                     : "=r"(b0), "=r"(b1)
-                     : "r"(smem_u32(&sv[k16 * 16 + (lane & 15)][nt * 8])));
-        tn_mma(c[nt], a0, a1, a2, a3, b0, b1);
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(a[i][0]), "=r"(a[i][1]), "=r"(a[i][2]), "=r"(a[i][3])
+                     : "r"(smem_u32(&su[k16 * 16 + (tile >> 1) * 8 + (lane & 7)][col_w + i * 16 + (tile & 1) * 8])));
+      }
+      auto multiply = [&](int plane) {
+#pragma unroll
+        for (int nt = 0; nt < NW; ++nt)
+        {
+          uint32_t b0, b1;
+          asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                       : "=r"(b0), "=r"(b1)
+                       : "r"(smem_u32(&sv[plane][k16 * 16 + (lane & 15)][rank_w + nt * 8])));
+#pragma unroll
+          for (int i = 0; i < WC; ++i)
+          {
+            tn_mma(c[i][nt], a[i][0], a[i][1], a[i][2], a[i][3], b0, b1);
+          }
+        }
+      };
+      multiply(0);
+      if (is_a)
+      {
+        multiply(1);
       }
     }
     __syncthreads();
@@ -721,14 +747,14 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
   float *part = j.part + static_cast<int64_t>(blockIdx.y) * (static_cast<int64_t>(j.out) + j.in) * R +
                 (is_a ? static_cast<int64_t>(j.out) * R : 0);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int i = 0; i < WC * NW; ++i)
   {
 #pragma unroll
     for (int half = 0; half < 2; ++half)
     {
-      const int64_t col = c0 + warp * 16 + g + 8 * half;
-      const int rr = nt * 8 + 2 * t;
-      const float lo = c[nt][2 * half], hi = c[nt][2 * half + 1];
+      const int64_t col = c0 + col_w + i / NW * 16 + g + 8 * half;
+      const int rr = rank_w + i % NW * 8 + 2 * t;
+      const float lo = c[i / NW][i % NW][2 * half], hi = c[i / NW][i % NW][2 * half + 1];
       if (j.d_b == nullptr)
       {
         *reinterpret_cast<float2 *>(part + col * R + rr) = make_float2(lo, hi);
@@ -749,13 +775,13 @@ __global__ void __launch_bounds__(256, kTnBlocks<NT>) act_tn_mma_kernel(const Gr
   }
 }
 
-// dH[m, r] = dy . B for the same adapters, with the transposed copy bt[r, out] of B: bf16, and times `mul` / *div, padded to 64 columns, as the
-// extra k-block of the product that gives dx.  A block takes 32 rows, so that bt crosses the SM's cache once for 32 rows and not once for
+// dH[m, r] = dy . B for the same adapters, with the transposed copy bt[r, out] of B: as two bf16 terms, and times `mul` / *div in bf16, padded to
+// 64 columns, as the extra k-block of the product that gives dx.  A block takes 32 rows, so that bt crosses the SM's cache once for 32 rows and not once for
 // 16 (8192 x 4096, rank 16: it is as many bytes as 16 rows of dy); eight warps split the columns, in 16-byte pieces straight into
 // fragments (the order of the columns inside a fragment is the same for both operands).
 template <int NT>
 __global__ void __launch_bounds__(256, NT <= 2 ? 3 : 2)
-act_nt_mma_kernel(const __nv_bfloat16 *dy, const __nv_bfloat16 *bt, __nv_bfloat16 *dh, __nv_bfloat16 *padded, float mul,
+act_nt_mma_kernel(const __nv_bfloat16 *dy, const __nv_bfloat16 *bt, __nv_bfloat16 *dh, __nv_bfloat16 *rest, __nv_bfloat16 *padded, float mul,
                   const float *div, int64_t m, int out)
 {
   constexpr int R = 8 * NT;
@@ -840,7 +866,9 @@ act_nt_mma_kernel(const __nv_bfloat16 *dy, const __nv_bfloat16 *bt, __nv_bfloat1
             sum.x += part[w][e >> 5][col];
             sum.y += part[w][e >> 5][col + 1];
           }
-          *reinterpret_cast<uint32_t *>(dh + row * R + col) = pack_bf16x2(sum.x, sum.y);
+          const uint32_t top = pack_bf16x2(sum.x, sum.y);
+          *reinterpret_cast<uint32_t *>(dh + row * R + col) = top;
+          *reinterpret_cast<uint32_t *>(rest + row * R + col) = rest_bf16x2(sum.x, sum.y, top);
           pad = pack_bf16x2(sum.x * factor, sum.y * factor);
         }
         *reinterpret_cast<uint32_t *>(padded + row * 64 + col) = pad;
@@ -1316,17 +1344,17 @@ int launch_gradients_dx(const GradientSums &j, int64_t sum_blocks, const float *
 }
 }  // namespace
 
-// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * dh^T . x, x packed; with dx (dh is fp32 then) dx[m, in] = factor * dh . a
+// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * (dh + dh_rest)^T . x, x packed, dh_rest for dh in bf16 alone; with dx (dh is fp32 then) dx[m, in] = factor * dh . a
 // too.  m >= 1; dy, h, a, d_b, d_a, dx in dtype
-int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
+int launch_act_gradients(const void *dy, const void *h, const void *dh, const void *dh_rest, int dh_dtype, const int8_t *x, const uint8_t *scales,
                          void *d_b, void *d_a, const void *a, void *dx, int dtype, float factor, float *scratch, int64_t m, int out,
                          int in, int r, cudaStream_t s)
 {
   auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   const bool tensor = dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
-                      (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(x);
+                      (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(dh_rest) && on_16(x);
   const bool direct = one_slice(tensor, m, out, in, r);
-  const Gradients j{dy, h, dh, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, dtype, dh_dtype, out, in, r};
+  const Gradients j{dy, h, dh, dh_rest, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, dtype, dh_dtype, out, in, r};
   int slices = 0;
   if (tensor)
   {
@@ -1382,16 +1410,16 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_d
   }
 }
 
-// dh[m, r] = dy . bt^T in bf16 and padded[m, 64] = bf16(dh * mul / *div): bf16 operands on 16-byte boundaries, r 8, 16, 32 or 64, out a
+// dh[m, r] = dy . bt^T in bf16, rest[m, r] what that rounding left, and padded[m, 64] = bf16(dh * mul / *div): bf16 operands on 16-byte boundaries, r 8, 16, 32 or 64, out a
 // multiple of 32, m >= 1
-int launch_act_nt(const void *dy, const void *bt, void *dh, void *padded, float mul, const float *div, int64_t m, int out, int r,
+int launch_act_nt(const void *dy, const void *bt, void *dh, void *rest, void *padded, float mul, const float *div, int64_t m, int out, int r,
                   cudaStream_t s)
 {
   auto kernel = r == 8 ? act_nt_mma_kernel<1>
                        : (r == 16 ? act_nt_mma_kernel<2> : (r == 32 ? act_nt_mma_kernel<4> : act_nt_mma_kernel<8>));
   CAIFQ_CHECK_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>((m + 31) / 32)), dim3(256), 0, s,
                                     static_cast<const __nv_bfloat16 *>(dy), static_cast<const __nv_bfloat16 *>(bt),
-                                    static_cast<__nv_bfloat16 *>(dh), static_cast<__nv_bfloat16 *>(padded), mul, div, m, out));
+                                    static_cast<__nv_bfloat16 *>(dh), static_cast<__nv_bfloat16 *>(rest), static_cast<__nv_bfloat16 *>(padded), mul, div, m, out));
   return CAIFQ_OK;
 }
 

@@ -141,10 +141,10 @@ int launch_lora_bank_frozen(const caifq_weight &w, const void *x, int dtype, int
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
 int launch_act_unpack(const int8_t *codes, const uint8_t *scales, void *x, int dtype, int64_t rows, int dim, cudaStream_t s);
 size_t act_gradients_scratch_bytes(int64_t m, int out, int in, int r);
-int launch_act_gradients(const void *dy, const void *h, const void *dh, int dh_dtype, const int8_t *x, const uint8_t *scales,
+int launch_act_gradients(const void *dy, const void *h, const void *dh, const void *dh_rest, int dh_dtype, const int8_t *x, const uint8_t *scales,
                          void *d_b, void *d_a, const void *a, void *dx, int dtype, float factor, float *scratch, int64_t m, int out,
                          int in, int r, cudaStream_t s);
-int launch_act_nt(const void *dy, const void *bt, void *dh, void *padded, float mul, const float *div, int64_t m, int out, int r,
+int launch_act_nt(const void *dy, const void *bt, void *dh, void *rest, void *padded, float mul, const float *div, int64_t m, int out, int r,
                   cudaStream_t s);
 int launch_dh(const void *dy, const void *b, float *dh, int dtype, int64_t m, int out, int r, cudaStream_t s);
 // layernorm.cu
@@ -169,7 +169,7 @@ int launch_lora_adamw(void *a, void *b, const void *d_a, const void *d_b, float 
                       float epsilon, float weight_decay, float bias_correction1, float bias_correction2,
                       cudaStream_t s);
 bool skinny_supported(int dtype, int rank, int k);
-int launch_skinny_nt(const void *x, const void *a, void *h, void *hs, float x_prescale, float hs_mul,
+int launch_skinny_nt(const void *x, const void *a, void *h, void *rest, void *hs, float x_prescale, float hs_mul,
                      const float *hs_div, int64_t m, int k, int rank, bool independent, cudaStream_t s);
 int launch_skinny_tn(const void *dy, const void *h, void *db, float prescale, int out, const void *x, const void *dh,
                      void *da, int in, float *sums, int64_t m, int rank, cudaStream_t s);
@@ -835,7 +835,7 @@ int lora_fwd_impl(const caifq_weight *w, const caifq_lora *lora, const void *x, 
                                   lora->rank, s);
     if (r == CAIFQ_OK)
     {
-      r = launch_skinny_nt(x, lora->a, hidden, base + ws.hs, 1.0f, scale, epilogue_scale_ptr(w), m, w->in_dim,
+      r = launch_skinny_nt(x, lora->a, hidden, nullptr, base + ws.hs, 1.0f, scale, epilogue_scale_ptr(w), m, w->in_dim,
                            lora->rank, true, s);
     }
     if (r != CAIFQ_OK)
@@ -950,7 +950,7 @@ int lora_bwd_impl(const caifq_weight *w, const caifq_lora *lora, const void *dy,
                                   expand ? n_b + n_a : n_b, lora->rank, s);
     if (r == CAIFQ_OK)
     {
-      r = launch_skinny_nt(dy, wbase + ws.bt, d_hidden, wbase + ws.dhs, scale, 1.0f, epilogue_scale_ptr(w), m,
+      r = launch_skinny_nt(dy, wbase + ws.bt, d_hidden, nullptr, wbase + ws.dhs, scale, 1.0f, epilogue_scale_ptr(w), m,
                            w->out_dim, lora->rank, false, s);
     }
     // dB[out, r] = (scale . dy)^T . hidden;  dA[r, in] = dH^T . x: one launch, or, where the scratch holds the sums of one
@@ -1350,20 +1350,21 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
   {
     const bool expand = packed_expand_ok(w, lora, dy, m, compute_dtype) && expansion_pays(w, true, m);
     void *wb = base + ws.weight;
-    // transposed B, padded A and, where the call expands, the weight in one launch; dH = dy . B, and its padded copy times
-    // alpha / rank for the product's extra k-block
+    void *rest = static_cast<char *>(d_hidden) + static_cast<size_t>(m) * lora->rank * 2;   // (what rounding left of dH, behind it)
+    // transposed B, padded A and, where the call expands, the weight in one launch; dH = dy . B as two bf16 terms for dA, and its padded copy
+    // times alpha / rank for the product's extra k-block, which has room for one: its rounding is at most 2^-8 of the adapter's part of dx
     int r = launch_expand_prepare(*w, expand ? wb : nullptr, lora->a, lora->b, nullptr, base + ws.lora.bt, base + ws.lora.ap,
                                   nullptr, 0, lora->rank, s);
     if (r == CAIFQ_OK)
     {
-      r = m > kActNtLeast ? launch_act_nt(dy, base + ws.lora.bt, d_hidden, base + ws.lora.dhs, scale, epilogue_scale_ptr(w), m, w->out_dim,
+      r = m > kActNtLeast ? launch_act_nt(dy, base + ws.lora.bt, d_hidden, rest, base + ws.lora.dhs, scale, epilogue_scale_ptr(w), m, w->out_dim,
                                           lora->rank, s)
-                          : launch_skinny_nt(dy, base + ws.lora.bt, d_hidden, base + ws.lora.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
+                          : launch_skinny_nt(dy, base + ws.lora.bt, d_hidden, rest, base + ws.lora.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
                                              w->out_dim, lora->rank, false, s);
     }
     if (r == CAIFQ_OK)
     {
-      r = launch_act_gradients(dy, hidden, d_hidden, sd, x_codes, x_scales, d_b, d_a, nullptr, nullptr, sd, scale, sums, m, w->out_dim,
+      r = launch_act_gradients(dy, hidden, d_hidden, rest, sd, x_codes, x_scales, d_b, d_a, nullptr, nullptr, sd, scale, sums, m, w->out_dim,
                                w->in_dim, lora->rank, s);
     }
     if (r != CAIFQ_OK)
@@ -1379,7 +1380,7 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
   int r = launch_dh(dy, lora->b, static_cast<float *>(d_hidden), sd, m, w->out_dim, lora->rank, s);
   if (r == CAIFQ_OK)
   {
-    r = launch_act_gradients(dy, hidden, d_hidden, CAIFQ_F32, x_codes, x_scales, d_b, d_a, lora->a, dx, sd, scale, sums, m, w->out_dim,
+    r = launch_act_gradients(dy, hidden, d_hidden, nullptr, CAIFQ_F32, x_codes, x_scales, d_b, d_a, lora->a, dx, sd, scale, sums, m, w->out_dim,
                              w->in_dim, lora->rank, s);
   }
   if (r != CAIFQ_OK)

@@ -156,7 +156,7 @@ __device__ __forceinline__ uint32_t scale2(uint32_t v, float s)
 template <int NT>  // NT = R / 8
 __global__ void __launch_bounds__(256)
 skinny_nt_kernel(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__restrict__ a,
-                 __nv_bfloat16 *__restrict__ h, __nv_bfloat16 *__restrict__ hs, float x_prescale, float hs_mul,
+                 __nv_bfloat16 *__restrict__ h, __nv_bfloat16 *__restrict__ rest, __nv_bfloat16 *__restrict__ hs, float x_prescale, float hs_mul,
                  const float *__restrict__ hs_div, int64_t m, int k, int cluster, int after)
 {
   // a CTA owns 16 rows; its 8 warps split K and add their partial tiles through shared memory
@@ -298,6 +298,10 @@ skinny_nt_kernel(const __nv_bfloat16 *__restrict__ x, const __nv_bfloat16 *__res
       }
       const uint32_t packed = pack2(v0, v1);
       *reinterpret_cast<uint32_t *>(h + row * R + col) = packed;
+      if (rest != nullptr)
+      {
+        *reinterpret_cast<uint32_t *>(rest + row * R + col) = rest_bf16x2(v0, v1, packed);
+      }
       if (hs != nullptr)
       {
         *reinterpret_cast<uint32_t *>(hs + row * 64 + col) = scale2(packed, mul);
@@ -563,7 +567,8 @@ bool skinny_supported(int dtype, int rank, int k)
   return dtype == CAIFQ_BF16 && (rank == 8 || rank == 16 || rank == 32 || rank == 64) && (k % 32) == 0;
 }
 
-int launch_skinny_nt(const void *x, const void *a, void *h, void *hs, float x_prescale, float hs_mul,
+// h = prescaled x . a^T in bf16; rest (or null): what that rounding left, in bf16; hs (or null): h padded and scaled
+int launch_skinny_nt(const void *x, const void *a, void *h, void *rest, void *hs, float x_prescale, float hs_mul,
                      const float *hs_div, int64_t m, int k, int rank, bool independent, cudaStream_t s)
 {
   if (m <= 0)
@@ -577,7 +582,7 @@ int launch_skinny_nt(const void *x, const void *a, void *h, void *hs, float x_pr
   {
     cluster *= 2;
   }
-  void (*kernel)(const __nv_bfloat16 *, const __nv_bfloat16 *, __nv_bfloat16 *, __nv_bfloat16 *, float, float,
+  void (*kernel)(const __nv_bfloat16 *, const __nv_bfloat16 *, __nv_bfloat16 *, __nv_bfloat16 *, __nv_bfloat16 *, float, float,
                  const float *, int64_t, int, int, int) = nullptr;
   switch (rank)
   {
@@ -612,7 +617,7 @@ int launch_skinny_nt(const void *x, const void *a, void *h, void *hs, float x_pr
   cfg.numAttrs = dependent_launches() ? 2 : 1;
   CAIFQ_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<const __nv_bfloat16 *>(x),
                                       static_cast<const __nv_bfloat16 *>(a), static_cast<__nv_bfloat16 *>(h),
-                                      static_cast<__nv_bfloat16 *>(hs), x_prescale, hs_mul, hs_div, m, k, cluster,
+                                      static_cast<__nv_bfloat16 *>(rest), static_cast<__nv_bfloat16 *>(hs), x_prescale, hs_mul, hs_div, m, k, cluster,
                                       independent ? 1 : 0));
   return CAIFQ_OK;
 }

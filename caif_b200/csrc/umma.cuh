@@ -301,6 +301,14 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi)
   return d;
 }
 
+// what the rounding of a pair to bf16, `top`, left of it, rounded to bf16 itself; nothing where the pair or its rounding is not finite
+__device__ __forceinline__ uint32_t rest_bf16x2(float lo, float hi, uint32_t top)
+{
+  const float r0 = lo - __uint_as_float(top << 16);
+  const float r1 = hi - __uint_as_float(top & 0xFFFF0000u);
+  return pack_bf16x2(isfinite(r0) ? r0 : 0.0f, isfinite(r1) ? r1 : 0.0f);
+}
+
 // four int8 codes (one 32-bit word, memory order) -> two bf16x2 registers, exact
 __device__ __forceinline__ void int8x4_to_bf16(uint32_t w, uint32_t &p01, uint32_t &p23)
 {

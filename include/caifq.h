@@ -409,7 +409,8 @@ CAIFQ_API int caifq_act_unpack(const int8_t *codes, const uint8_t *scales, void 
 /*
  * caifq_lora_linear_bwd_expanded for an adapter whose input was kept by caifq_act_pack: the same gradients, with dA taken
  * from the codes, which are never expanded in memory.  Sums over tokens run in a fixed order (equal calls give equal bits),
- * and alpha / rank multiplies fp32 sums instead of rounded copies of dy.  With m == 0 dA and dB are zeros.  dx may not overlap dy.
+ * and alpha / rank multiplies fp32 sums instead of rounded copies of dy.  dH = dy . B enters dA in fp32 or as two bf16 terms (2^-16);
+ * on the tensor core (bf16, rank 8, 16, 32 or 64, 32 rows or more) it enters dx as one.  With m == 0 dA and dB are zeros.  dx may not overlap dy.
  * in and out are at most 2^29.
  */
 CAIFQ_API size_t caifq_lora_bwd_packed_workspace_bytes(const caifq_weight *w, const caifq_lora *lora, int64_t m,

@@ -96,3 +96,35 @@ def test_bank_of_a_large_rank(rank, out_dim, m):
     y = nv.lora_bank_linear_fwd(zeros(in_dim, out_dim), bank, torch.zeros(m, dtype=torch.int32, device="cuda"), x)
     want = 4.0 + (rank - 4) * U
     assert float((y.double() - want).abs().max()) <= bound(rank) * want
+
+
+@pytest.mark.parametrize("storage,compute", [(nv.I8, nv.F32), (nv.I4, nv.BF16)])
+@pytest.mark.parametrize("in_dim,out_dim,m,rank", [(256, 384, 32, 16), (384, 256, 100, 8), (512, 128, 128, 64), (256, 640, 333, 16), (1024, 1024, 700, 32),
+                                                   (256, 1024, 2049, 8), (128, 1408, 3000, 16), (256, 896, 2500, 64), (256, 1024, 4097, 32)])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_gradient_of_a_has_the_whole_hidden_gradient(storage, compute, in_dim, out_dim, m, rank, aligned):
+    """bf16 rows: dH is a sum of eight whole numbers up to 127, which bf16 does not hold, and every sum is below 2^24: dA is exact but for
+    its own rounding."""
+    g = torch.Generator(device="cuda").manual_seed(m + rank)
+    if storage == nv.I8:
+        weight = zeros(in_dim, out_dim)
+    else:
+        weight = nv.Weight(torch.zeros(out_dim * in_dim // 2, dtype=torch.uint8, device="cuda"), nv.I4, in_dim, out_dim,
+                           torch.ones(out_dim * in_dim // 128, dtype=torch.float16, device="cuda"))
+    b = torch.randint(-127, 128, (out_dim, rank), generator=g, device="cuda").bfloat16()
+    lora = nv.Lora(torch.zeros(rank, in_dim, dtype=torch.bfloat16, device="cuda"), b, float(rank))
+    dy = torch.zeros(m, out_dim, dtype=torch.bfloat16, device="cuda")
+    at = torch.rand(m, out_dim, generator=g, device="cuda").topk(8, dim=1).indices
+    dy.scatter_(1, at, (torch.randint(0, 2, (m, 8), generator=g, device="cuda") * 2 - 1).bfloat16())
+    x = torch.randint(-3, 4, (m, in_dim), generator=g, device="cuda").bfloat16()
+    packed = nv.act_pack(x)
+    hidden = torch.randint(-3, 4, (m, rank), generator=g, device="cuda").bfloat16()
+    if not aligned:
+        flat = torch.empty(hidden.numel() + 1, dtype=torch.bfloat16, device="cuda")
+        flat[1:] = hidden.view(-1)
+        hidden = flat[1:].view(m, rank)
+    dx, d_a, d_b = nv.lora_linear_bwd_packed(weight, lora, dy, packed, hidden, compute)
+    dh = dy.double() @ b.double()
+    assert torch.equal(d_a, (dh.t() @ x.double()).bfloat16())
+    assert torch.equal(d_b, (dy.double().t() @ hidden.double()).bfloat16())
+    assert not bool(dx.any())
