@@ -404,8 +404,6 @@ struct Gradients
   void *d_b;               // with one slice: the results themselves, rounded here; else null
   void *d_a;
   float factor;
-  int dtype;               // of dy, h and the results
-  int dh_dtype;
   int out, in, r;
 };
 
@@ -1354,7 +1352,7 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, const vo
   const bool tensor = dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
                       (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(dh_rest) && on_16(x);
   const bool direct = one_slice(tensor, m, out, in, r);
-  const Gradients j{dy, h, dh, dh_rest, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, dtype, dh_dtype, out, in, r};
+  const Gradients j{dy, h, dh, dh_rest, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, out, in, r};
   int slices = 0;
   if (tensor)
   {

@@ -1272,9 +1272,12 @@ namespace
 {
 struct PackedBwdWs
 {
-  LoraBwdWs lora;
-  size_t weight;   // the expanded weight, where there is one
-  size_t sums;     // fp32, of the reductions over tokens
+  size_t d_hidden;  // [m, r] in fp32, or twice in bf16
+  size_t bt;        // [r, out] bf16: this and the next three where the tensor core may take the call
+  size_t dhs;       // [m, 64] bf16
+  size_t ap;        // [64, in] bf16
+  size_t weight;    // the expanded weight, where there is one
+  size_t sums;      // fp32, of the reductions over tokens
   size_t total;
 };
 
@@ -1294,8 +1297,14 @@ bool packed_expand_ok(const caifq_weight *w, const caifq_lora *l, const void *ac
 PackedBwdWs packed_bwd_ws(const caifq_weight *w, const caifq_lora *l, int64_t m, int compute_dtype)
 {
   PackedBwdWs o{};
-  o.lora = lora_bwd_ws(w, l, m);
-  o.weight = o.lora.total;
+  const size_t rank = static_cast<size_t>(l->rank);
+  const size_t rows = static_cast<size_t>(m);
+  const bool fused = fused_lora_ok(w, l, kAlignedProbe, m, compute_dtype);
+  o.d_hidden = 0;
+  o.bt = align256(rows * rank * 4);
+  o.dhs = o.bt + (fused ? align256(rank * w->out_dim * 2) : 0);
+  o.ap = o.dhs + (fused ? align256(rows * 64 * 2) : 0);
+  o.weight = o.ap + (fused ? align256(static_cast<size_t>(64) * w->in_dim * 2) : 0);
   o.sums = o.weight + (packed_expand_ok(w, l, kAlignedProbe, m, compute_dtype) ? expanded_weight_bytes(w) : 0);
   o.total = o.sums + align256(act_gradients_scratch_bytes(m, w->out_dim, w->in_dim, l->rank));
   return o;
@@ -1344,7 +1353,7 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
                   "%s: dx and dy overlap", who);
   const float scale = lora->alpha / static_cast<float>(lora->rank);
   char *base = static_cast<char *>(workspace);
-  void *d_hidden = base + ws.lora.d_hidden;
+  void *d_hidden = base + ws.d_hidden;
   float *sums = reinterpret_cast<float *>(base + ws.sums);
   if (fused_lora_ok(w, lora, dy, m, compute_dtype) && aligned_to(dx, 16))
   {
@@ -1353,13 +1362,13 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
     void *rest = static_cast<char *>(d_hidden) + static_cast<size_t>(m) * lora->rank * 2;   // (what rounding left of dH, behind it)
     // transposed B, padded A and, where the call expands, the weight in one launch; dH = dy . B as two bf16 terms for dA, and its padded copy
     // times alpha / rank for the product's extra k-block, which has room for one: its rounding is at most 2^-8 of the adapter's part of dx
-    int r = launch_expand_prepare(*w, expand ? wb : nullptr, lora->a, lora->b, nullptr, base + ws.lora.bt, base + ws.lora.ap,
+    int r = launch_expand_prepare(*w, expand ? wb : nullptr, lora->a, lora->b, nullptr, base + ws.bt, base + ws.ap,
                                   nullptr, 0, lora->rank, s);
     if (r == CAIFQ_OK)
     {
-      r = m > kActNtLeast ? launch_act_nt(dy, base + ws.lora.bt, d_hidden, rest, base + ws.lora.dhs, scale, epilogue_scale_ptr(w), m, w->out_dim,
+      r = m > kActNtLeast ? launch_act_nt(dy, base + ws.bt, d_hidden, rest, base + ws.dhs, scale, epilogue_scale_ptr(w), m, w->out_dim,
                                           lora->rank, s)
-                          : launch_skinny_nt(dy, base + ws.lora.bt, d_hidden, rest, base + ws.lora.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
+                          : launch_skinny_nt(dy, base + ws.bt, d_hidden, rest, base + ws.dhs, 1.0f, scale, epilogue_scale_ptr(w), m,
                                              w->out_dim, lora->rank, false, s);
     }
     if (r == CAIFQ_OK)
@@ -1372,8 +1381,8 @@ int caifq_lora_linear_bwd_packed(const caifq_weight *w, const caifq_lora *lora, 
       return r;
     }
     const caifq_weight wbf = float_weight(wb, CAIFQ_BF16, w->out_dim, w->in_dim);
-    return linear_any(expand ? &wbf : w, true, dy, sd, 1.0f, m, dx, sd, false, compute_dtype, s, who, base + ws.lora.dhs,
-                      base + ws.lora.ap, expand ? epilogue_scale_ptr(w) : nullptr);
+    return linear_any(expand ? &wbf : w, true, dy, sd, 1.0f, m, dx, sd, false, compute_dtype, s, who, base + ws.dhs,
+                      base + ws.ap, expand ? epilogue_scale_ptr(w) : nullptr);
   }
   // dH = dy . B stays in fp32, and with it the adapter's products: both gradients, then dx = (scale dH) . A and the frozen base on
   // top.  (dx in 16 bits is rounded after each of the two, as in the backward pass on full rows: the product adds onto what y holds)
