@@ -399,7 +399,7 @@ CAIFQ_API int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora
  * dtype).  codes int8 [rows, dim]; scales uint8 [rows, ceil(dim / 32)]: one byte for 32 columns of a row, the last block
  * shorter where dim is not a multiple.  The byte b stands for the scale s = 2^(b - 127), the smallest power of two, at least
  * 2^-126, with max|x| <= 127 s over the block; codes are x / s rounded to the nearest integer, ties to even, and
- * |x - code * s| <= s / 2 <= max|x| / 126.  A block that holds an infinity or NaN has b = 255 and codes of 0 and stands for
+ * |x - code * s| <= s / 2; s / 2 < max|x| / 127 unless s is the least scale, 2^-126.  A block that holds an infinity or NaN has b = 255 and codes of 0 and stands for
  * NaN throughout.  code * s is exact in F32 and BF16 (F16 results round, and overflow where the value does).
  */
 CAIFQ_API int caifq_act_pack(const void *x, int32_t dtype, int8_t *codes, uint8_t *scales, int64_t rows, int32_t dim,

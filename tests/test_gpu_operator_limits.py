@@ -40,3 +40,23 @@ def test_layernorm_of_the_most_rows():
     assert float(y[-1]) == 7.0
     for i in range(0, rows, step):
         assert not bool(out[i:min(rows, i + step)].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 45])
+def test_pack_error_down_to_the_least_scale(dtype, dim):
+    """Half a step of error everywhere; less than a 127th of the block's largest value above the least scale, and at it as much as that value."""
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    tops = torch.tensor([2.0 ** e for e in (-133, -128, -127, -126, -121, -120, -119, -100, 0, 100, 127)], device="cuda", dtype=torch.float64)
+    x = (torch.rand(len(tops), dim, generator=g, device="cuda", dtype=torch.float64) * 2 - 1) * tops[:, None]
+    x[:, 3::32] = tops[:, None]
+    x = x.to(dtype)
+    p = nv.act_pack(x)
+    s = torch.exp2(p.scales.double() - 127).repeat_interleave(32, 1)[:, :dim]
+    error = (x.double() - p.codes.double() * s).abs()
+    assert bool((error <= s / 2).all()) and bool((p.scales >= 1).all())
+    assert torch.equal(p.scales.min(1).values == 1, tops <= 127 * 2.0 ** -126) and torch.equal(p.scales.max(1).values == 1, tops <= 127 * 2.0 ** -126)
+    above = tops > 127 * 2.0 ** -126
+    assert bool((s[above] / 2 < tops[above][:, None] / 127).all())
+    lost = p.codes[tops == 2.0 ** -127]
+    assert not bool(lost.any()) and float(error[tops == 2.0 ** -127].max()) == 2.0 ** -127
