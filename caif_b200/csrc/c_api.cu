@@ -135,7 +135,7 @@ int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of
                           const void *y, void *scratch, cudaStream_t s);
 int launch_lora_bank_up(const caifq_lora_bank &bank, const int32_t *adapter_of_row, const void *x, const float *frozen, int64_t m,
                         void *y, void *scratch, cudaStream_t s);
-bool lora_bank_frozen_supported(const caifq_weight &w, const void *x, int64_t m);
+bool lora_bank_frozen_supported(const caifq_weight &w, const void *x, int dtype, int64_t m);
 int launch_lora_bank_frozen(const caifq_weight &w, const void *x, int dtype, int64_t m, float *frozen, cudaStream_t s);
 // act8.cu
 int launch_act_pack(const void *x, int dtype, int8_t *codes, uint8_t *scales, int64_t rows, int dim, cudaStream_t s);
@@ -1235,7 +1235,7 @@ int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *ban
   int r = launch_lora_bank_down(*bank, adapter_of_row, x, frozen, m, y, workspace, s);
   if (r == CAIFQ_OK)
   {
-    const bool own = compute_dtype == CAIFQ_F32 && forced_path() == Force::None && lora_bank_frozen_supported(*w, x, m) &&
+    const bool own = compute_dtype == CAIFQ_F32 && forced_path() == Force::None && lora_bank_frozen_supported(*w, x, bank->dtype, m) &&
                      any_cell_only(w, x, bank->dtype, m, frozen);
     r = own ? launch_lora_bank_frozen(*w, x, bank->dtype, m, frozen, s)
             : linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who, true);

@@ -1160,10 +1160,26 @@ int launch_lora_bank_down(const caifq_lora_bank &bank, const int32_t *adapter_of
 }
 
 // frozen[m, out] = x . W^T in fp32 by bank_frozen_kernel, where it takes the call: int8 with one scale or none, int4 with groups of eights,
-// rows of x on 16-byte boundaries, few of them
-bool lora_bank_frozen_supported(const caifq_weight &w, const void *x, int64_t m)
+// rows of x on 16-byte boundaries, few of them.
+// It reads the codes once for eight rows, the kernel for any cell once for 64 but by blocks of 64 x 64 that leave SMs idle where there are few:
+// the time of one goes with eights of rows x columns, that of the other with its waves of two blocks an SM.  Whole call, own kernel and any
+// cell, us:                        rows 32          64          96          128
+//   fp32  1408 -> 1776 int4     28 / 179    52 / 183    76 / 183   101 / 185
+//         2048 -> 4104 int4     81 / 259   153 / 265   221 / 269   294 / 271
+//         4096 -> 14344 int4   472 / 631   917 / 642  1362 / 1294 1806 / 1313
+//         4096 -> 14344 int8   283 / 474   671 / 490   894 / 969  1353 / 992
+//   bf16  1408 -> 14344 int4   149 / 217   290 / 222   432 / 442   573 / 447
+//         4096 -> 14344 int4   293 / 618   573 / 627   860 / 1272 1141 / 1281
+//         4096 -> 14344 int8   250 / 459   510 / 465   756 / 958  1004 / 960
+//   fp16  4096 -> 14344 int8   225 / 467   508 / 481   760 / 978   911 / 991
+//         2048 -> 4104 int8     41 / 168    77 / 172   112 / 176   147 / 178
+bool lora_bank_frozen_supported(const caifq_weight &w, const void *x, int dtype, int64_t m)
 {
-  return m <= 128 && (w.in_dim % 8) == 0 && on_16(x) && (reinterpret_cast<uintptr_t>(w.codes) & 3u) == 0 &&
+  const int64_t out = w.out_dim;
+  const int64_t waves = ((out + 63) / 64 * ((m + 63) / 64) + 2 * 148 - 1) / (2 * 148);
+  const int64_t most = (dtype == CAIFQ_F32 ? 60000 : 90000) * waves;
+  return m <= 128 && (m + kFrozenRows - 1) / kFrozenRows * out <= most && (w.in_dim % 8) == 0 && on_16(x) &&
+         (reinterpret_cast<uintptr_t>(w.codes) & 3u) == 0 &&
          ((w.storage == CAIFQ_I8 && (w.scales == nullptr || w.scheme == CAIFQ_PER_TENSOR)) ||
           (w.storage == CAIFQ_I4 && w.scales != nullptr && w.group_size > 0 && (w.group_size % 8) == 0));
 }

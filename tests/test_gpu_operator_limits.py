@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from caif_b200 import native as nv
+from gpu_util import kernels_of
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +61,29 @@ def test_pack_error_down_to_the_least_scale(dtype, dim):
     assert bool((s[above] / 2 < tops[above][:, None] / 127).all())
     lost = p.codes[tops == 2.0 ** -127]
     assert not bool(lost.any()) and float(error[tops == 2.0 ** -127].max()) == 2.0 ** -127
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("storage", [nv.I8, nv.I4])
+@pytest.mark.parametrize("out_dim,m,few_32,few_16", [(14344, 32, True, True), (14344, 48, False, True), (14344, 64, False, False), (14344, 128, False, False),
+                                                     (4104, 96, True, True), (1776, 128, True, True), (60008, 8, True, True), (60008, 33, False, True),
+                                                     (60008, 64, False, False)])
+def test_bank_takes_the_product_of_odd_widths_by_its_size(out_dim, m, few_32, few_16, storage, dtype):
+    """Few rows of few columns by the kernel that reads the codes once for eight rows, others by the one for any cell: the same sums."""
+    in_dim = 136
+    few = few_32 if dtype == torch.float32 else few_16
+    g = torch.Generator(device="cuda").manual_seed(out_dim + m)
+    if storage == nv.I8:
+        codes = torch.randint(-127, 128, (out_dim, in_dim), generator=g, device="cuda", dtype=torch.int8)
+        weight = nv.Weight(codes, nv.I8, in_dim, out_dim, torch.full((1,), 0.25, device="cuda"))
+    else:
+        codes = torch.randint(0, 256, (out_dim * in_dim // 2,), generator=g, device="cuda", dtype=torch.uint8)
+        weight = nv.Weight(codes, nv.I4, in_dim, out_dim, torch.full((out_dim * in_dim // 8,), 0.25, device="cuda", dtype=torch.float16), 0, 8)
+    bank = nv.LoraBank([nv.Lora(torch.zeros(8, in_dim, device="cuda", dtype=dtype), torch.zeros(out_dim, 8, device="cuda", dtype=dtype), 8.0)])
+    x = torch.randint(-2, 3, (m, in_dim), generator=g, device="cuda").to(dtype)     # (whole numbers: sums without rounding)
+    rows = torch.zeros(m, dtype=torch.int32, device="cuda")
+    got = []
+    names = [n for n, _ in kernels_of(lambda: got.append(nv.lora_bank_linear_fwd(weight, bank, rows, x)))]
+    assert any("bank_frozen_kernel" in n for n in names) == few and any("linear_generic" in n for n in names) == (not few)
+    want = x.double() @ nv.weight_materialize(weight).double().t()
+    assert torch.equal(got[0], want.to(dtype))
