@@ -128,3 +128,19 @@ def test_gradient_of_a_has_the_whole_hidden_gradient(storage, compute, in_dim, o
     assert torch.equal(d_a, (dh.t() @ x.double()).bfloat16())
     assert torch.equal(d_b, (dy.double().t() @ hidden.double()).bfloat16())
     assert not bool(dx.any())
+
+
+# (slices: the blocks or clusters that walk over the rows, and the slices of rows of the form for any width)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,dim,slices", [(3000, 4096, 148), (3000, 12288, 74), (3000, 20480, 32), (3000, 40000, 16), (5000, 33003, 16), (4000, 70000, 62),
+                                             (9000, 9001, 72)])
+def test_layernorm_gradients_over_many_wide_rows(rows, dim, slices, dtype):
+    """A column's sum is a chain of rows / slices and the slices' sums, 32 of them side by side: row 0 gives 1, the others 2^-25."""
+    dy = torch.full((rows, dim), 2.0 ** -25, dtype=dtype, device="cuda")
+    dy[0] = 1.0
+    x = torch.ones(rows, dim, dtype=dtype, device="cuda")
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    _, d_gamma, d_beta = nv.layernorm_bwd(dy, x, mean, rstd)
+    want = 1.0 + (rows - 1) * 2.0 ** -25
+    for got in (d_gamma, d_beta):
+        assert float((got.double() - want).abs().max()) <= (rows / slices + slices / 32 + 16) * U * want
