@@ -1237,6 +1237,10 @@ int caifq_lora_bank_linear_fwd(const caifq_weight *w, const caifq_lora_bank *ban
   {
     const bool own = compute_dtype == CAIFQ_F32 && forced_path() == Force::None && lora_bank_frozen_supported(*w, x, bank->dtype, m) &&
                      any_cell_only(w, x, bank->dtype, m, frozen);
+    if (own)
+    {
+      set_path("decode");
+    }
     r = own ? launch_lora_bank_frozen(*w, x, bank->dtype, m, frozen, s)
             : linear_ws(w, false, x, bank->dtype, m, frozen, CAIFQ_F32, compute_dtype, base + ws.weight, ws.total - ws.weight, s, who, true);
   }

@@ -243,7 +243,7 @@ CAIFQ_API int caifq_linear_fwd_multi(const caifq_weight *ws, int32_t num_weights
                                      int64_t m, void *y, int32_t y_dtype, int32_t compute_dtype, void *stream);
 
 /* Name of the kernel family the last caifq_linear_fwd / caifq_linear_dx call
- * on this thread chose ("decode", "umma", "generic"); for tests and reports.
+ * on this thread, or the frozen product of a call around one, chose ("decode", "umma", "generic"); for tests and reports.
  * Calls for a run of experts report "umma-grouped" for launches over all of them,
  * whichever kernel these were (experts of few rows: the few-token or the streaming one). */
 CAIFQ_API const char *caifq_last_path(void);

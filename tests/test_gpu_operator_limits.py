@@ -3,7 +3,6 @@ import pytest
 import torch
 
 from caif_b200 import native as nv
-from gpu_util import kernels_of
 
 pytestmark = pytest.mark.gpu
 
@@ -82,8 +81,10 @@ def test_bank_takes_the_product_of_odd_widths_by_its_size(out_dim, m, few_32, fe
     bank = nv.LoraBank([nv.Lora(torch.zeros(8, in_dim, device="cuda", dtype=dtype), torch.zeros(out_dim, 8, device="cuda", dtype=dtype), 8.0)])
     x = torch.randint(-2, 3, (m, in_dim), generator=g, device="cuda").to(dtype)     # (whole numbers: sums without rounding)
     rows = torch.zeros(m, dtype=torch.int32, device="cuda")
-    got = []
-    names = [n for n, _ in kernels_of(lambda: got.append(nv.lora_bank_linear_fwd(weight, bank, rows, x)))]
-    assert any("bank_frozen_kernel" in n for n in names) == few and any("linear_generic" in n for n in names) == (not few)
+    other = nv.Weight(torch.zeros(128, 128, dtype=torch.int8, device="cuda"), nv.I8, 128, 128, torch.ones(1, device="cuda"))
+    nv.linear_fwd(other, torch.zeros(200, 128, dtype=torch.bfloat16, device="cuda"))
+    assert nv.last_path() == "umma"
+    got = nv.lora_bank_linear_fwd(weight, bank, rows, x)
+    assert nv.last_path() == ("decode" if few else "generic")
     want = x.double() @ nv.weight_materialize(weight).double().t()
-    assert torch.equal(got[0], want.to(dtype))
+    assert torch.equal(got, want.to(dtype))
