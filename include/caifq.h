@@ -358,6 +358,11 @@ CAIFQ_API int caifq_lora_linear_bwd_noalloc(const caifq_weight *w, const caifq_l
  * once.  (Under bf16 compute code times scale of an int4 weight is rounded to bf16 first; where a tensor-core kernel converts the
  * codes itself on more than 768 rows the scale is too.)
  *
+ * Speed: the tensor core takes banks whose adapters ALL have bf16 factors on 16-byte boundaries and ranks of 8, 16, ... 64 (`vectors`), with
+ * widths of whole 32s in and whole 8s out and, above 128 rows, at most 4096 adapters.  One adapter of another rank sends every row of its bank
+ * to fp32 multiply-adds (4096 -> 4096, 24 adapters, 2300 rows: 89 us, and 595 with one of rank 72): pad ranks below 64 with zeros
+ * and scale alpha with the rank, and serve larger ones by calls of their own rows.
+ *
  * A bank is a table of `count` (up to 2^24) entries in device memory.  caifq_lora_bank_entries checks the factors (all of bank->dtype;
  * ranks 1 to 1024, not necessarily equal; A [rank, in], B [out, rank], in at most 2^29, out at most 65535 * 64), fills the table's image in HOST memory and every
  * field of *bank but `entries`; the caller copies the image to the device and sets bank->entries to it.  It needs no GPU.
@@ -384,9 +389,10 @@ typedef struct caifq_lora_bank
 
 CAIFQ_API int caifq_lora_bank_entries(const caifq_lora *loras, int32_t count, int32_t in_dim, int32_t out_dim,
                                       caifq_lora_entry *entries_host, caifq_lora_bank *bank);
-/* Scratch of the call below (x . A^T, the frozen product where y has 16 bits, and, for many tokens, the weight expanded as by
- * caifq_linear_fwd_ws): 256-byte aligned,
- * at least this large; nothing in it outlives the call.  Calls that may overlap on the GPU need workspaces of their own. */
+/* Scratch of the call below: 4 max_rank bytes a row (rounded up to sixteens of an adapter's rows) for x . A^T, 4 bytes for every element of y
+ * where y has 16 bits (the frozen product in fp32: 0.94 GB for 16384 rows of 14336 columns; split a longer call by rows), and, for many
+ * tokens, the weight expanded as by caifq_linear_fwd_ws.  256-byte aligned, at least this large; nothing in it outlives the call.
+ * Calls that may overlap on the GPU need workspaces of their own. */
 CAIFQ_API size_t caifq_lora_bank_workspace_bytes(const caifq_weight *w, const caifq_lora_bank *bank, int64_t m,
                                                  int32_t compute_dtype);
 /* x [m, in], y [m, out] in bank->dtype, not overlapping; adapter_of_row int32 [m], device memory. */
@@ -410,8 +416,10 @@ CAIFQ_API int caifq_act_unpack(const int8_t *codes, const uint8_t *scales, void 
  * caifq_lora_linear_bwd_expanded for an adapter whose input was kept by caifq_act_pack: the same gradients, with dA taken
  * from the codes, which are never expanded in memory.  Sums over tokens run in a fixed order (equal calls give equal bits),
  * and alpha / rank multiplies fp32 sums instead of rounded copies of dy.  dH = dy . B enters dA in fp32 or as two bf16 terms (2^-16);
- * on the tensor core (bf16, rank 8, 16, 32 or 64, 32 rows or more) it enters dx as one.  With m == 0 dA and dB are zeros.  dx may not overlap dy.
- * in and out are at most 2^29.
+ * on the tensor core (bf16, rank 8, 16, 32 or 64, 32 rows or more) it enters dx as one.  With m == 0 dA and dB are zeros.  Results overlap neither
+ * operands nor one another (dx and dy: refused).  in and out are at most 2^29.  bf16 adapters of rank 8, 16, 32 or 64 on widths of whole 128s
+ * run on the tensor core from 32 rows on; others take fp32 multiply-adds and add the frozen base onto dx in dx's type, which then is
+ * rounded twice.
  */
 CAIFQ_API size_t caifq_lora_bwd_packed_workspace_bytes(const caifq_weight *w, const caifq_lora *lora, int64_t m,
                                                        int32_t compute_dtype);
