@@ -1261,12 +1261,9 @@ int64_t general_tiles(int out, int in, int r)
 }
 
 // So few tokens make one slice, whose sums are rounded where they are made, a launch less.  The whole pass, tensor core: 4096 -> 4096 int8,
-// 64 rows 37.6 -> 35.4 us, 128 rows 39.0 -> 37.3, 200 rows 38.9 and 39.4 so.  Multiply-adds, fp32, where the tiles are many: 2048 -> 2048,
-// rank 64, 64 rows 37.1 -> 35.1, 128 rows the same; 1024 -> 1024, rank 16, 40 rows 18.5 and 18.6 so, 64 rows 19.7 and 20.5.
-bool one_slice(bool tensor, int64_t m, int out, int in, int r)
-{
-  return tensor ? m <= 128 : m <= (general_tiles(out, in, r) >= 64 ? 64 : 32);
-}
+// 64 rows 35.9 -> 33.4 us, 128 rows 36.7 -> 34.7, 200 rows 36.5 and 36.2 so.  Multiply-adds (one chain of a sum: 64 tokens at most), fp32: 2048 ->
+// 2048, rank 64, 64 rows 35.6 -> 31.7; 1024 -> 1024, rank 16, 33 rows 20.5 -> 18.6, 64 rows 21.3 -> 20.5; 256 -> 256, rank 8, 17.5 and 17.7, 18.1 and 18.2.
+bool one_slice(bool tensor, int64_t m) { return m <= (tensor ? 128 : 64); }
 
 }  // namespace
 
@@ -1351,7 +1348,7 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, const vo
   auto on_16 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
   const bool tensor = dtype == CAIFQ_BF16 && dh_dtype == CAIFQ_BF16 && (r == 8 || r == 16 || r == 32 || r == 64) && (out % kTnColumns) == 0 &&
                       (in % kTnColumns) == 0 && on_16(dy) && on_16(h) && on_16(dh) && on_16(dh_rest) && on_16(x);
-  const bool direct = one_slice(tensor, m, out, in, r);
+  const bool direct = one_slice(tensor, m);
   const Gradients j{dy, h, dh, dh_rest, x, scales, scratch, direct ? d_b : nullptr, direct ? d_a : nullptr, factor, out, in, r};
   int slices = 0;
   if (tensor)

@@ -1286,8 +1286,8 @@ struct PackedBwdWs
 };
 
 // More rows than this take dH = dy . B by 32 rows a block, fewer the kernel of 16 rows, whose blocks are twice as many.  The whole backward
-// pass, 4096 -> 4096 int8, rank 16: 1024 rows 59.4 us by 32 and 54.6 by 16, 2048 rows 82.4 and 79.0, 3000 rows 106 and 108; at 8192 rows the
-// launch alone takes 17 and 26.
+// pass, 4096 -> 4096 int8, rank 16: 1024 rows 57.7 us by 32 and 53.3 by 16, 2048 rows 82.2 and 78.3, 3000 rows 107.6 and 110.0, 8192 rows 234.8 and
+// 237.8.
 constexpr int64_t kActNtLeast = 2048;
 
 // whether the weight may be expanded once for the call: as expand_ok, from 32 rows on (whole pass, rank 16, 32 to 127 rows: 4096 -> 14336 int4
