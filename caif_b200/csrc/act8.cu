@@ -409,8 +409,8 @@ struct Gradients
 
 // any type and width: 64 x 32 tiles of the result, fp32 multiply-adds, eight a thread for six values from shared memory.  The next
 // tokens' loads are issued before this trip's products.  (32 x 32 tiles with four for four: 500 rows, 2048 columns each way, rank 64, 37 us instead of 23)
-// A trip's 32 products are added up by themselves and then to the trips before (64 tokens or fewer: one chain): with one chain over a slice, 8192 tokens of a layer so wide that
-// it has three slices lost 8e-5 of a sum to small terms.
+// A trip's 32 products are added up by themselves and then to the trips before (64 tokens or fewer: one chain): with one chain over a slice,
+// 8192 tokens of a layer so wide that it has three slices lost 8e-5 of a sum to small terms.
 constexpr int kTnWide = 64;
 constexpr int kTnTile = 32;
 constexpr int kTnRows = 32;
@@ -558,9 +558,9 @@ __global__ void __launch_bounds__(256) act_tn_kernel(const Gradients j, int64_t 
 // operands have the token as their slow axis: tiles lie in shared memory as they come, fragments are read transposed).  A tile of
 // 64 tokens x 128 columns is 16 KB of dy, or 8 KB of codes, which become bf16 numbers on the way to shared memory: code * s has
 // seven bits of significand, so the products are those of the expanded rows.  dH comes as two bf16 terms, whose products with the codes meet in
-// one sum (2^-16 of dH; as one term the error of dA is 2.4e-3 instead of 1.7e-3, and a caller of fp32 compute does not expect it; the second costs
-// 4 us of 227 at 4096 -> 4096, 8192 tokens, rank 16, and 26 of 260 at rank 64, where a third of the blocks' slices for dA alone got back 8 of
-// them and cost 3 of 131 at 14336 -> 4096, 1000 tokens).  Bound by HBM: dy and the codes once.
+// one sum (2^-16 of dH; as one term the error of dA is 2.4e-3 instead of 1.7e-3, and a caller of fp32 compute does not expect it; the second
+// costs 4 us of 227 at 4096 -> 4096, 8192 tokens, rank 16, and 26 of 260 at rank 64.  More slices for dA than for dB got back 8 of these, and
+// cost 3 of 131 at 14336 -> 4096, 1000 tokens, rank 16).  Bound by HBM: dy and the codes once.
 constexpr int kTnColumns = 128;
 constexpr int kTnTokens = 64;
 constexpr int kTnPitch = kTnColumns + 8;   // bf16 elements: 272-byte rows keep the transposed reads free of conflicts
@@ -1339,8 +1339,8 @@ int launch_gradients_dx(const GradientSums &j, int64_t sum_blocks, const float *
 }
 }  // namespace
 
-// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * (dh + dh_rest)^T . x, x packed, dh_rest for dh in bf16 alone; with dx (dh is fp32 then) dx[m, in] = factor * dh . a
-// too.  m >= 1; dy, h, a, d_b, d_a, dx in dtype
+// d_b[out, r] = factor * dy^T . h and d_a[r, in] = factor * (dh + dh_rest)^T . x, x packed, dh_rest for dh in bf16 alone; with dx (dh is fp32
+// then) dx[m, in] = factor * dh . a too.  m >= 1; dy, h, a, d_b, d_a, dx in dtype
 int launch_act_gradients(const void *dy, const void *h, const void *dh, const void *dh_rest, int dh_dtype, const int8_t *x, const uint8_t *scales,
                          void *d_b, void *d_a, const void *a, void *dx, int dtype, float factor, float *scratch, int64_t m, int out,
                          int in, int r, cudaStream_t s)
@@ -1405,7 +1405,8 @@ int launch_act_gradients(const void *dy, const void *h, const void *dh, const vo
   }
 }
 
-// dh[m, r] = dy . bt^T in bf16, rest[m, r] what that rounding left, and padded[m, 64] = bf16(dh * mul / *div): bf16 operands on 16-byte boundaries, r 8, 16, 32 or 64, out a
+// dh[m, r] = dy . bt^T in bf16, rest[m, r] what that rounding left, and padded[m, 64] = bf16(dh * mul / *div): bf16 operands on 16-byte
+// boundaries, r 8, 16, 32 or 64, out a
 // multiple of 32, m >= 1
 int launch_act_nt(const void *dy, const void *bt, void *dh, void *rest, void *padded, float mul, const float *div, int64_t m, int out, int r,
                   cudaStream_t s)
